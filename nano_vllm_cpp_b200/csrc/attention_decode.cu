@@ -58,6 +58,11 @@ struct DecArgs {
   const int* row_entry;
   const int* positions;
   const int* rows;        // which batch rows to process (null: all, row = blockIdx.x)
+  // REST kernels: a row is read from the page on that holds position first[row] (its keys before are another kernel's); the
+  // results are partial ones, whatever the number of splits, and slots 0 .. splits - 1 of the `slots` that part_o and part_ml
+  // hold for a (row, head)
+  const int* first;
+  int slots;
   void* out;
   float* part_o;          // [rows, Hq, splits, D]
   float* part_ml;         // [rows, Hq, splits, 2]
@@ -188,7 +193,7 @@ __device__ __forceinline__ void merge_when_last(const DecArgs& a, int r, int t, 
 }
 
 // CPL: chunks of 8 elements per lane (D <= 64 * CPL); GB: query heads per block.
-template <typename TC, int CPL, int GB>
+template <typename TC, int CPL, int GB, bool REST>
 __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecArgs a) {
   extern __shared__ __align__(128) uint8_t dec_smem[];
   __shared__ __align__(16) float q_s[GB][256];           // (read four floats at a time)
@@ -210,10 +215,10 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
   const int D = a.D, chunks = D / 8;
 
   const int n = a.positions[t] + 1;
-  const int lo = first_visible(n - 1, a.window, a.chunk);
+  const int lo = REST ? a.first[r] / a.page * a.page : first_visible(n - 1, a.window, a.chunk);
   // this split's pages
   const int p_lo = lo / a.page, p_hi = (n - 1) / a.page + 1;
-  const int per = (p_hi - p_lo + a.splits - 1) / a.splits;
+  const int per = ((REST ? max(0, p_hi - p_lo) : p_hi - p_lo) + a.splits - 1) / a.splits;
   const int pb = p_lo + split * per;
   const int n_pages = max(0, min(p_hi, pb + per) - pb);
   const uint32_t chunk_bytes = (uint32_t)a.page * D * sizeof(TC);
@@ -391,11 +396,11 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
       o = fmaf(mrg_o[w][g][d], sc, o);
     }
     const int h = kvh * G + g0 + g;
-    if (a.splits == 1) {
+    if (!REST && a.splits == 1) {
       if (a.has_sink) ll += __expf(a.sink - mm);
       st_dt(a.out, a.out_dt, ((size_t)t * a.Hq + h) * D + d, ll > 0.f ? o / ll * head_gate_of(a.gate, t, h) : 0.f);
     } else {
-      const size_t pi = ((size_t)r * a.Hq + h) * a.splits + split;
+      const size_t pi = ((size_t)r * a.Hq + h) * (REST ? a.slots : a.splits) + split;
       a.part_o[pi * D + d] = o;
       if (d == 0) {
         a.part_ml[pi * 2] = mm;
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
       }
     }
   }
-  if (a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, D, (float*)dec_smem);
+  if (!REST && a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, D, (float*)dec_smem);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -442,7 +447,7 @@ constexpr int TC_ROWS = 16;      // query heads per block (rows of the MMA)
 // D: head dimension rounded up to a multiple of 64 (compile time: it sizes the fragments); a.D: the head's own elements.
 // MOD 1: scores pass a cap and a bias by distance; they are then in base-2 units (and a.scale is 1).  MOD 2: the same with a
 // cap whose tangent is tanhf's (capped_log2 is off by some 2^-22 of the cap, however small the score).
-template <int D, int TERMS, int MOD>
+template <int D, int TERMS, int MOD, bool REST>
 __global__ void __launch_bounds__((WARPS + 1) * 32, D <= 128 ? 3 : 1)
 attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            DecArgs a) {
@@ -465,23 +470,23 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   const int n = a.positions[t] + 1;
-  const int lo = first_visible(n - 1, a.window, a.chunk);
+  const int lo = REST ? a.first[r] / a.page * a.page : first_visible(n - 1, a.window, a.chunk);
   const int p_lo = lo / a.page, p_hi = (n - 1) / a.page + 1;
-  const int pages = p_hi - p_lo;
+  const int pages = REST ? max(0, p_hi - p_lo) : p_hi - p_lo;
   int per = (pages + a.splits - 1) / a.splits;
   if ((pages + a.long_pages - 1) / a.long_pages >= a.many_shares) per = max(per, a.long_pages);
   else if (per < a.short_pages) per = a.mid_pages;
   const int pb = p_lo + split * per;
   const int n_pages = max(0, min(p_hi, pb + per) - pb);
-  if (n_pages == 0 && a.splits > 1) {                // nothing for this split: say so and leave
+  if (n_pages == 0 && (REST || a.splits > 1)) {      // nothing for this split: say so and leave
     grid_dep_wait();
     grid_dep_launch();
     for (int i = threadIdx.x; i < ng * a.D; i += (WARPS + 1) * 32) {
-      const size_t pi = ((size_t)r * a.Hq + kvh * G + g0 + i / a.D) * a.splits + split;
+      const size_t pi = ((size_t)r * a.Hq + kvh * G + g0 + i / a.D) * (REST ? a.slots : a.splits) + split;
       a.part_o[pi * a.D + i % a.D] = 0.f;
       if (i % a.D == 0) { a.part_ml[pi * 2] = -1e30f; a.part_ml[pi * 2 + 1] = 0.f; }
     }
-    if (a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
+    if (!REST && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
     return;
   }
   const uint32_t box_bytes = (uint32_t)a.page * 128;           // one box: `page` keys x 64 elements
@@ -657,6 +662,15 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
             o[i2][0] *= al_lo; o[i2][1] *= al_lo; o[i2][2] *= al_hi; o[i2][3] *= al_hi;
           }
         }
+        // What lies behind the row's position in its newest page may be anything, infinities of an earlier holder too, and a weight
+        // of zero would not keep them out of the sums.  (The values are this warp's, and no load follows them.)
+        if (REST && j0 + 15 >= n) {
+          for (int x = lane; x < (j0 + 16 - n) * (D / 8); x += 32) {
+            const int key = kb * 16 + (n - j0) + x / (D / 8), c = x % (D / 8);
+            *(uint4*)(dec_smem + (vbase - smem0) + (c / 8) * box_bytes + key * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+        }
         // TERMS = 3: the float32 weights are split into three bfloat16 terms (hi, the rest, the rest of the rest:
         // all 24 bits), and each term is multiplied with the values into the same accumulators
         uint32_t pa[TERMS][4];
@@ -739,11 +753,11 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
       ov = fmaf(mrg_o[((size_t)w * ng + gg) * D + d], sc, ov);
     }
     const int h = kvh * G + g0 + gg;
-    if (a.splits == 1) {
+    if (!REST && a.splits == 1) {
       if (a.has_sink) ll += exp2f(a.sink * 1.4426950408889634f - mms);
       st_dt(a.out, a.out_dt, ((size_t)t * a.Hq + h) * a.D + d, ll > 0.f ? ov / ll * head_gate_of(a.gate, t, h) : 0.f);
     } else {
-      const size_t pi = ((size_t)r * a.Hq + h) * a.splits + split;
+      const size_t pi = ((size_t)r * a.Hq + h) * (REST ? a.slots : a.splits) + split;
       a.part_o[pi * a.D + d] = ov;
       if (d == 0) {                                             // the merge kernel works in natural-log units
         a.part_ml[pi * 2] = mm == -INFINITY ? -1e30f : mms * 0.6931471805599453f;
@@ -751,7 +765,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
       }
     }
   }
-  if (a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
+  if (!REST && a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
 }
 
 // Combines the splits of one (row, head) in split order.
@@ -782,26 +796,27 @@ __global__ void attention_decode_merge_kernel(const float* __restrict__ part_o, 
     st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, split_sum(part_o + pi * D + d, w_s, splits, D));
 }
 
-template <typename TC, int CPL, int GB>
+template <typename TC, int CPL, int GB, bool REST>
 int launch_decode_g(const DecArgs& a, int R, int G, size_t smem, cudaStream_t s) {
   static bool attr_done = false;
   if (!attr_done) {
-    cudaError_t e = cudaFuncSetAttribute(attention_decode_kernel<TC, CPL, GB>,
+    cudaError_t e = cudaFuncSetAttribute(attention_decode_kernel<TC, CPL, GB, REST>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != cudaSuccess) return (int)e;
     attr_done = true;
   }
   dim3 grid(R, a.Hkv * ((G + GB - 1) / GB), a.splits);
-  NV_RETURN_IF(launch_dep(attention_decode_kernel<TC, CPL, GB>, grid, dim3((WARPS + 1) * 32), smem, s, a));
+  NV_RETURN_IF(launch_dep(attention_decode_kernel<TC, CPL, GB, REST>, grid, dim3((WARPS + 1) * 32), smem, s, a));
   NV_RETURN_LAST();
 }
 
 template <typename TC, int CPL>
 int launch_decode(const DecArgs& a, int R, int G, size_t smem, cudaStream_t s) {
-  return G == 1 ? launch_decode_g<TC, CPL, 1>(a, R, G, smem, s) : launch_decode_g<TC, CPL, 4>(a, R, G, smem, s);
+  if (a.first) return G == 1 ? launch_decode_g<TC, CPL, 1, true>(a, R, G, smem, s) : launch_decode_g<TC, CPL, 4, true>(a, R, G, smem, s);
+  return G == 1 ? launch_decode_g<TC, CPL, 1, false>(a, R, G, smem, s) : launch_decode_g<TC, CPL, 4, false>(a, R, G, smem, s);
 }
 
-template <int D, int TERMS, int MOD>
+template <int D, int TERMS, int MOD, bool REST>
 int launch_decode_tc(DecArgs a, int R, const void* kc, const void* vc, int num_pages, float scale, cudaStream_t s) {
   const int G = a.Hq / a.Hkv;
   CUtensorMap tm_k, tm_v;
@@ -816,26 +831,26 @@ int launch_decode_tc(DecArgs a, int R, const void* kc, const void* vc, int num_p
   const size_t smem = (ring > merge ? ring : merge) + 1024;
   static bool attr_done = false;
   if (!attr_done) {
-    cudaError_t e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          160 * 1024);
     if (e != cudaSuccess) return (int)e;
     // three CTAs with a 64 KB ring each need nearly all of a multiprocessor's shared memory
-    e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD>, cudaFuncAttributePreferredSharedMemoryCarveout,
+    e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, REST>, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return (int)e;
     attr_done = true;
   }
   dim3 grid(R, a.Hkv * ((G + TC_ROWS - 1) / TC_ROWS), a.splits);
-  NV_RETURN_IF(launch_dep(attention_decode_tc_kernel<D, TERMS, MOD>, grid, dim3((WARPS + 1) * 32), smem, s, tm_k, tm_v, a));
+  NV_RETURN_IF(launch_dep(attention_decode_tc_kernel<D, TERMS, MOD, REST>, grid, dim3((WARPS + 1) * 32), smem, s, tm_k, tm_v, a));
   NV_RETURN_LAST();
 }
 
-template <int TERMS, int MOD>
+template <int TERMS, int MOD, bool REST = false>
 int launch_decode_tc_d(const DecArgs& a, int DT, int R, const void* kc, const void* vc, int num_pages, float scale, cudaStream_t s) {
-  return DT == 64 ? launch_decode_tc<64, TERMS, MOD>(a, R, kc, vc, num_pages, scale, s)
-       : DT == 128 ? launch_decode_tc<128, TERMS, MOD>(a, R, kc, vc, num_pages, scale, s)
-       : DT == 192 ? launch_decode_tc<192, TERMS, MOD>(a, R, kc, vc, num_pages, scale, s)
-                   : launch_decode_tc<256, TERMS, MOD>(a, R, kc, vc, num_pages, scale, s);
+  return DT == 64 ? launch_decode_tc<64, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
+       : DT == 128 ? launch_decode_tc<128, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
+       : DT == 192 ? launch_decode_tc<192, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
+                   : launch_decode_tc<256, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s);
 }
 
 // Stages of the page ring for a page of `page` keys of `D` elements of `esize` bytes: as many as fit in
@@ -900,13 +915,18 @@ NV_API int nv_attention_decode_splits_of(int rows, int Hq, int Hkv, int D, int m
 // arrays, the block table and every page but each row's newest one before that kernel has ended: the kernel
 // directly before it may write only the query rows and the newest page of each row (the engine's rotary kernel
 // over single rows does exactly that).
-NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
-                               const int* block_table, int max_blocks, const int* row_entry, const int* positions,
-                               const int* rows, int R, float scale, int window, void* out, int out_dt, int Hq,
-                               int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
-                               int* split_count, int split_count_len, int has_sink, float sink_score,
-                               int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
-                               const float* slopes, const float* bias_table, int bias_len, cudaStream_t stream) {
+//
+// first != nullptr ([R], positions): a row reads its keys from the start of that position's page on (none where that lies behind
+// its own position) and leaves partial results, slot 0 .. splits - 1 of the `slots` that scratch holds for a (row, head): [R, Hq, slots, D] sums and then
+// [R, Hq, slots, 2] pairs of maximum (natural units; -1e30: no key) and sum.  Sink and gate are then the joining kernel's.
+namespace {
+int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
+               const int* block_table, int max_blocks, const int* row_entry, const int* positions,
+               const int* rows, int R, float scale, int window, void* out, int out_dt, int Hq,
+               int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
+               int* split_count, int split_count_len, int has_sink, float sink_score,
+               int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
+               const float* slopes, const float* bias_table, int bias_len, const int* first, int slots, cudaStream_t stream) {
   // gate: head h's output of batch row t is multiplied by sigmoid(gate[t * gate_ld + h]) (nullptr: it is not); the
   // gates must have been written before the kernel that precedes this one on the stream.
   // softcap > 0: scaled scores are capped, s -> softcap * tanh(s / softcap).  chunk > 0: a row at position p sees the
@@ -924,14 +944,17 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
   if (((uintptr_t)kc & 15) || ((uintptr_t)vc & 15)) return NV_ERR_UNSUPPORTED;
   if (R == 0) return NV_OK;
   if (splits < 1) splits = 1;
-  if (splits > 1 && !scratch) return NV_ERR_BAD_SIZE;
+  if ((splits > 1 || first) && !scratch) return NV_ERR_BAD_SIZE;
+  if (!first) slots = splits;
+  if (slots < splits) return NV_ERR_BAD_SIZE;
   DecArgs a;
   a.qkv = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions;
   a.rows = rows; a.out = out; a.scale = scale; a.q_dt = q_dt; a.out_dt = out_dt; a.q_stride = q_stride;
   a.max_blocks = max_blocks; a.window = window; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.splits = splits;
   a.long_pages = 1; a.many_shares = 0x7fffffff; a.short_pages = a.mid_pages = 0;      // even shares
   a.part_o = scratch;
-  a.part_ml = scratch ? scratch + (size_t)R * Hq * splits * D : nullptr;
+  a.first = first; a.slots = slots;
+  a.part_ml = scratch ? scratch + (size_t)R * Hq * slots * D : nullptr;
   a.err = err;
   a.has_sink = has_sink; a.sink = sink_score;
   a.softcap = softcap > 0.f ? softcap : 0.f;
@@ -944,7 +967,7 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
   // then added up by the block that finishes last instead of by a second kernel.  For a few rows only: with many,
   // the last blocks' sums lengthen the kernel's tail by more than the second kernel's launch costs (measured per
   // decode step: batch 1 507 -> 511 tokens/s, batch 8 2,209 -> 2,212, batch 64 6,252 -> 6,192).
-  a.split_count = (split_count && (long long)R * Hq <= split_count_len && R * Hq <= 256) ? split_count : nullptr;
+  a.split_count = (split_count && !first && (long long)R * Hq <= split_count_len && R * Hq <= 256) ? split_count : nullptr;
   const int one_by_one = splits > MAX_SPLITS || ((uintptr_t)a.part_ml & 7) != 0;
   // ... and only while the last block's sum is short: its 160 threads add the block's outputs up one after the other, each
   // with loads from the second-level cache (one row of 4,096 keys, 28 heads of 128 on 4: 33 us so and 24 with the second kernel,
@@ -999,7 +1022,12 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
     // tensor-core form (a page of keys per warp); its blocks take up to 16 query heads of a kv head; with
     // float_weights or a sink the weights enter the product with the values as three bfloat16 terms
     const bool mod = a.softcap > 0.f || slopes || bias_table;
-    if (float_weights || has_sink)
+    if (first)                                     // (a cap by tanhf: one form for all of them)
+      rc = float_weights ? (mod ? launch_decode_tc_d<3, 2, true>(a, DT, R, kc, vc, num_pages, scale, stream)
+                                : launch_decode_tc_d<3, 0, true>(a, DT, R, kc, vc, num_pages, scale, stream))
+                         : (mod ? launch_decode_tc_d<1, 2, true>(a, DT, R, kc, vc, num_pages, scale, stream)
+                                : launch_decode_tc_d<1, 0, true>(a, DT, R, kc, vc, num_pages, scale, stream));
+    else if (float_weights || has_sink)
       rc = has_sink && a.softcap > 0.f ? launch_decode_tc_d<3, 2>(a, DT, R, kc, vc, num_pages, scale, stream)
            : mod ? launch_decode_tc_d<3, 1>(a, DT, R, kc, vc, num_pages, scale, stream)
                  : launch_decode_tc_d<3, 0>(a, DT, R, kc, vc, num_pages, scale, stream);
@@ -1017,12 +1045,36 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
                              : launch_decode<float, 4>(a, R, G, smem, stream));
   }
   if (rc) return rc;
-  if (splits > 1 && !a.split_count) {
+  if (splits > 1 && !a.split_count && !first) {
     dim3 grid(R, Hq);
     NV_RETURN_IF(launch_dep(attention_decode_merge_kernel, grid, dim3(128), 0, stream, (const float*)a.part_o,
                             (const float*)a.part_ml, rows, out, out_dt, Hq, D, splits, has_sink, sink_score, a.gate, one_by_one));
   }
   NV_RETURN_LAST();
+}
+}  // namespace
+
+NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
+                               const int* block_table, int max_blocks, const int* row_entry, const int* positions,
+                               const int* rows, int R, float scale, int window, void* out, int out_dt, int Hq,
+                               int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
+                               int* split_count, int split_count_len, int has_sink, float sink_score,
+                               int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
+                               const float* slopes, const float* bias_table, int bias_len, cudaStream_t stream) {
+  return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, window,
+                    out, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, split_count, split_count_len, has_sink,
+                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, stream);
+}
+
+// The keys from position first[r] on, as partial results (see decode_run): what attention over a shared prefix joins with it.
+int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
+                             const int* block_table, int max_blocks, const int* row_entry, const int* positions, const int* rows,
+                             const int* first, int R, float scale, int out_dt, int Hq, int Hkv, int D, int page, int num_pages,
+                             int splits, int slots, float* scratch, int* err, int float_weights, float softcap, cudaStream_t stream) {
+  if (!first) return NV_ERR_BAD_SIZE;
+  return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, 0,
+                    nullptr, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, nullptr, 0, 0, 0.f, float_weights, softcap,
+                    nullptr, 0, 0, nullptr, nullptr, 0, first, slots, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

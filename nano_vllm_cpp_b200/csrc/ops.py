@@ -223,6 +223,14 @@ def _cuda_contig(*ts) -> None:
         _need(t.is_contiguous(), "tensor is not contiguous")
 
 
+def _here(*ts) -> None:
+    """The kernels run on the current device: a tensor of another one is refused."""
+    at = torch.cuda.current_device()
+    for t in ts:
+        if t is not None:
+            _need(t.device.index == at, f"tensor is on {t.device}, the current device is {at}")
+
+
 def _i32(*ts) -> None:
     for t in ts:
         if t is not None:
@@ -442,6 +450,82 @@ def attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, s
                                  (0 if sink_score is None else 1), float(sink_score or 0.0),
                                  (1 if float_weights else 0), float(softcap), *_head_gates(gate, qkv.shape[0], Hq),
                                  *_score_bias(chunk, slopes, bias_table, Hq), _stream()), "attention_decode")
+
+
+class SharedPrefix:
+    """Which rows of a step share a prefix, for ``attention_decode_shared``: made once a step, read by all of its layers.
+
+    ``groups``: (rows, positions) pairs: the rows (places among the ``rows`` rows that the call takes) hold the same keys and
+    values at their first so many positions, each in pages of its own or in common ones; whole pages of them are read through
+    the block table of the first of them.  A row is in one group at most; the others read all their keys themselves."""
+
+    def __init__(self, groups, rows: int, device):
+        packed, self.members, self.longest = self.pack(groups, rows)
+        self.R, self.groups = rows, len(groups)
+        self.bind(torch.tensor(packed, dtype=torch.int32).to(device))
+
+    @staticmethod
+    def pack(groups, rows: int):
+        """The host's arrays in one list: per row its shared positions and its group (or -1), the groups' rows one after the
+        other (``rows`` places), where each group's start, and its positions; the number of grouped rows; the longest prefix."""
+        first, group, members, cu, lens = [0] * rows, [-1] * rows, [], [0], []
+        for g, (own, n) in enumerate(groups):
+            _need(len(own) > 0 and n >= 0, "SharedPrefix: a group has a row at least and no negative prefix")
+            for r in own:
+                _need(0 <= r < rows, f"SharedPrefix: row {r} is not among the {rows} rows")
+                _need(group[r] < 0, f"SharedPrefix: row {r} is named twice")
+                first[r], group[r] = int(n), g
+                members.append(int(r))
+            cu.append(len(members))
+            lens.append(int(n))
+        return first + group + members + [0] * (rows - len(members)) + cu + lens, len(members), max(lens, default=0)
+
+    def bind(self, buf) -> None:
+        R, G = self.R, self.groups
+        self.buf = buf
+        self.first, self.group, self.rows_of, self.cu, self.lens = (buf[a:b] for a, b in (
+            (0, R), (R, 2 * R), (2 * R, 3 * R), (3 * R, 3 * R + G + 1), (3 * R + G + 1, 3 * R + 2 * G + 1)))
+
+
+def attention_decode_shared_usable(k_cache, D: int) -> bool:
+    return bool(lib().nv_attention_shared_usable(D, k_cache.shape[2])) and attention_decode_usable(k_cache, D)
+
+
+def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, positions, scale: float, out, Hq: int, Hkv: int,
+                            D: int, max_context: int, shared: SharedPrefix, rows=None, err=None, sink_score=None,
+                            float_weights: bool = False, softcap: float = 0.0, gate=None) -> None:
+    """``attention_decode`` for rows of which some share a prefix (``shared``): a group's shared keys and values are read once
+    for all its rows, as one product of their query heads, and joined with what each row has of its own.  A row sees the
+    positions up to its own, none of them masked otherwise (layers with a window, chunks or biases by distance take
+    ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``,
+    ``gate``: see there.  As there, the kernel in front may write the query rows and each row's newest page, nothing else that
+    is read here."""
+    _cuda_contig(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
+    _i32(block_table, row_entry, positions, rows)
+    _here(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
+    T = qkv.shape[0]
+    R = T if rows is None else rows.numel()
+    page = k_cache.shape[2]
+    _need(Hq > 0 and Hkv > 0 and Hq % Hkv == 0, "attention_decode_shared: query heads are a multiple of kv heads")
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == Hkv and k_cache.shape[3] == D,
+          "attention_decode_shared: keys and values are [pages, kv heads, slots, head size]")
+    _need(qkv.dtype == k_cache.dtype == v_cache.dtype == out.dtype, "attention_decode_shared: queries, cache and result have one type")
+    _need(qkv.dim() == 2 and qkv.shape[1] >= Hq * D and out.shape == (T, Hq * D) and positions.numel() == T and row_entry.numel() == T,
+          "attention_decode_shared: shapes")
+    _need(shared.R == R, f"attention_decode_shared: {R} rows, and shared prefixes for {shared.R}")
+    _need(scale > 0 and softcap >= 0, "attention_decode_shared: the scale is positive, a cap is not negative")
+    _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
+    L = lib()
+    splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, max_context, num_sms())
+    ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, shared.longest)
+    scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
+    _check(L.nv_attention_decode_shared(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table),
+                                        block_table.shape[1], _p(row_entry), _p(positions), _p(rows), R, _p(shared.first),
+                                        _p(shared.group), _p(shared.rows_of), shared.members, _p(shared.cu), _p(shared.lens),
+                                        shared.groups, scale, _p(out), dt(out), Hq, Hkv, D, page, k_cache.shape[0], splits, ours,
+                                        _p(scratch), _p(err.t if err is not None else _global_err().t),
+                                        (0 if sink_score is None else 1), float(sink_score or 0.0), (1 if float_weights else 0),
+                                        float(softcap), *_head_gates(gate, T, Hq), _stream()), "attention_decode_shared")
 
 
 def _score_bias(chunk: int, slopes, table, Hq: int):
@@ -954,6 +1038,85 @@ def sample_nucleus(logits, params, recent, recent_off, out) -> None:
     work = torch.empty_like(logits)
     _check(lib().nv_sample_nucleus(_p(logits), _p(work), R, V, _p(params), _p(recent), _p(recent_off),
                                    _p(out), _stream()), "sample_nucleus")
+
+
+class PageArrays:
+    """The arrays of a cache whose pages ``copy_pages`` copies together, described once: tensors ``[pages, heads, slots,
+    elements]`` (keys, values), or ``[places, elements]`` (state slots: one head, one slot).  All have as many pages; heads,
+    elements and types may differ, slots not."""
+
+    def __init__(self, tensors):
+        _need(len(tensors) > 0, "PageArrays: at least one array")
+        self.tensors = list(tensors)
+        words, pages, slots = [], {t.shape[0] for t in self.tensors}, set()
+        _need(len(pages) == 1, "PageArrays: the arrays have different numbers of pages")
+        self.page_bytes = 0
+        for t in self.tensors:
+            _cuda_contig(t)
+            _need(t.dim() in (2, 4) and t.numel() > 0, "PageArrays: arrays are [pages, heads, slots, elements] or [places, elements]")
+            _need(t.device == self.tensors[0].device, "PageArrays: the arrays are on one device")
+            heads, n, elements = t.shape[1:] if t.dim() == 4 else (1, 1, t.shape[1])
+            slot = elements * t.element_size()
+            unit = next((u for u in (16, 8, 4, 2) if slot % u == 0 and t.data_ptr() % u == 0), 0)
+            _need(unit > 0, "PageArrays: a slot's bytes are even")
+            words += [t.data_ptr(), heads * n * slot, heads, n * slot, slot, n, t.shape[0], unit]
+            slots.add(n)
+            self.page_bytes = max(self.page_bytes, heads * n * slot)
+        _need(len(slots) == 1, "PageArrays: the arrays' pages have different numbers of slots")
+        self.pages, self.slots = pages.pop(), slots.pop()
+        self.table = torch.tensor(words, dtype=torch.int64).to(self.tensors[0].device)
+
+
+def copy_pages(arrays: PageArrays, src, dst, slots=None, err=None) -> None:
+    """``a[dst[i], :, :slots[i]] = a[src[i], :, :slots[i]]`` for every copy i and every array of ``arrays``, in one launch
+    (int32 on the device; ``slots`` None: whole pages).  What lies behind the slots stays as it was.  The destinations are
+    distinct and none of them is a source of another copy.  A page that the arrays do not have is not copied and sets the
+    error flag."""
+    _cuda_contig(src, dst, slots)
+    _i32(src, dst, slots)
+    _here(arrays.table, src, dst, slots)
+    N = src.numel()
+    _need(dst.numel() == N and (slots is None or slots.numel() == N), "copy_pages: a source, a destination and slots per copy")
+    for at in range(0, N, 32768):               # (a grid has so many rows of blocks)
+        n = min(32768, N - at)
+        _check(lib().nv_copy_pages(_p(arrays.table), len(arrays.tensors), arrays.page_bytes, _p(src[at:at + n]), _p(dst[at:at + n]),
+                                   None if slots is None else _p(slots[at:at + n]), n,
+                                   _p(err.t if err is not None else _global_err().t), _stream()), "copy_pages")
+
+
+def max_top_logprobs() -> int:
+    return int(lib().nv_token_logprobs_max_top())
+
+
+def token_logprobs(logits, tokens, logprob, *, entropy=None, rank=None, top_ids=None, top_logprobs=None, err=None) -> None:
+    """Per row of ``logits`` [R, V] (float32 or bfloat16, rows of unit stride any distance apart): the log probability of
+    ``tokens[r]`` under the row's softmax, into ``logprob`` [R]; the distribution's ``entropy`` [R] in nats; the token's ``rank`` [R],
+    how many ids come before it in the order of (logit descending, id ascending); the first K ids of that order and their log
+    probabilities, ``top_ids`` and ``top_logprobs`` [R, K] (at most ``max_top_logprobs()``).  ``tokens`` and ``logprob`` may be None
+    for the rest alone.  Log probabilities and entropies are float32, ids and ranks int32.  Masked logits (minus infinity) have no part in
+    the softmax; a row with a NaN, with plus infinity or with nothing above minus infinity has NaN for its numbers.  A
+    token outside the vocabulary sets the error flag and gets NaN and the rank -1."""
+    _need(logits.is_cuda and logits.dim() == 2 and logits.shape[1] > 0, "token_logprobs: logits [rows, vocabulary] on a CUDA device")
+    R, V = logits.shape
+    _need(V == 1 or logits.stride(1) == 1, "token_logprobs: a row's logits are one after the other")
+    stride = logits.stride(0) if R > 1 else V
+    _need(stride >= V, "token_logprobs: rows overlap")
+    _cuda_contig(tokens, logprob, entropy, rank, top_ids, top_logprobs)
+    _i32(tokens, rank, top_ids)
+    _f32(logprob, entropy, top_logprobs)
+    _here(logits, tokens, logprob, entropy, rank, top_ids, top_logprobs)
+    _need(tokens is not None or (logprob is None and rank is None), "token_logprobs: log probabilities and ranks are of tokens")
+    for t in (tokens, logprob, entropy, rank):
+        _need(t is None or t.numel() == R, "token_logprobs: one entry per row")
+    K = 0
+    _need((top_ids is None) == (top_logprobs is None), "token_logprobs: the alternatives' ids and log probabilities go together")
+    if top_ids is not None:
+        _need(top_ids.dim() == 2 and top_ids.shape[0] == R and top_ids.shape == top_logprobs.shape, "token_logprobs: alternatives are [rows, K]")
+        K = top_ids.shape[1]
+        _need(K <= min(V, max_top_logprobs()), f"token_logprobs: at most {min(V, max_top_logprobs())} alternatives, found {K}")
+    _check(lib().nv_token_logprobs(_p(logits), dt(logits), stride, R, V, _p(tokens), _p(logprob), _p(entropy), _p(rank), K,
+                                   _p(top_ids) if K else None, _p(top_logprobs) if K else None,
+                                   _p(err.t if err is not None else _global_err().t), _stream()), "token_logprobs")
 
 
 # ----------------------------------------------------------------------------- state mixers and their layer pieces

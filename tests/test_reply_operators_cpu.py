@@ -1,0 +1,73 @@
+"""What the operators of several replies to one prompt refuse, without a GPU: sizes at the C entries (which return before any
+launch), tensors and plans at the Python ones."""
+import pytest
+import torch
+
+from nano_vllm_cpp_b200.csrc import ops
+
+BAD_DTYPE, BAD_SIZE, UNSUPPORTED = -2, -3, -4
+
+
+def logprobs(dt=0, stride=100, R=1, V=100, K=0, ids=None, lps=None):
+    return ops.lib().nv_token_logprobs(None, dt, stride, R, V, None, None, None, None, K, ids, lps, None, None)
+
+
+def test_log_probabilities_refuse_sizes():
+    assert logprobs(R=0) == 0
+    assert logprobs(dt=2) == BAD_DTYPE
+    assert logprobs(R=-1) == BAD_SIZE
+    assert logprobs(V=0) == BAD_SIZE
+    assert logprobs(stride=99) == BAD_SIZE
+    assert logprobs(K=-1) == BAD_SIZE
+    assert logprobs(K=5) == BAD_SIZE                                        # alternatives without a place for them
+    assert logprobs(K=ops.max_top_logprobs() + 1, ids=16, lps=16) == BAD_SIZE
+    assert logprobs(V=3, stride=3, K=4, ids=16, lps=16) == BAD_SIZE         # more alternatives than ids
+
+
+def test_page_copies_refuse_sizes():
+    call = lambda A, n, N: ops.lib().nv_copy_pages(None, A, n, None, None, None, N, None, None)
+    assert call(0, 0, 5) == 0 and call(5, 64, 0) == 0
+    for bad in ((-1, 0, 1), (1, 0, -1), (1, -1, 1), (70000, 64, 1), (1, 64, 70000)):
+        assert call(*bad) == BAD_SIZE
+
+
+def shared(q_dt=1, R=1, M=0, groups=0, scale=1.0, Hq=4, Hkv=2, D=64, page=16, pages=8, own=1, ours=0):
+    return ops.lib().nv_attention_decode_shared(None, q_dt, 512, None, None, 1, None, 4, None, None, None, R, None, None, None, M, None,
+                                                None, groups, scale, None, 1, Hq, Hkv, D, page, pages, own, ours, None, None, 0, 0.0,
+                                                0, 0.0, None, 0, None)
+
+
+def test_shared_attention_refuses_sizes():
+    assert shared(R=0) == 0
+    assert shared(q_dt=2) == BAD_DTYPE
+    for kw in (dict(Hq=3), dict(Hkv=0), dict(Hq=0), dict(D=60), dict(D=264), dict(D=0), dict(page=24), dict(page=0), dict(scale=0.0),
+               dict(scale=-1.0), dict(scale=float("nan"))):
+        assert shared(**kw) == UNSUPPORTED, kw
+    for kw in (dict(R=-1), dict(M=-1), dict(groups=-1), dict(own=0), dict(ours=-1), dict(pages=0), dict()):        # (no scratch)
+        assert shared(**kw) == BAD_SIZE, kw
+
+
+def test_shared_prefix_packs_its_groups():
+    packed, members, longest = ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6)
+    assert members == 3 and longest == 32
+    assert packed[:6] == [0, 32, 7, 0, 32, 0]                               # shared positions of every row
+    assert packed[6:12] == [-1, 0, 1, -1, 0, -1]                            # its group
+    assert packed[12:15] == [4, 1, 2]                                       # the groups' rows, the leading one first
+    assert packed[18:21] == [0, 2, 3] and packed[21:] == [32, 7]
+    assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0, 0)
+
+
+@pytest.mark.parametrize("groups", [[([], 16)], [([0], -1)], [([3], 16)], [([-1], 16)], [([0, 0], 16)], [([0], 16), ([1, 0], 16)]])
+def test_shared_prefix_refuses_groups(groups):
+    with pytest.raises(ops.KernelError):
+        ops.SharedPrefix.pack(groups, 3)
+
+
+def test_tensors_of_the_host_are_refused():
+    x, i = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ops.KernelError):
+        ops.token_logprobs(x, i, torch.zeros(2))
+    with pytest.raises(ops.KernelError):
+        ops.PageArrays([torch.zeros(4, 2, 16, 8)])
+    with pytest.raises(ops.KernelError):
+        ops.PageArrays([])
