@@ -13,42 +13,29 @@
 
 namespace {
 
-constexpr int LP_THREADS = 512;
-
 // A float as an integer of the same order: NaN lowest, minus zero equal to zero.
 __device__ __forceinline__ uint32_t order_of(float x) {
   if (x != x) return 0u;
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-// ... and with the id as the second criterion, lower ids first.
-__device__ __forceinline__ unsigned long long key_of(float x, int id) {
-  return ((unsigned long long)order_of(x) << 32) | (uint32_t)(0x7fffffff - id);
+// ... and with the id as the second criterion, lower ids first.  (No key is zero.)
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float x, int id) { return ((Key)order_of(x) << 32) | (uint32_t)(0x7fffffff - id); }
+__device__ __forceinline__ int id_of(Key key) { return 0x7fffffff - (int)(uint32_t)key; }
+__device__ __forceinline__ float logit_of(Key key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return o == 0u ? NAN : __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
-__device__ __forceinline__ int id_of(unsigned long long key) { return 0x7fffffff - (int)(uint32_t)key; }
+__device__ __forceinline__ float max_nan(float a, float b) {       // (fmaxf drops a NaN)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 struct Stats {
   float m, n1, s, e;
 };
-__device__ __forceinline__ void add_value(Stats& a, float x) {
-  if (x > a.m) {
-    if (a.m != -INFINITY) {
-      const float d = a.m - x, c = expf(d);                  // (d is minus infinity where x is plus infinity: c is zero)
-      a.e = c > 0.f ? c * (a.e + d * (a.n1 + a.s)) : 0.f;
-      a.s = c * (a.n1 + a.s);
-    } else {
-      a.s *= 0.f;                                            // (nothing, or the NaN of an earlier element)
-    }
-    a.m = x;
-    a.n1 = 1.f;
-  } else if (x == a.m) {
-    a.n1 += 1.f;
-  } else {
-    const float d = x - a.m, c = expf(d);                    // (NaN stays NaN)
-    a.s += c;
-    if (c > 0.f) a.e = fmaf(c, d, a.e);
-  }
-}
 __device__ __forceinline__ Stats merge(const Stats& a, const Stats& b) {
   const Stats& hi = a.m >= b.m ? a : b;
   const Stats& lo = a.m >= b.m ? b : a;
@@ -59,9 +46,8 @@ __device__ __forceinline__ Stats merge(const Stats& a, const Stats& b) {
     r.e = hi.e + lo.e;
   } else {
     const float d = lo.m - hi.m, c = expf(d), all = lo.n1 + lo.s;
-    r.s = hi.s + c * all;
+    r.s = hi.s + c * all;                                    // (c is zero where nothing was there; a NaN in `all` stays)
     if (c > 0.f) r.e = hi.e + c * (lo.e + d * all);
-    if (lo.s != lo.s) r.s = lo.s;                            // a NaN among the lower ones
   }
   return r;
 }
@@ -76,28 +62,234 @@ struct LpArgs {
   int* top_ids;
   float* top_logprobs;
   int* err;
-  int V, K;
+  int R, V, K;
 };
 
+constexpr int LP_E = 16;               // elements a thread takes at a time: four (bfloat16: two) 16-byte loads under way
+constexpr int LP_LIST = 512;           // candidates that are kept before they are thinned out to the best K
+
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(LpArgs a) {
-  __shared__ Stats st_s[LP_THREADS / 32];
-  __shared__ int rank_s[LP_THREADS / 32];
-  __shared__ unsigned long long key_s[LP_THREADS / 32], best_s;
+struct Vec;                            // a 16-byte load as floats
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const float* p, float* x) {
+    const float4 v = __ldg((const float4*)p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  }
+};
+template <>
+struct Vec<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const bf16* p, float* x) {
+    const uint4 v = __ldg((const uint4*)p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {    // the address of block `rank`'s copy of a shared variable
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ Key ld_cluster_key(uint32_t a) {
+  Key v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// The K largest of the n keys in list[] come to its front, in descending order (fewer keys: zeros behind them); every thread of
+// the block calls.  n is small as a rule: a key's place is the number of larger ones.  More than LP_LIST keys (a row of equal or
+// rising logits) are first thinned out to the K by finding the K-th largest bit by bit.
+template <int THREADS>
+__device__ void keep_best(Key* list, int n, int K, Key* best, int* count) {
+  const int tid = threadIdx.x;
+  if (n > LP_LIST) {
+    Key kth = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const Key c = kth | ((Key)1 << bit);
+      int mine = 0;
+      for (int i = tid; i < n; i += THREADS) mine += list[i] >= c;
+      if (tid == 0) *count = 0;
+      __syncthreads();
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if (tid % 32 == 0 && mine) atomicAdd(count, mine);
+      __syncthreads();
+      if (*count >= K) kth = c;
+      __syncthreads();
+    }
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS)
+      if (list[i] >= kth) best[atomicAdd(count, 1)] = list[i];       // (the keys are distinct: K of them)
+    __syncthreads();
+    n = K;
+    if (tid < K) list[tid] = best[tid];
+    __syncthreads();
+  }
+  if (tid < K) best[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += THREADS) {
+    const Key k = list[i];
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += list[j] > k;
+    if (place < K) best[place] = k;
+  }
+  __syncthreads();
+  if (tid < K) list[tid] = best[tid];
+  __syncthreads();
+}
+
+// A cluster of blocks takes a row, each block a run of its 16-byte pieces; a thread keeps its own maximum and sums, which are
+// rescaled when the maximum moves.  Alternatives: the first tile gives a bound that at least K of its elements reach (of every
+// full warp's thread maxima the ceil(K / full warps)-th largest; the smallest of these), what lies above the bound goes into a list, and a
+// list that has grown long is thinned out, which raises the bound: a row costs a few hundred candidates, whatever its length.
+// The first block of the cluster joins the sums and lists.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
+  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, NV = LP_E / N;
+  extern __shared__ __align__(16) Key lp_list[];                     // LP_LIST + THREADS * LP_E candidates (K > 0)
+  __shared__ Stats st_s[WARPS], mine_s;
+  __shared__ Key best_s[32];
+  __shared__ int rank_s, bound_s[WARPS], n_s, count_s;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int cluster = (int)gridDim.x / a.R, row = blockIdx.x / cluster, part = blockIdx.x % cluster;
+  if (tid == 0) rank_s = n_s = 0;
   grid_dep_wait();
   grid_dep_launch();
-  const int row = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const T* x = (const T*)a.logits + (long long)row * a.stride;
-  const int token = a.tokens ? a.tokens[row] : 0;
-  const bool known = a.tokens && token >= 0 && token < a.V;
-  const unsigned long long mine = known ? key_of(to_f32(x[token]), token) : ~0ull;
+  const int token = a.tokens ? a.tokens[row] : -1;
+  const bool known = token >= 0 && token < a.V;
+  const float xt = known ? to_f32(x[token]) : 0.f;
+  const bool by_key = xt != xt;                                      // a NaN's place is found by keys, a number's by comparing numbers
+  const bool ranked = known && a.rank;
 
+  const int off = (int)(((uintptr_t)x / sizeof(T)) % N);              // elements between the 16-byte boundary below and the row
+  const int pieces = (int)(((long long)a.V + off + N - 1) / N), per = (pieces + cluster - 1) / cluster;
+  const int q0 = min(pieces, part * per), q1 = min(pieces, q0 + per);
   Stats st = {-INFINITY, 0.f, 0.f, 0.f};
   int ahead = 0;
-  for (int i = tid; i < a.V; i += LP_THREADS) {
-    const float v = to_f32(x[i]);
-    add_value(st, v);
-    ahead += key_of(v, i) > mine;
+  Key bound = 0;                                                      // candidates are above it
+  bool bounded = false;
+  for (int q = q0; q < q1; q += THREADS * NV) {
+    float v[LP_E];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int p = q + j * THREADS + tid, i0 = p * N - off;
+      if (p < q1 && i0 >= 0 && i0 + N <= a.V) {
+        Vec<T>::load(x + i0, v + j * N);
+      } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[j * N + u] = (p < q1 && i0 + u >= 0 && i0 + u < a.V) ? to_f32(x[i0 + u]) : -INFINITY;
+      }
+    }
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < LP_E; ++i) mx = fmaxf(mx, v[i]);
+    if (mx >= st.m) {                          // (or nothing but NaN and minus infinity so far)
+      if (mx > st.m) {
+        const float d = st.m - mx, c = ex2_fast(d * 1.4426950408889634f), all = st.n1 + st.s;
+        st.e = c > 0.f ? c * fmaf(d, all, st.e) : 0.f;
+        st.s = c * all;
+        st.n1 = 0.f;
+        st.m = mx;
+      }
+#pragma unroll
+      for (int i = 0; i < LP_E; ++i) {
+        const float d = v[i] - st.m, e = ex2_fast(d * 1.4426950408889634f);
+        if (v[i] == st.m) st.n1 += 1.f;
+        else if (st.m > -INFINITY || v[i] != v[i]) st.s += e;
+        if (e > 0.f) st.e = fmaf(e, d, st.e);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LP_E; ++i) {
+        const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * 1.4426950408889634f);
+        st.s += e;
+        st.e = fmaf(e, d, st.e);
+      }
+    }
+    if (ranked) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int i0 = (q + j * THREADS + tid) * N - off;
+        if (by_key || (i0 <= token && i0 + N > token)) {
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            ahead += i0 + u >= 0 && i0 + u < a.V && q + j * THREADS + tid < q1 && key_of(v[j * N + u], i0 + u) > key_of(xt, token);
+        } else {
+          const bool before = i0 < token && q + j * THREADS + tid < q1;      // equal logits of lower ids are ahead
+#pragma unroll
+          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > xt || (before && v[j * N + u] == xt && i0 + u >= 0);
+        }
+      }
+    }
+    if (a.K > 0) {
+      const uint32_t top = order_of(mx);
+      if (!bounded) {
+        const int full = min(WARPS, (q1 - q) / 32);                   // warps all of whose threads have elements
+        uint32_t o = mx > -INFINITY ? top : 0u, least = 0;
+        for (int j = 0; j < a.K && j * full < a.K; ++j) {
+          least = __reduce_max_sync(0xffffffffu, o);
+          const uint32_t who = __ballot_sync(0xffffffffu, o == least);
+          if (lane == __ffs(who) - 1) o = 0u;
+        }
+        if (lane == 0) bound_s[warp] = (int)least;
+        __syncthreads();
+        least = full > 0 ? (uint32_t)bound_s[0] : 0u;
+        for (int w = 1; w < full; ++w) least = min(least, (uint32_t)bound_s[w]);
+        bound = least ? ((Key)least << 32) - 1 : 0;
+        bounded = true;
+      }
+      if (__any_sync(0xffffffffu, bound == 0 || top >= (uint32_t)(bound >> 32))) {
+        uint32_t mine = 0;                                            // a bit for each of this thread's candidates
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int p = q + j * THREADS + tid, i0 = p * N - off;
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            mine |= (p < q1 && i0 + u >= 0 && i0 + u < a.V && key_of(v[j * N + u], i0 + u) > bound ? 1u : 0u) << (j * N + u);
+        }
+        int at = __popc(mine);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int before = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += before;
+        }
+        int base = 0;
+        if (lane == 31 && at > 0) base = atomicAdd(&n_s, at);
+        at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
+#pragma unroll
+        for (int i = 0; i < LP_E; ++i)
+          if (mine >> i & 1u) lp_list[at++] = key_of(v[i], (q + i / N * THREADS + tid) * N - off + i % N);
+      }
+      __syncthreads();
+      const int n = n_s;
+      if (n > LP_LIST) {
+        keep_best<THREADS>(lp_list, n, a.K, best_s, &count_s);
+        bound = lp_list[a.K - 1];
+        if (tid == 0) n_s = a.K;
+      }
+      __syncthreads();
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -107,53 +299,91 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(LpArgs a) {
     other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
     other.e = __shfl_xor_sync(0xffffffffu, st.e, o);
     st = (lane & o) ? merge(other, st) : merge(st, other);
-    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
   }
-  if (lane == 0) {
-    st_s[warp] = st;
-    rank_s[warp] = ahead;
-  }
-  __syncthreads();
-  st = st_s[0];
-  ahead = rank_s[0];
-  for (int w = 1; w < LP_THREADS / 32; ++w) {
-    st = merge(st, st_s[w]);
-    ahead += rank_s[w];
-  }
-  const bool proper = fabsf(st.m) < INFINITY;
-  const float log_z = proper ? logf(st.n1) + log1pf(st.s / st.n1) : NAN;
+  if (lane == 0) st_s[warp] = st;
+  ahead = __reduce_add_sync(0xffffffffu, ahead);
+  __syncthreads();                                                    // (rank_s is zero)
+  if (lane == 0 && ahead) atomicAdd(&rank_s, ahead);
   if (tid == 0) {
-    if (a.tokens) {
-      if (!known && a.err) atomicExch(a.err, 1 + row);
-      if (a.logprob) a.logprob[row] = known ? (to_f32(x[token]) - st.m) - log_z : NAN;
-      if (a.rank) a.rank[row] = known ? ahead : -1;
-    }
-    if (a.entropy) a.entropy[row] = log_z - st.e / (st.n1 + st.s);
+    for (int w = 1; w < WARPS; ++w) st = merge(st, st_s[w]);
+    mine_s = st;
   }
-  unsigned long long below = ~0ull;
-  for (int k = 0; k < a.K; ++k) {
-    unsigned long long best = 0;
-    for (int i = tid; i < a.V; i += LP_THREADS) {
-      const unsigned long long key = key_of(to_f32(x[i]), i);
-      if (key < below && key > best) best = key;
+  if (a.K > 0) keep_best<THREADS>(lp_list, n_s, a.K, best_s, &count_s);
+  if (cluster > 1) cluster_sync_all();
+  else __syncthreads();
+  if (part == 0) {
+    st = mine_s;
+    ahead = rank_s;
+    for (int c = 1; c < cluster; ++c) {
+      const uint32_t at = of_rank(&mine_s, c);
+      const Stats other = {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8), ld_cluster_f32(at + 12)};
+      st = merge(st, other);
+      ahead += __float_as_int(ld_cluster_f32(of_rank(&rank_s, c)));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
-    if (lane == 0) key_s[warp] = best;
-    __syncthreads();
+    const bool proper = fabsf(st.m) < INFINITY;
+    const float log_z = proper ? logf(st.n1) + log1pf(st.s / st.n1) : NAN;
     if (tid == 0) {
-      for (int w = 1; w < LP_THREADS / 32; ++w) best = key_s[w] > best ? key_s[w] : best;
-      best_s = best;
-      const int id = id_of(best);
-      a.top_ids[(long long)row * a.K + k] = id;
-      a.top_logprobs[(long long)row * a.K + k] = (to_f32(x[id]) - st.m) - log_z;
+      if (a.tokens) {
+        if (!known && a.err) atomicExch(a.err, 1 + row);
+        if (a.logprob) a.logprob[row] = known ? (xt - st.m) - log_z : NAN;
+        if (a.rank) a.rank[row] = known ? ahead : -1;
+      }
+      if (a.entropy) a.entropy[row] = log_z - st.e / (st.n1 + st.s);
     }
-    __syncthreads();
-    below = best_s;
+    if (a.K > 0) {
+      const int n = cluster * a.K;                                    // every block's best, in order
+      if (cluster > 1) {
+        for (int i = tid; i < n - a.K; i += THREADS) lp_list[a.K + i] = ld_cluster_key(of_rank(&best_s[i % a.K], 1 + i / a.K));
+        __syncthreads();
+        // (zeros, of blocks with fewer than K elements, have the same place, behind the row's K and more keys)
+        for (int i = tid; i < n; i += THREADS) {
+          const Key k = lp_list[i];
+          int place = 0;
+          for (int j = 0; j < n; ++j) place += lp_list[j] > k;
+          if (place < a.K) {
+            a.top_ids[(long long)row * a.K + place] = id_of(k);
+            a.top_logprobs[(long long)row * a.K + place] = (logit_of(k) - st.m) - log_z;
+          }
+        }
+      } else if (tid < a.K) {
+        const Key k = lp_list[tid];
+        a.top_ids[(long long)row * a.K + tid] = id_of(k);
+        a.top_logprobs[(long long)row * a.K + tid] = (logit_of(k) - st.m) - log_z;
+      }
+    }
   }
+  if (cluster > 1) cluster_sync_all();                                // nobody leaves while its lists are read
+}
+
+template <typename T, int THREADS>
+int launch_logprobs(const LpArgs& a, unsigned cluster, cudaStream_t s) {
+  const size_t smem = a.K > 0 ? (size_t)(LP_LIST + THREADS * LP_E) * sizeof(Key) : 0;
+  if (smem > 48 * 1024) {
+    static bool attr_done = false;
+    if (!attr_done) {
+      NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (LP_LIST + THREADS * LP_E) * (int)sizeof(Key)));
+      attr_done = true;
+    }
+  }
+  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T, THREADS>, dim3(a.R * cluster), dim3(THREADS), smem, s, a));
+  NV_RETURN_LAST();
+}
+
+// Blocks a row, and threads a block: a handful of rows takes large blocks, as many as a cluster has, of at least a tile each (a
+// row's latency is what counts); more rows take blocks of 256 threads, of which several live on a multiprocessor, in clusters until
+// there are enough for all multiprocessors.
+template <typename T>
+int run_logprobs(const LpArgs& a, cudaStream_t s) {
+  const long long sms = num_multiprocessors();
+  if (a.R * 8LL <= sms) {
+    unsigned cluster = 8;
+    while (cluster > 1 && a.V / (int)cluster < 1024 * LP_E / 4) cluster /= 2;
+    return launch_logprobs<T, 1024>(a, cluster, s);
+  }
+  unsigned cluster = 1;
+  while (cluster < 8 && a.R * (long long)cluster < 4 * sms && a.V / (int)(2 * cluster) >= 256 * LP_E) cluster *= 2;
+  return launch_logprobs<T, 256>(a, cluster, s);
 }
 
 }  // namespace
@@ -166,11 +396,9 @@ NV_API int nv_token_logprobs_max_top(void) { return 32; }
 NV_API int nv_token_logprobs(const void* logits, int dt, long long stride, int R, int V, const int* tokens, float* logprob,
                              float* entropy, int* rank, int K, int* top_ids, float* top_logprobs, int* err, cudaStream_t s) {
   if (!dt_ok(dt)) return NV_ERR_BAD_DTYPE;
-  if (R < 0 || V < 1 || stride < V || K < 0 || K > V || K > nv_token_logprobs_max_top()) return NV_ERR_BAD_SIZE;
+  if (R < 0 || V < 1 || V > 1 << 30 || stride < V || K < 0 || K > V || K > nv_token_logprobs_max_top()) return NV_ERR_BAD_SIZE;
   if (K > 0 && (!top_ids || !top_logprobs)) return NV_ERR_BAD_SIZE;
   if (R == 0) return NV_OK;
-  LpArgs a = {logits, stride, tokens, logprob, entropy, rank, top_ids, top_logprobs, err, V, K};
-  if (dt == NV_DT_F32) NV_RETURN_IF(launch_dep(token_logprobs_kernel<float>, dim3(R), dim3(LP_THREADS), 0, s, a));
-  else NV_RETURN_IF(launch_dep(token_logprobs_kernel<bf16>, dim3(R), dim3(LP_THREADS), 0, s, a));
-  NV_RETURN_LAST();
+  const LpArgs a = {logits, stride, tokens, logprob, entropy, rank, top_ids, top_logprobs, err, R, V, K};
+  return dt == NV_DT_F32 ? run_logprobs<float>(a, s) : run_logprobs<bf16>(a, s);
 }
