@@ -23,10 +23,11 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 typedef unsigned long long Key;
 __device__ __forceinline__ Key key_of(float x, int id) { return ((Key)order_of(x) << 32) | (uint32_t)(0x7fffffff - id); }
 __device__ __forceinline__ int id_of(Key key) { return 0x7fffffff - (int)(uint32_t)key; }
-__device__ __forceinline__ float logit_of(Key key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return o == 0u ? NAN : __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+__device__ __forceinline__ float float_of(uint32_t order) {
+  return order == 0u ? NAN : __uint_as_float((order & 0x80000000u) ? (order & 0x7fffffffu) : ~order);
 }
+// The next number below (minus zero, which equals zero, is none of its own).
+__device__ __forceinline__ float below_of(uint32_t order) { return float_of(order == 0x80000000u ? 0x7ffffffeu : order - 1); }
 __device__ __forceinline__ float max_nan(float a, float b) {       // (fmaxf drops a NaN)
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -158,8 +159,8 @@ __device__ void keep_best(Key* list, int n, int K, Key* best, int* count) {
   __syncthreads();
 }
 
-// A cluster of blocks takes a row, each block a run of its 16-byte pieces; a thread keeps its own maximum and sums, which are
-// rescaled when the maximum moves.  Alternatives: the first tile gives a bound that at least K of its elements reach (of every
+// A cluster of blocks takes a row, each block a run of its 16-byte pieces; a warp has a maximum, its threads their
+// sums, which are rescaled when it moves.  Alternatives: the first tile gives a bound that at least K of its elements reach (of every
 // full warp's thread maxima the ceil(K / full warps)-th largest; the smallest of these), what lies above the bound goes into a list, and a
 // list that has grown long is thinned out, which raises the bound: a row costs a few hundred candidates, whatever its length.
 // The first block of the cluster joins the sums and lists.
@@ -179,15 +180,19 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
   const int token = a.tokens ? a.tokens[row] : -1;
   const bool known = token >= 0 && token < a.V;
   const float xt = known ? to_f32(x[token]) : 0.f;
-  const bool by_key = xt != xt;                                      // a NaN's place is found by keys, a number's by comparing numbers
+  // places are found by comparing numbers, those of a NaN or minus infinity by keys; the next number below xt
+  const bool by_key = !(xt > -INFINITY);
+  const float xt_below = below_of(order_of(xt));
   const bool ranked = known && a.rank;
 
   const int off = (int)(((uintptr_t)x / sizeof(T)) % N);              // elements between the 16-byte boundary below and the row
   const int pieces = (int)(((long long)a.V + off + N - 1) / N), per = (pieces + cluster - 1) / cluster;
   const int q0 = min(pieces, part * per), q1 = min(pieces, q0 + per);
   Stats st = {-INFINITY, 0.f, 0.f, 0.f};
+  uint32_t m_order = 0x007fffffu;                                     // (minus infinity's)
   int ahead = 0;
   Key bound = 0;                                                      // candidates are above it
+  float above = -INFINITY;                                            // ... as a number, where it is one
   bool bounded = false;
   for (int q = q0; q < q1; q += THREADS * NV) {
     float v[LP_E];
@@ -204,20 +209,31 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < LP_E; ++i) mx = fmaxf(mx, v[i]);
-    if (mx >= st.m) {                          // (or nothing but NaN and minus infinity so far)
-      if (mx > st.m) {
-        const float d = st.m - mx, c = ex2_fast(d * 1.4426950408889634f), all = st.n1 + st.s;
+    // the warp's maximum: all its threads keep their sums against one m, and a tile that does not reach it (most of them) takes the
+    // short way, where no term is the largest
+    const uint32_t top = order_of(mx), tile_top = __reduce_max_sync(0xffffffffu, top);
+    if (tile_top >= m_order) {
+      if (tile_top > m_order) {
+        m_order = tile_top;
+        const float m = float_of(tile_top), d = st.m - m, c = ex2_fast(d * 1.4426950408889634f), all = st.n1 + st.s;
         st.e = c > 0.f ? c * fmaf(d, all, st.e) : 0.f;
-        st.s = c * all;
+        st.s = c * all;                                               // (zero where nothing was there; a NaN stays)
         st.n1 = 0.f;
-        st.m = mx;
+        st.m = m;
       }
+      if (st.m > -INFINITY) {
 #pragma unroll
-      for (int i = 0; i < LP_E; ++i) {
-        const float d = v[i] - st.m, e = ex2_fast(d * 1.4426950408889634f);
-        if (v[i] == st.m) st.n1 += 1.f;
-        else if (st.m > -INFINITY || v[i] != v[i]) st.s += e;
-        if (e > 0.f) st.e = fmaf(e, d, st.e);
+        for (int i = 0; i < LP_E; ++i) {
+          const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * 1.4426950408889634f);
+          const float other = d == 0.f ? 0.f : e;
+          st.s += other;
+          st.n1 += e - other;                                         // (2^0 is one)
+          st.e = fmaf(e, d, st.e);
+        }
+      } else {                                                        // nothing but NaN and minus infinity so far
+#pragma unroll
+        for (int i = 0; i < LP_E; ++i)
+          if (v[i] != v[i]) st.s = NAN;
       }
     } else {
 #pragma unroll
@@ -230,20 +246,19 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
     if (ranked) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int i0 = (q + j * THREADS + tid) * N - off;
+        const int p = q + j * THREADS + tid, i0 = p * N - off;
         if (by_key || (i0 <= token && i0 + N > token)) {
 #pragma unroll
           for (int u = 0; u < N; ++u)
-            ahead += i0 + u >= 0 && i0 + u < a.V && q + j * THREADS + tid < q1 && key_of(v[j * N + u], i0 + u) > key_of(xt, token);
+            ahead += i0 + u >= 0 && i0 + u < a.V && p < q1 && key_of(v[j * N + u], i0 + u) > key_of(xt, token);
         } else {
-          const bool before = i0 < token && q + j * THREADS + tid < q1;      // equal logits of lower ids are ahead
+          const float above = i0 < token ? xt_below : xt;             // equal logits of lower ids are ahead
 #pragma unroll
-          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > xt || (before && v[j * N + u] == xt && i0 + u >= 0);
+          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > above;
         }
       }
     }
     if (a.K > 0) {
-      const uint32_t top = order_of(mx);
       if (!bounded) {
         const int full = min(WARPS, (q1 - q) / 32);                   // warps all of whose threads have elements
         uint32_t o = mx > -INFINITY ? top : 0u, least = 0;
@@ -257,16 +272,22 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
         least = full > 0 ? (uint32_t)bound_s[0] : 0u;
         for (int w = 1; w < full; ++w) least = min(least, (uint32_t)bound_s[w]);
         bound = least ? ((Key)least << 32) - 1 : 0;
+        above = least ? below_of(least) : -INFINITY;
         bounded = true;
       }
-      if (__any_sync(0xffffffffu, bound == 0 || top >= (uint32_t)(bound >> 32))) {
+      if (above > -INFINITY ? float_of(tile_top) > above : bound == 0 || tile_top >= (uint32_t)(bound >> 32)) {
         uint32_t mine = 0;                                            // a bit for each of this thread's candidates
+        if (above > -INFINITY) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int p = q + j * THREADS + tid, i0 = p * N - off;
+          for (int i = 0; i < LP_E; ++i) mine |= (v[i] > above ? 1u : 0u) << i;
+        } else {                                                      // no bound, or one among what is masked
 #pragma unroll
-          for (int u = 0; u < N; ++u)
-            mine |= (p < q1 && i0 + u >= 0 && i0 + u < a.V && key_of(v[j * N + u], i0 + u) > bound ? 1u : 0u) << (j * N + u);
+          for (int j = 0; j < NV; ++j) {
+            const int p = q + j * THREADS + tid, i0 = p * N - off;
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+              mine |= (p < q1 && i0 + u >= 0 && i0 + u < a.V && key_of(v[j * N + u], i0 + u) > bound ? 1u : 0u) << (j * N + u);
+          }
         }
         int at = __popc(mine);
 #pragma unroll
@@ -286,20 +307,15 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
       if (n > LP_LIST) {
         keep_best<THREADS>(lp_list, n, a.K, best_s, &count_s);
         bound = lp_list[a.K - 1];
+        above = float_of((uint32_t)(bound >> 32));                    // (equal logits from here on have higher ids)
         if (tid == 0) n_s = a.K;
       }
       __syncthreads();
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.n1 = __shfl_xor_sync(0xffffffffu, st.n1, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.e = __shfl_xor_sync(0xffffffffu, st.e, o);
-    st = (lane & o) ? merge(other, st) : merge(st, other);
-  }
+  st.n1 = warp_sum(st.n1);
+  st.s = warp_sum(st.s);
+  st.e = warp_sum(st.e);
   if (lane == 0) st_s[warp] = st;
   ahead = __reduce_add_sync(0xffffffffu, ahead);
   __syncthreads();                                                    // (rank_s is zero)
@@ -342,13 +358,13 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
           for (int j = 0; j < n; ++j) place += lp_list[j] > k;
           if (place < a.K) {
             a.top_ids[(long long)row * a.K + place] = id_of(k);
-            a.top_logprobs[(long long)row * a.K + place] = (logit_of(k) - st.m) - log_z;
+            a.top_logprobs[(long long)row * a.K + place] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
           }
         }
       } else if (tid < a.K) {
         const Key k = lp_list[tid];
         a.top_ids[(long long)row * a.K + tid] = id_of(k);
-        a.top_logprobs[(long long)row * a.K + tid] = (logit_of(k) - st.m) - log_z;
+        a.top_logprobs[(long long)row * a.K + tid] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
       }
     }
   }
