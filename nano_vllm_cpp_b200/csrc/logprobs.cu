@@ -37,19 +37,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {       // (fmaxf dro
 struct Stats {
   float m, n1, s, e;
 };
-__device__ __forceinline__ Stats merge(const Stats& a, const Stats& b) {
-  const Stats& hi = a.m >= b.m ? a : b;
-  const Stats& lo = a.m >= b.m ? b : a;
-  Stats r = hi;
-  if (lo.m == hi.m) {
-    r.n1 = hi.n1 + lo.n1;
-    r.s = hi.s + lo.s;
-    r.e = hi.e + lo.e;
-  } else {
-    const float d = lo.m - hi.m, c = expf(d), all = lo.n1 + lo.s;
-    r.s = hi.s + c * all;                                    // (c is zero where nothing was there; a NaN in `all` stays)
-    if (c > 0.f) r.e = hi.e + c * (lo.e + d * all);
-  }
+// The sums of a warp's lanes, each against its own maximum, against the largest of them; every lane gets them.
+__device__ __forceinline__ Stats join(const Stats& a) {
+  Stats r;
+  r.m = warp_max(a.m);
+  const bool mine = a.m == r.m;
+  const float d = a.m - r.m, c = mine ? 1.f : expf(d), all = a.n1 + a.s;
+  r.n1 = warp_sum(mine ? a.n1 : 0.f);
+  r.s = warp_sum(mine ? a.s : c * all);                      // (c is zero where nothing was there; a NaN in `all` stays)
+  r.e = warp_sum(mine ? a.e : c > 0.f ? c * (a.e + d * all) : 0.f);
   return r;
 }
 
@@ -67,7 +63,9 @@ struct LpArgs {
 };
 
 constexpr int LP_E = 16;               // elements a thread takes at a time: four (bfloat16: two) 16-byte loads under way
-constexpr int LP_LIST = 512;           // candidates that are kept before they are thinned out to the best K
+constexpr int LP_LIST = 1024;          // candidates a block has room for (and at least 512 beside a bound that a tile may bring)
+constexpr int LP_LONG = 256;           // ... and from how many on they are thinned out to the best K
+constexpr float LOG2E = 1.4426950408889634f;
 
 template <typename T>
 struct Vec;                            // a 16-byte load as floats
@@ -117,41 +115,24 @@ __device__ __forceinline__ Key ld_cluster_key(uint32_t a) {
   return v;
 }
 
-// The K largest of the n keys in list[] come to its front, in descending order (fewer keys: zeros behind them); every thread of
-// the block calls.  n is small as a rule: a key's place is the number of larger ones.  More than LP_LIST keys (a row of equal or
-// rising logits) are first thinned out to the K by finding the K-th largest bit by bit.
+// The K largest of the n keys in list[] come to its front and to best[], in descending order (fewer keys: zeros behind them); every
+// thread of the block calls, between two barriers.  A key's place is the number of larger ones.
 template <int THREADS>
-__device__ void keep_best(Key* list, int n, int K, Key* best, int* count) {
+__device__ void keep_best(Key* list, int n, int K, Key* best) {
   const int tid = threadIdx.x;
-  if (n > LP_LIST) {
-    Key kth = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const Key c = kth | ((Key)1 << bit);
-      int mine = 0;
-      for (int i = tid; i < n; i += THREADS) mine += list[i] >= c;
-      if (tid == 0) *count = 0;
-      __syncthreads();
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      if (tid % 32 == 0 && mine) atomicAdd(count, mine);
-      __syncthreads();
-      if (*count >= K) kth = c;
-      __syncthreads();
-    }
-    if (tid == 0) *count = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += THREADS)
-      if (list[i] >= kth) best[atomicAdd(count, 1)] = list[i];       // (the keys are distinct: K of them)
-    __syncthreads();
-    n = K;
-    if (tid < K) list[tid] = best[tid];
-    __syncthreads();
-  }
   if (tid < K) best[tid] = 0;
   __syncthreads();
   for (int i = tid; i < n; i += THREADS) {
     const Key k = list[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += list[j] > k;
+    int place = 0, j = 0;
+    for (; j + 8 <= n; j += 8) {
+      Key other[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) other[u] = list[j + u];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) place += other[u] > k;
+    }
+    for (; j < n; ++j) place += list[j] > k;
     if (place < K) best[place] = k;
   }
   __syncthreads();
@@ -159,18 +140,44 @@ __device__ void keep_best(Key* list, int n, int K, Key* best, int* count) {
   __syncthreads();
 }
 
-// A cluster of blocks takes a row, each block a run of its 16-byte pieces; a warp has a maximum, its threads their
-// sums, which are rescaled when it moves.  Alternatives: the first tile gives a bound that at least K of its elements reach (of every
-// full warp's thread maxima the ceil(K / full warps)-th largest; the smallest of these), what lies above the bound goes into a list, and a
-// list that has grown long is thinned out, which raises the bound: a row costs a few hundred candidates, whatever its length.
-// The first block of the cluster joins the sums and lists.
+// One after the other in runs of a warp's width, whatever the logits are: for rows whose bound let too many candidates through
+// (rising ones) or too few (fewer than K logits above minus infinity).
+template <typename T, int THREADS>
+__device__ void collect_slowly(const T* x, int i0, int i1, int K, Key* list, Key* best, int* n_s) {
+  constexpr int RUN = THREADS < LP_LIST - LP_LONG ? THREADS : LP_LIST - LP_LONG;
+  Key bound = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) *n_s = 0;
+  __syncthreads();
+  for (int i = i0; i < i1; i += RUN) {
+    if (threadIdx.x < RUN && i + (int)threadIdx.x < i1) {
+      const Key k = key_of(to_f32(x[i + threadIdx.x]), i + threadIdx.x);
+      if (k > bound) list[atomicAdd(n_s, 1)] = k;
+    }
+    __syncthreads();
+    const int n = *n_s;
+    if (n > LP_LONG) {
+      keep_best<THREADS>(list, n, K, best);
+      bound = list[K - 1];
+      if (threadIdx.x == 0) *n_s = K;
+    }
+    __syncthreads();
+  }
+}
+
+// A cluster of blocks takes a row, each block a run of its 16-byte pieces; a warp has a maximum, its threads their sums, which are
+// rescaled when it moves.  Alternatives: the first tile gives a bound that at least K of its logits reach (the K-th largest among
+// every full warp's few largest thread maxima), what lies above it goes into a list, and a list that has grown long is thinned
+// out, which raises the bound: a tile adds some K candidates and fewer and fewer, whatever the row's length.  The first block of
+// the cluster joins the sums and lists.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
-  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, NV = LP_E / N;
-  extern __shared__ __align__(16) Key lp_list[];                     // LP_LIST + THREADS * LP_E candidates (K > 0)
-  __shared__ Stats st_s[WARPS], mine_s;
+  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, NV = LP_E / N, TILE = THREADS * NV;      // (a tile in pieces)
+  __shared__ Key list_s[LP_LIST];
   __shared__ Key best_s[32];
-  __shared__ int rank_s, bound_s[WARPS], n_s, count_s;
+  __shared__ Stats st_s[WARPS], mine_s;
+  __shared__ uint32_t most_s[64];
+  __shared__ int rank_s, n_s;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int cluster = (int)gridDim.x / a.R, row = blockIdx.x / cluster, part = blockIdx.x % cluster;
   if (tid == 0) rank_s = n_s = 0;
@@ -182,40 +189,46 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
   const float xt = known ? to_f32(x[token]) : 0.f;
   // places are found by comparing numbers, those of a NaN or minus infinity by keys; the next number below xt
   const bool by_key = !(xt > -INFINITY);
-  const float xt_below = below_of(order_of(xt));
+  const uint32_t xt_order = order_of(xt);
+  const float xt_below = below_of(xt_order);
   const bool ranked = known && a.rank;
 
   const int off = (int)(((uintptr_t)x / sizeof(T)) % N);              // elements between the 16-byte boundary below and the row
   const int pieces = (int)(((long long)a.V + off + N - 1) / N), per = (pieces + cluster - 1) / cluster;
   const int q0 = min(pieces, part * per), q1 = min(pieces, q0 + per);
   Stats st = {-INFINITY, 0.f, 0.f, 0.f};
-  uint32_t m_order = 0x007fffffu;                                     // (minus infinity's)
-  int ahead = 0;
-  Key bound = 0;                                                      // candidates are above it
-  float above = -INFINITY;                                            // ... as a number, where it is one
-  bool bounded = false;
-  for (int q = q0; q < q1; q += THREADS * NV) {
+  uint32_t m_order = 0x007fffffu;                                     // st.m's (minus infinity's)
+  int ahead = 0, tile = 0;
+  float above = -INFINITY;                                            // candidates are above it
+  bool bounded = false, lost = false;
+  for (int q = q0; q < q1; q += TILE, ++tile) {
     float v[LP_E];
+    if (q * N >= off && q + TILE <= q1 && (long long)(q + TILE) * N - off <= a.V) {
+      const T* from = x + ((long long)(q + tid) * N - off);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int p = q + j * THREADS + tid, i0 = p * N - off;
-      if (p < q1 && i0 >= 0 && i0 + N <= a.V) {
-        Vec<T>::load(x + i0, v + j * N);
-      } else {
+      for (int j = 0; j < NV; ++j) Vec<T>::load(from + j * (THREADS * N), v + j * N);
+    } else {
 #pragma unroll
-        for (int u = 0; u < N; ++u) v[j * N + u] = (p < q1 && i0 + u >= 0 && i0 + u < a.V) ? to_f32(x[i0 + u]) : -INFINITY;
+      for (int j = 0; j < NV; ++j) {
+        const int p = q + j * THREADS + tid, i0 = p * N - off;
+        if (p < q1 && i0 >= 0 && i0 + N <= a.V) {
+          Vec<T>::load(x + i0, v + j * N);
+        } else {
+#pragma unroll
+          for (int u = 0; u < N; ++u) v[j * N + u] = (p < q1 && i0 + u >= 0 && i0 + u < a.V) ? to_f32(x[i0 + u]) : -INFINITY;
+        }
       }
     }
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < LP_E; ++i) mx = fmaxf(mx, v[i]);
-    // the warp's maximum: all its threads keep their sums against one m, and a tile that does not reach it (most of them) takes the
-    // short way, where no term is the largest
+    // all threads of a warp keep their sums against one m, and a tile that does not reach it (most of them) takes the short way,
+    // where no term is the largest
     const uint32_t top = order_of(mx), tile_top = __reduce_max_sync(0xffffffffu, top);
     if (tile_top >= m_order) {
       if (tile_top > m_order) {
         m_order = tile_top;
-        const float m = float_of(tile_top), d = st.m - m, c = ex2_fast(d * 1.4426950408889634f), all = st.n1 + st.s;
+        const float m = float_of(tile_top), d = st.m - m, c = ex2_fast(d * LOG2E), all = st.n1 + st.s;
         st.e = c > 0.f ? c * fmaf(d, all, st.e) : 0.f;
         st.s = c * all;                                               // (zero where nothing was there; a NaN stays)
         st.n1 = 0.f;
@@ -224,8 +237,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
       if (st.m > -INFINITY) {
 #pragma unroll
         for (int i = 0; i < LP_E; ++i) {
-          const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * 1.4426950408889634f);
-          const float other = d == 0.f ? 0.f : e;
+          const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * LOG2E), other = d == 0.f ? 0.f : e;
           st.s += other;
           st.n1 += e - other;                                         // (2^0 is one)
           st.e = fmaf(e, d, st.e);
@@ -238,12 +250,12 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < LP_E; ++i) {
-        const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * 1.4426950408889634f);
+        const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * LOG2E);
         st.s += e;
         st.e = fmaf(e, d, st.e);
       }
     }
-    if (ranked) {
+    if (ranked && (by_key || tile_top >= xt_order)) {                  // (else nothing of the tile is ahead of the token)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int p = q + j * THREADS + tid, i0 = p * N - off;
@@ -252,43 +264,44 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
           for (int u = 0; u < N; ++u)
             ahead += i0 + u >= 0 && i0 + u < a.V && p < q1 && key_of(v[j * N + u], i0 + u) > key_of(xt, token);
         } else {
-          const float above = i0 < token ? xt_below : xt;             // equal logits of lower ids are ahead
+          const float over = i0 < token ? xt_below : xt;              // equal logits of lower ids are ahead
 #pragma unroll
-          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > above;
+          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > over;
         }
       }
     }
-    if (a.K > 0) {
-      if (!bounded) {
-        const int full = min(WARPS, (q1 - q) / 32);                   // warps all of whose threads have elements
-        uint32_t o = mx > -INFINITY ? top : 0u, least = 0;
-        for (int j = 0; j < a.K && j * full < a.K; ++j) {
-          least = __reduce_max_sync(0xffffffffu, o);
-          const uint32_t who = __ballot_sync(0xffffffffu, o == least);
+    if (a.K > 0 && !lost) {
+      const int full = min(WARPS, (q1 - q) / 32);                     // warps all of whose threads have elements
+      if (!bounded && full > 0) {
+        const int each = min(32, min((a.K + full - 1) / full + 1, 64 / full));       // (K <= 32: enough, with one to spare where there is room)
+        uint32_t o = mx > -INFINITY ? top : 0u;
+        for (int j = 0; j < each; ++j) {
+          const uint32_t most = __reduce_max_sync(0xffffffffu, o);
+          const uint32_t who = __ballot_sync(0xffffffffu, o == most);
           if (lane == __ffs(who) - 1) o = 0u;
+          if (lane == 0 && warp < full) most_s[warp * each + j] = most;
         }
-        if (lane == 0) bound_s[warp] = (int)least;
         __syncthreads();
-        least = full > 0 ? (uint32_t)bound_s[0] : 0u;
-        for (int w = 1; w < full; ++w) least = min(least, (uint32_t)bound_s[w]);
-        bound = least ? ((Key)least << 32) - 1 : 0;
-        above = least ? below_of(least) : -INFINITY;
-        bounded = true;
-      }
-      if (above > -INFINITY ? float_of(tile_top) > above : bound == 0 || tile_top >= (uint32_t)(bound >> 32)) {
-        uint32_t mine = 0;                                            // a bit for each of this thread's candidates
-        if (above > -INFINITY) {
-#pragma unroll
-          for (int i = 0; i < LP_E; ++i) mine |= (v[i] > above ? 1u : 0u) << i;
-        } else {                                                      // no bound, or one among what is masked
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const int p = q + j * THREADS + tid, i0 = p * N - off;
-#pragma unroll
-            for (int u = 0; u < N; ++u)
-              mine |= (p < q1 && i0 + u >= 0 && i0 + u < a.V && key_of(v[j * N + u], i0 + u) > bound ? 1u : 0u) << (j * N + u);
-          }
+        // the K-th largest of these (at least K: `each` from every full warp); equal ones in their order
+        const int n = full * each;
+        uint32_t kth = 0u;
+        for (int i = lane; i < n; i += 32) {
+          const uint32_t w = most_s[i];
+          int place = 0;
+          for (int j = 0; j < n; ++j) place += most_s[j] > w || (most_s[j] == w && j < i);
+          if (place == a.K - 1) kth = w;
         }
+        kth = __reduce_max_sync(0xffffffffu, kth);
+        if (kth > 0u) {
+          above = below_of(kth);
+          bounded = true;
+        }
+        __syncthreads();
+      }
+      if (float_of(tile_top) > above) {
+        uint32_t mine = 0;                                            // a bit for each of this thread's candidates
+#pragma unroll
+        for (int i = 0; i < LP_E; ++i) mine |= (v[i] > above ? 1u : 0u) << i;
         int at = __popc(mine);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -296,46 +309,70 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
           if (lane >= o) at += before;
         }
         int base = 0;
-        if (lane == 31 && at > 0) base = atomicAdd(&n_s, at);
+        if (lane == 31) base = atomicAdd(&n_s, at);
         at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
+        if (mine) {
 #pragma unroll
-        for (int i = 0; i < LP_E; ++i)
-          if (mine >> i & 1u) lp_list[at++] = key_of(v[i], (q + i / N * THREADS + tid) * N - off + i % N);
+          for (int i = 0; i < LP_E; ++i)
+            if (mine >> i & 1u) {
+              if (at < LP_LIST) list_s[at] = key_of(v[i], (q + i / N * THREADS + tid) * N - off + i % N);
+              ++at;
+            }
+        }
       }
-      __syncthreads();
-      const int n = n_s;
-      if (n > LP_LIST) {
-        keep_best<THREADS>(lp_list, n, a.K, best_s, &count_s);
-        bound = lp_list[a.K - 1];
-        above = float_of((uint32_t)(bound >> 32));                    // (equal logits from here on have higher ids)
-        if (tid == 0) n_s = a.K;
+      if (tile % 8 == 7) {
+        __syncthreads();
+        const int n = n_s;
+        __syncthreads();
+        lost = n > LP_LIST;                                           // (collected again at the end)
+        if (n > LP_LONG && !lost) {
+          keep_best<THREADS>(list_s, n, a.K, best_s);
+          above = float_of((uint32_t)(list_s[a.K - 1] >> 32));        // (equal logits from here on have higher ids)
+          bounded = true;
+          if (tid == 0) n_s = a.K;
+          __syncthreads();
+        }
       }
-      __syncthreads();
     }
+  }
+  const int first = max(0, q0 * N - off), last = min(a.V, q1 * N - off);          // this block's elements
+  if (a.K > 0) {
+    __syncthreads();
+    const int n = n_s;
+    if (n > LP_LIST || n < min(a.K, last - first)) collect_slowly<T, THREADS>(x, first, last, a.K, list_s, best_s, &n_s);
+    keep_best<THREADS>(list_s, n_s, a.K, best_s);
   }
   st.n1 = warp_sum(st.n1);
   st.s = warp_sum(st.s);
   st.e = warp_sum(st.e);
   if (lane == 0) st_s[warp] = st;
-  ahead = __reduce_add_sync(0xffffffffu, ahead);
-  __syncthreads();                                                    // (rank_s is zero)
-  if (lane == 0 && ahead) atomicAdd(&rank_s, ahead);
-  if (tid == 0) {
-    for (int w = 1; w < WARPS; ++w) st = merge(st, st_s[w]);
-    mine_s = st;
+  if (ranked) {
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (lane == 0 && ahead) atomicAdd(&rank_s, ahead);
   }
-  if (a.K > 0) keep_best<THREADS>(lp_list, n_s, a.K, best_s, &count_s);
+  __syncthreads();
+  const Stats none = {-INFINITY, 0.f, 0.f, 0.f};
+  if (warp == 0) {
+    st = join(lane < WARPS ? st_s[lane] : none);
+    if (lane == 0) mine_s = st;
+  }
   if (cluster > 1) cluster_sync_all();
   else __syncthreads();
   if (part == 0) {
-    st = mine_s;
-    ahead = rank_s;
-    for (int c = 1; c < cluster; ++c) {
-      const uint32_t at = of_rank(&mine_s, c);
-      const Stats other = {ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8), ld_cluster_f32(at + 12)};
-      st = merge(st, other);
-      ahead += __float_as_int(ld_cluster_f32(of_rank(&rank_s, c)));
+    // every warp for itself: the sums are needed by all that write
+    st = lane == 0 ? mine_s : none;
+    ahead = lane == 0 ? rank_s : 0;
+    if (lane > 0 && lane < cluster) {
+      const uint32_t at = of_rank(&mine_s, lane);
+      st = Stats{ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8), ld_cluster_f32(at + 12)};
+      ahead = __float_as_int(ld_cluster_f32(of_rank(&rank_s, lane)));
     }
+    if (a.K > 0 && cluster > 1) {                                     // every block's best behind this one's
+      const int n = cluster * a.K;
+      for (int i = a.K + tid; i < n; i += THREADS) list_s[i] = ld_cluster_key(of_rank(&best_s[i % a.K], i / a.K));
+    }
+    st = join(st);
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
     const bool proper = fabsf(st.m) < INFINITY;
     const float log_z = proper ? logf(st.n1) + log1pf(st.s / st.n1) : NAN;
     if (tid == 0) {
@@ -347,22 +384,12 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
       if (a.entropy) a.entropy[row] = log_z - st.e / (st.n1 + st.s);
     }
     if (a.K > 0) {
-      const int n = cluster * a.K;                                    // every block's best, in order
       if (cluster > 1) {
-        for (int i = tid; i < n - a.K; i += THREADS) lp_list[a.K + i] = ld_cluster_key(of_rank(&best_s[i % a.K], 1 + i / a.K));
         __syncthreads();
-        // (zeros, of blocks with fewer than K elements, have the same place, behind the row's K and more keys)
-        for (int i = tid; i < n; i += THREADS) {
-          const Key k = lp_list[i];
-          int place = 0;
-          for (int j = 0; j < n; ++j) place += lp_list[j] > k;
-          if (place < a.K) {
-            a.top_ids[(long long)row * a.K + place] = id_of(k);
-            a.top_logprobs[(long long)row * a.K + place] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
-          }
-        }
-      } else if (tid < a.K) {
-        const Key k = lp_list[tid];
+        keep_best<THREADS>(list_s, cluster * a.K, a.K, best_s);
+      }
+      if (tid < a.K) {
+        const Key k = best_s[tid];
         a.top_ids[(long long)row * a.K + tid] = id_of(k);
         a.top_logprobs[(long long)row * a.K + tid] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
       }
@@ -373,22 +400,13 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
 
 template <typename T, int THREADS>
 int launch_logprobs(const LpArgs& a, unsigned cluster, cudaStream_t s) {
-  const size_t smem = a.K > 0 ? (size_t)(LP_LIST + THREADS * LP_E) * sizeof(Key) : 0;
-  if (smem > 48 * 1024) {
-    static bool attr_done = false;
-    if (!attr_done) {
-      NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (LP_LIST + THREADS * LP_E) * (int)sizeof(Key)));
-      attr_done = true;
-    }
-  }
-  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T, THREADS>, dim3(a.R * cluster), dim3(THREADS), smem, s, a));
+  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T, THREADS>, dim3(a.R * cluster), dim3(THREADS), 0, s, a));
   NV_RETURN_LAST();
 }
 
-// Blocks a row, and threads a block: a handful of rows takes large blocks, as many as a cluster has, of at least a tile each (a
-// row's latency is what counts); more rows take blocks of 256 threads, of which several live on a multiprocessor, in clusters until
-// there are enough for all multiprocessors.
+// Blocks a row, and threads a block: a handful of rows takes large blocks, as many as a cluster has, of at least a quarter of a
+// tile each (a row's latency is what counts); more rows take blocks of 256 threads, of which several live on a multiprocessor, in
+// clusters until there are enough for all multiprocessors.
 template <typename T>
 int run_logprobs(const LpArgs& a, cudaStream_t s) {
   const long long sms = num_multiprocessors();
