@@ -2,6 +2,9 @@
 //
 //   m = max x,  Z = sum e^(x - m),  logprob(t) = x_t - m - log Z,  entropy = log Z - sum e^(x - m) (x - m) / Z
 //
+// What bounds it: the logits, read once.  2,048 rows of 151,936 float32 take 204 us, 6.1 TB/s; a handful of rows takes the latency
+// of a launch, of two or three tiles and of a cluster's exchange (one row: 6 us above an empty kernel, with five alternatives 10).
+//
 // One pass keeps m, n1 (how many logits equal m), s (the sum of the others' e^(x - m)) and e (the sum of e^(x - m) (x - m)):
 // log Z = log n1 + log1p(s / n1).  The largest term is never added to the small ones, so the logarithm of an all but certain
 // token's probability, -s, keeps its bits instead of being what 1 + s rounds to.
@@ -10,6 +13,8 @@
 // comes after everything else.  A row that holds a NaN or plus infinity, or nothing above minus infinity, has no softmax: its
 // numbers are NaN, its order is defined all the same.
 #include "common.cuh"
+
+#include <cfloat>
 
 namespace {
 
@@ -32,6 +37,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {       // (fmaxf dro
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+__device__ __forceinline__ unsigned long long pair_of(float2 v) { return *(unsigned long long*)&v; }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return *(float2*)&r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return *(float2*)&r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
+  return *(float2*)&r;
 }
 
 struct Stats {
@@ -62,26 +84,26 @@ struct LpArgs {
   int R, V, K;
 };
 
-constexpr int LP_E = 16;               // elements a thread takes at a time: four (bfloat16: two) 16-byte loads under way
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int LP_E = 16;               // elements a thread takes at a time: four (bfloat16: two) 16-byte pieces
+constexpr int LP_STAGES = 4;           // tiles under way: a thread copies its own pieces into shared memory, three tiles ahead
 constexpr int LP_LIST = 1024;          // candidates a block has room for (and at least 512 beside a bound that a tile may bring)
 constexpr int LP_LONG = 256;           // ... and from how many on they are thinned out to the best K
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <typename T>
-struct Vec;                            // a 16-byte load as floats
+struct Vec;                            // a 16-byte piece as floats
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const float* p, float* x) {
-    const float4 v = __ldg((const float4*)p);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  static __device__ __forceinline__ void read(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
   }
 };
 template <>
 struct Vec<bf16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const bf16* p, float* x) {
-    const uint4 v = __ldg((const uint4*)p);
+  static __device__ __forceinline__ void read(const uint4& v, float* x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -117,7 +139,6 @@ __device__ __forceinline__ Key ld_cluster_key(uint32_t a) {
 
 // The K largest of the n keys in list[] come to its front and to best[], in descending order (fewer keys: zeros behind them); every
 // thread of the block calls, between two barriers.  A key's place is the number of larger ones.
-template <int THREADS>
 __device__ void keep_best(Key* list, int n, int K, Key* best) {
   const int tid = threadIdx.x;
   if (tid < K) best[tid] = 0;
@@ -142,7 +163,7 @@ __device__ void keep_best(Key* list, int n, int K, Key* best) {
 
 // One after the other in runs of a warp's width, whatever the logits are: for rows whose bound let too many candidates through
 // (rising ones) or too few (fewer than K logits above minus infinity).
-template <typename T, int THREADS>
+template <typename T>
 __device__ void collect_slowly(const T* x, int i0, int i1, int K, Key* list, Key* best, int* n_s) {
   constexpr int RUN = THREADS < LP_LIST - LP_LONG ? THREADS : LP_LIST - LP_LONG;
   Key bound = 0;
@@ -157,7 +178,7 @@ __device__ void collect_slowly(const T* x, int i0, int i1, int K, Key* list, Key
     __syncthreads();
     const int n = *n_s;
     if (n > LP_LONG) {
-      keep_best<THREADS>(list, n, K, best);
+      keep_best(list, n, K, best);
       bound = list[K - 1];
       if (threadIdx.x == 0) *n_s = K;
     }
@@ -167,12 +188,13 @@ __device__ void collect_slowly(const T* x, int i0, int i1, int K, Key* list, Key
 
 // A cluster of blocks takes a row, each block a run of its 16-byte pieces; a warp has a maximum, its threads their sums, which are
 // rescaled when it moves.  Alternatives: the first tile gives a bound that at least K of its logits reach (the K-th largest among
-// every full warp's few largest thread maxima), what lies above it goes into a list, and a list that has grown long is thinned
-// out, which raises the bound: a tile adds some K candidates and fewer and fewer, whatever the row's length.  The first block of
+// every full warp's few largest thread maxima), what lies above it goes into a list, and behind 2, 4, 8 ... tiles the list is thinned
+// out to its K best, which raises the bound.  The first block of
 // the cluster joins the sums and lists.
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
-  constexpr int WARPS = THREADS / 32, N = Vec<T>::N, NV = LP_E / N, TILE = THREADS * NV;      // (a tile in pieces)
+template <typename T>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprobs_kernel(LpArgs a) {
+  constexpr int N = Vec<T>::N, NV = LP_E / N, TILE = THREADS * NV;     // (a tile in pieces)
+  extern __shared__ __align__(16) uint4 ring[];                       // [LP_STAGES][NV][THREADS]
   __shared__ Key list_s[LP_LIST];
   __shared__ Key best_s[32];
   __shared__ Stats st_s[WARPS], mine_s;
@@ -184,15 +206,6 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
   grid_dep_wait();
   grid_dep_launch();
   const T* x = (const T*)a.logits + (long long)row * a.stride;
-  const int token = a.tokens ? a.tokens[row] : -1;
-  const bool known = token >= 0 && token < a.V;
-  const float xt = known ? to_f32(x[token]) : 0.f;
-  // places are found by comparing numbers, those of a NaN or minus infinity by keys; the next number below xt
-  const bool by_key = !(xt > -INFINITY);
-  const uint32_t xt_order = order_of(xt);
-  const float xt_below = below_of(xt_order);
-  const bool ranked = known && a.rank;
-
   const int off = (int)(((uintptr_t)x / sizeof(T)) % N);              // elements between the 16-byte boundary below and the row
   const int pieces = (int)(((long long)a.V + off + N - 1) / N), per = (pieces + cluster - 1) / cluster;
   const int q0 = min(pieces, part * per), q1 = min(pieces, q0 + per);
@@ -201,73 +214,63 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
   int ahead = 0, tile = 0;
   float above = -INFINITY;                                            // candidates are above it
   bool bounded = false, lost = false;
-  for (int q = q0; q < q1; q += TILE, ++tile) {
-    float v[LP_E];
-    if (q * N >= off && q + TILE <= q1 && (long long)(q + TILE) * N - off <= a.V) {
-      const T* from = x + ((long long)(q + tid) * N - off);
+  auto fetch = [&](int t) {                                            // tile t's whole pieces
+    const int q = q0 + t * TILE;
+    uint4* to = ring + (t % LP_STAGES) * TILE + tid;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) Vec<T>::load(from + j * (THREADS * N), v + j * N);
-    } else {
+    for (int j = 0; j < NV; ++j) {
+      const int p = q + j * THREADS + tid, i0 = p * N - off;
+      if (p < q1 && i0 >= 0 && i0 + N <= a.V)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to + j * THREADS)), "l"(x + i0) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < LP_STAGES - 1; ++t) fetch(t);
+  const int token = a.tokens ? a.tokens[row] : -1;
+  const bool known = token >= 0 && token < a.V;
+  const float xt = known ? to_f32(x[token]) : 0.f;
+  // places are found by comparing numbers, those of a NaN or minus infinity by keys; the next number below xt
+  const bool by_key = !(xt > -INFINITY);
+  const uint32_t xt_order = order_of(xt);
+  const float xt_below = below_of(xt_order);
+  const bool ranked = known && a.rank;
+  for (int q = q0; q < q1; q += TILE, ++tile) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LP_STAGES - 2) : "memory");
+    float v[LP_E];
+    const uint4* from = ring + (tile % LP_STAGES) * TILE + tid;
+    const bool whole = q * N >= off && q + TILE <= q1 && (long long)(q + TILE) * N - off <= a.V;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) Vec<T>::read(from[j * THREADS], v + j * N);
+    if (!whole) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int p = q + j * THREADS + tid, i0 = p * N - off;
-        if (p < q1 && i0 >= 0 && i0 + N <= a.V) {
-          Vec<T>::load(x + i0, v + j * N);
-        } else {
+        if (!(p < q1 && i0 >= 0 && i0 + N <= a.V)) {                  // a piece that the row covers a part of, or nothing
 #pragma unroll
           for (int u = 0; u < N; ++u) v[j * N + u] = (p < q1 && i0 + u >= 0 && i0 + u < a.V) ? to_f32(x[i0 + u]) : -INFINITY;
         }
       }
     }
+    fetch(tile + LP_STAGES - 1);                                      // (into the stage that was read a tile ago)
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < LP_E; ++i) mx = fmaxf(mx, v[i]);
-    // all threads of a warp keep their sums against one m, and a tile that does not reach it (most of them) takes the short way,
-    // where no term is the largest
     const uint32_t top = order_of(mx), tile_top = __reduce_max_sync(0xffffffffu, top);
-    if (tile_top >= m_order) {
-      if (tile_top > m_order) {
-        m_order = tile_top;
-        const float m = float_of(tile_top), d = st.m - m, c = ex2_fast(d * LOG2E), all = st.n1 + st.s;
-        st.e = c > 0.f ? c * fmaf(d, all, st.e) : 0.f;
-        st.s = c * all;                                               // (zero where nothing was there; a NaN stays)
-        st.n1 = 0.f;
-        st.m = m;
-      }
-      if (st.m > -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < LP_E; ++i) {
-          const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * LOG2E), other = d == 0.f ? 0.f : e;
-          st.s += other;
-          st.n1 += e - other;                                         // (2^0 is one)
-          st.e = fmaf(e, d, st.e);
-        }
-      } else {                                                        // nothing but NaN and minus infinity so far
-#pragma unroll
-        for (int i = 0; i < LP_E; ++i)
-          if (v[i] != v[i]) st.s = NAN;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < LP_E; ++i) {
-        const float d = max_nan(v[i] - st.m, -150.f), e = ex2_fast(d * LOG2E);
-        st.s += e;
-        st.e = fmaf(e, d, st.e);
-      }
-    }
     if (ranked && (by_key || tile_top >= xt_order)) {                  // (else nothing of the tile is ahead of the token)
+      const int lowest = q * N - off;
+      if (by_key || (lowest <= token && lowest + TILE * N > token)) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int p = q + j * THREADS + tid, i0 = p * N - off;
-        if (by_key || (i0 <= token && i0 + N > token)) {
+        for (int j = 0; j < NV; ++j) {
+          const int p = q + j * THREADS + tid, i0 = p * N - off;
 #pragma unroll
           for (int u = 0; u < N; ++u)
             ahead += i0 + u >= 0 && i0 + u < a.V && p < q1 && key_of(v[j * N + u], i0 + u) > key_of(xt, token);
-        } else {
-          const float over = i0 < token ? xt_below : xt;              // equal logits of lower ids are ahead
-#pragma unroll
-          for (int u = 0; u < N; ++u) ahead += v[j * N + u] > over;
         }
+      } else {
+        const float over = lowest < token ? xt_below : xt;            // equal logits of lower ids are ahead
+#pragma unroll
+        for (int i = 0; i < LP_E; ++i) ahead += v[i] > over;
       }
     }
     if (a.K > 0 && !lost) {
@@ -299,34 +302,22 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
         __syncthreads();
       }
       if (float_of(tile_top) > above) {
-        uint32_t mine = 0;                                            // a bit for each of this thread's candidates
-#pragma unroll
-        for (int i = 0; i < LP_E; ++i) mine |= (v[i] > above ? 1u : 0u) << i;
-        int at = __popc(mine);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int before = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += before;
-        }
-        int base = 0;
-        if (lane == 31) base = atomicAdd(&n_s, at);
-        at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
-        if (mine) {
+        if (mx > above) {
 #pragma unroll
           for (int i = 0; i < LP_E; ++i)
-            if (mine >> i & 1u) {
+            if (v[i] > above) {
+              const int at = atomicAdd(&n_s, 1);
               if (at < LP_LIST) list_s[at] = key_of(v[i], (q + i / N * THREADS + tid) * N - off + i % N);
-              ++at;
             }
         }
       }
-      if (tile % 8 == 7) {
+      if (tile > 0 && (tile & (tile + 1)) == 0) {                     // behind 2, 4, 8 ... tiles: as many again add some K
         __syncthreads();
         const int n = n_s;
         __syncthreads();
         lost = n > LP_LIST;                                           // (collected again at the end)
-        if (n > LP_LONG && !lost) {
-          keep_best<THREADS>(list_s, n, a.K, best_s);
+        if (n > a.K && !lost) {
+          keep_best(list_s, n, a.K, best_s);
           above = float_of((uint32_t)(list_s[a.K - 1] >> 32));        // (equal logits from here on have higher ids)
           bounded = true;
           if (tid == 0) n_s = a.K;
@@ -334,13 +325,44 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
         }
       }
     }
+    // all threads of a warp keep their sums against one m; most tiles do not reach it
+    if (tile_top >= m_order) {
+      if (tile_top > m_order) {
+        m_order = tile_top;
+        const float m = float_of(tile_top), d = st.m - m, c = ex2_fast(d * LOG2E), all = st.n1 + st.s;
+        st.e = c > 0.f ? c * fmaf(d, all, st.e) : 0.f;
+        st.s = c * all;                                               // (zero where nothing was there; a NaN stays)
+        st.n1 = 0.f;
+        st.m = m;
+      }
+#pragma unroll
+      for (int i = 0; i < LP_E; ++i) {                                // the largest are counted and leave the sums
+        const bool largest = v[i] == st.m;
+        st.n1 += largest ? 1.f : 0.f;
+        v[i] = largest ? -INFINITY : v[i];
+      }
+    }
+    const float m = fmaxf(st.m, -FLT_MAX);                            // (nothing but NaN and minus infinity so far)
+    float2 sum = make_float2(st.s, 0.f), by = make_float2(st.e, 0.f);
+    const float2 m2 = make_float2(-m, -m), scale = make_float2(LOG2E, LOG2E);
+#pragma unroll
+    for (int i = 0; i < LP_E; i += 2) {                               // two elements an instruction
+      float2 d = add2(make_float2(v[i], v[i + 1]), m2);
+      d.x = max_nan(d.x, -150.f);
+      d.y = max_nan(d.y, -150.f);
+      const float2 t = mul2(d, scale), e = make_float2(ex2_fast(t.x), ex2_fast(t.y));
+      sum = add2(sum, e);
+      by = fma2(e, d, by);
+    }
+    st.s = sum.x + sum.y;
+    st.e = by.x + by.y;
   }
   const int first = max(0, q0 * N - off), last = min(a.V, q1 * N - off);          // this block's elements
   if (a.K > 0) {
     __syncthreads();
     const int n = n_s;
-    if (n > LP_LIST || n < min(a.K, last - first)) collect_slowly<T, THREADS>(x, first, last, a.K, list_s, best_s, &n_s);
-    keep_best<THREADS>(list_s, n_s, a.K, best_s);
+    if (n > LP_LIST || n < min(a.K, last - first)) collect_slowly<T>(x, first, last, a.K, list_s, best_s, &n_s);
+    keep_best(list_s, n_s, a.K, best_s);
   }
   st.n1 = warp_sum(st.n1);
   st.s = warp_sum(st.s);
@@ -386,7 +408,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
     if (a.K > 0) {
       if (cluster > 1) {
         __syncthreads();
-        keep_best<THREADS>(list_s, cluster * a.K, a.K, best_s);
+        keep_best(list_s, cluster * a.K, a.K, best_s);
       }
       if (tid < a.K) {
         const Key k = best_s[tid];
@@ -398,26 +420,23 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LpArgs a) {
   if (cluster > 1) cluster_sync_all();                                // nobody leaves while its lists are read
 }
 
-template <typename T, int THREADS>
-int launch_logprobs(const LpArgs& a, unsigned cluster, cudaStream_t s) {
-  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T, THREADS>, dim3(a.R * cluster), dim3(THREADS), 0, s, a));
-  NV_RETURN_LAST();
-}
-
-// Blocks a row, and threads a block: a handful of rows takes large blocks, as many as a cluster has, of at least a quarter of a
-// tile each (a row's latency is what counts); more rows take blocks of 256 threads, of which several live on a multiprocessor, in
-// clusters until there are enough for all multiprocessors.
+// Blocks a row: a cluster of them while that leaves two or so a multiprocessor, each with a tile at least.  One row of 151,936 logits,
+// five alternatives, on 1 / 2 / 4 / 8 / 16 blocks: 38 / 27 / 21 / 18 / 16 us (with an event's 6); 16 rows 37 / 29 / 23 / 21 / 21; 64
+// rows, twenty: 45 / 33 / 31 / 43 / 76; 150 rows, five: 45 / 39 / 49; 512: 97 / 92 / 117; 2,048: 244 / 291.
 template <typename T>
 int run_logprobs(const LpArgs& a, cudaStream_t s) {
-  const long long sms = num_multiprocessors();
-  if (a.R * 8LL <= sms) {
-    unsigned cluster = 8;
-    while (cluster > 1 && a.V / (int)cluster < 1024 * LP_E / 4) cluster /= 2;
-    return launch_logprobs<T, 1024>(a, cluster, s);
+  constexpr size_t smem = (size_t)LP_STAGES * THREADS * LP_E * sizeof(T);
+  static bool attr_done = false;
+  if (!attr_done) {
+    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    attr_done = true;
   }
+  const long long sms = num_multiprocessors();
   unsigned cluster = 1;
-  while (cluster < 8 && a.R * (long long)cluster < 4 * sms && a.V / (int)(2 * cluster) >= 256 * LP_E) cluster *= 2;
-  return launch_logprobs<T, 256>(a, cluster, s);
+  while (cluster < 16 && a.R * (long long)cluster * 8 <= sms * 9 && a.V / (int)(2 * cluster) >= THREADS * LP_E) cluster *= 2;
+  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T>, dim3(a.R * cluster), dim3(THREADS), smem, s, a));
+  NV_RETURN_LAST();
 }
 
 }  // namespace
