@@ -9,7 +9,7 @@
 // row: per kv head it is a matrix product of the (row, query head) pairs that read it.  Three launches: the shared parts (here),
 // every row's own keys, from the page on that holds position len[g] (the split-key kernel of attention_decode.cu), and their join (here).  A row that
 // belongs to no group has no shared part; of a group's keys a row sees those up to its own position.
-#include "pipeline.cuh"
+#include "tcgen05.cuh"
 
 int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                              const int* block_table, int max_blocks, const int* row_entry, const int* positions, const int* rows,
@@ -170,6 +170,309 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
   }
 }
 
+// The tensor-core form, for bfloat16 and head sizes in steps of 16 from 32 on: a CTA takes 128 pairs of one kv head and one split
+// of the keys, 64 keys at a time.  S = Q K^T and O += P V are tcgen05.mma with S (two buffers) and O in tensor memory:
+//   warp 0     fetches the pages of K (two buffers) and V as TMA boxes of one page x 64 elements, a lane a box
+//   warp 1     allocates tensor memory; one thread issues the products
+//   warps 2-5  gather the queries of the tile's pairs into shared memory (128-byte swizzle), then a thread owns a pair: it reads its
+//              row of S, keeps its maximum and sum, writes P as bfloat16 into shared memory, and at the end its row of O, undivided,
+//              with maximum and sum to the scratch
+// All keys of a split are seen by all pairs, but for those behind a row's own position, so there is no mask in most blocks.  TERMS =
+// 3: the float32 weights enter the product with the values as three bfloat16 terms (all their bits) instead of one rounded.
+// Heads between the forms' sizes: the boxes reach beyond the pages' rows and are filled with zeros.
+constexpr int ST_PAIRS = 128, ST_KEYS = 64, ST_THREADS = 192;
+constexpr int ST_PAGES = 1024;           // block-table entries of a split kept in shared memory
+
+template <int D>
+constexpr int st_tmem_cols() { return 2 * ST_KEYS + D <= 256 ? 256 : 512; }
+
+template <int D, int TERMS>
+__global__ void __launch_bounds__(ST_THREADS, D <= 128 ? 2 : 1)
+shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, SharedArgs a, ScoreMap map) {
+  constexpr int SL = D / 64;
+  constexpr uint32_t Q_SLAB = ST_PAIRS * 128, KV_SLAB = ST_KEYS * 128, P_TILE = ST_PAIRS * 128;
+  extern __shared__ __align__(1024) uint8_t st_smem_raw[];
+  __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full, pv_done;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int2 tile_s;
+  __shared__ int bt_s[ST_PAGES];
+
+  uint8_t* smem = (uint8_t*)(((uintptr_t)st_smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* Qs = smem;
+  uint8_t* Ks = Qs + SL * Q_SLAB;                  // two buffers
+  uint8_t* Vs = Ks + 2 * SL * KV_SLAB;
+  uint8_t* Ps = Vs + SL * KV_SLAB;                 // TERMS tiles of [128 pairs][64 keys]
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int kvh = blockIdx.y, split = blockIdx.z, G = a.Hq / a.Hkv;
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tm_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&tm_v) : "memory");
+    mbar_init(&q_full, 4);                         // one arrival per softmax warp
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&k_full[b], 1);
+      mbar_init(&k_empty[b], 1);
+      mbar_init(&s_full[b], 1);
+    }
+    mbar_init(&v_full, 1);
+    mbar_init(&v_empty, 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&pv_done, 1);
+    mbar_fence_init();
+  }
+  // keys of a block that are not loaded (behind the split's end) must be finite numbers: their weights are zero
+  for (int i = tid; i < (int)(3 * SL * KV_SLAB / 16); i += ST_THREADS) ((uint4*)Ks)[i] = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  if (warp == 1) tmem_alloc(&tmem_base_s, st_tmem_cols<D>());
+  grid_dep_wait();
+  grid_dep_launch();
+  if (tid == 0) tile_s = find_tile(a, blockIdx.x, G, ST_PAIRS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+  const int g = tile_s.x, pair0 = tile_s.y;
+  if (g >= 0) {
+    const int m0 = a.cu[g], pairs = min(ST_PAIRS, (a.cu[g + 1] - m0) * G - pair0), len = a.len[g] / a.page * a.page;
+    const int share = max(a.split_keys, ((len + a.splits - 1) / a.splits + ST_KEYS - 1) / ST_KEYS * ST_KEYS);
+    const int j_lo = min(len, split * share), j_hi = min(len, j_lo + share);
+    const int n_blocks = (j_hi - j_lo + ST_KEYS - 1) / ST_KEYS;
+    const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 2 * ST_KEYS;
+    const int lead = a.members[m0], lead_t = a.rows ? a.rows[lead] : lead;
+    const int* bt = a.block_table + (long long)a.row_entry[lead_t] * a.max_blocks;
+    const int page_shift = 31 - __clz(a.page);     // pages are 16, 32 or 64 keys
+    const int pg0 = j_lo >> page_shift, n_pg = min((j_hi - j_lo) >> page_shift, ST_PAGES);
+    for (int i = tid; i < n_pg; i += ST_THREADS) bt_s[i] = bt[pg0 + i];
+    __syncthreads();
+
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      const int pages = ST_KEYS >> page_shift;
+      const uint32_t box = (uint32_t)a.page * 128;
+      const int my_p = lane / SL, my_s = lane % SL;
+      auto load = [&](int i, bool values) {
+        const int j = j_lo + i * ST_KEYS + (my_p << page_shift);
+        int blk = -1;
+        if (my_p < pages && j < j_hi) {
+          const int pi = (j >> page_shift) - pg0;
+          blk = pi < ST_PAGES ? bt_s[pi] : bt[pg0 + pi];
+          if (blk < 0 || blk >= a.num_pages) {                           // it should be there and is not
+            atomicExch(a.err, 1 + lead_t);
+            blk = -1;
+          }
+        }
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, blk >= 0));
+        uint64_t* full = values ? &v_full : &k_full[i & 1];
+        if (lane == 0) {
+          if (values) mbar_wait(&v_empty, (i & 1) ^ 1, a.err, 0x7302);
+          else mbar_wait(&k_empty[i & 1], ((i >> 1) & 1) ^ 1, a.err, 0x7301);
+          mbar_expect_tx(full, boxes * box);
+        }
+        __syncwarp();
+        if (blk >= 0) {
+          uint8_t* dst = (values ? Vs : Ks + (i & 1) * SL * KV_SLAB) + my_s * KV_SLAB + my_p * box;
+          tma_load_2d(dst, values ? &tm_v : &tm_k, full, my_s * 64, (blk * a.Hkv + kvh) * a.page);
+        }
+      };
+      if (n_blocks > 0) load(0, false);
+      for (int i = 0; i < n_blocks; ++i) {         // the next keys go out before these values: they are free earlier
+        if (i + 1 < n_blocks) load(i + 1, false);
+        load(i, true);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (lane == 0 && n_blocks > 0) {
+        const uint32_t idesc_s = instr_desc(ST_KEYS), idesc_o = instr_desc_b_mn(D);
+        const uint32_t q_addr = smem_u32(Qs), k_addr = smem_u32(Ks), v_addr = smem_u32(Vs), p_addr = smem_u32(Ps);
+        uint64_t dq[SL], dk[2][SL], dp[TERMS];
+#pragma unroll
+        for (int s = 0; s < SL; ++s) {
+          dq[s] = smem_desc_sw128(q_addr + s * Q_SLAB);
+          dk[0][s] = smem_desc_sw128(k_addr + s * KV_SLAB);
+          dk[1][s] = smem_desc_sw128(k_addr + (SL + s) * KV_SLAB);
+        }
+        const uint64_t dv = smem_desc_sw128_mn(v_addr, KV_SLAB, 1024);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) dp[t] = smem_desc_sw128(p_addr + t * P_TILE);
+        auto issue_s = [&](int i) {
+          const int b = i & 1;
+          mbar_wait(&k_full[b], (i >> 1) & 1, a.err, 0x7303);
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < SL; ++s)
+            umma_bf16_x4(tmem_s + b * ST_KEYS, dq[s], b ? dk[1][s] : dk[0][s], idesc_s, s ? 1u : 0u);
+          umma_commit(&k_empty[b]);
+          umma_commit(&s_full[b]);
+        };
+        mbar_wait(&q_full, 0, a.err, 0x7304);
+        tc_fence_after();
+        issue_s(0);
+        if (n_blocks > 1) issue_s(1);
+        for (int i = 0; i < n_blocks; ++i) {
+          mbar_wait(&p_full, i & 1, a.err, 0x7305);  // P(i) is written, S(i) is read, O is rescaled
+          mbar_wait(&v_full, i & 1, a.err, 0x7306);
+          tc_fence_after();
+          // 16 keys per product: 32 bytes (2 units) along P's rows, two 8-key groups (2,048 bytes = 128 units) of V
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) umma_bf16_x4s(tmem_o, dp[t], dv, idesc_o, (i || t) ? 1u : 0u, 2, 128);
+          umma_commit(&v_empty);
+          umma_commit(&pv_done);
+          if (i + 2 < n_blocks) issue_s(i + 2);      // into the buffer that S(i) has left
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------- a thread a pair
+      const int q = warp % 4;                        // a warp may touch tensor-memory lanes [32q, 32q + 32) only
+      const int p = q * 32 + lane;
+      const bool live = p < pairs, some = q * 32 < pairs;       // (a warp without pairs only arrives where it is waited for)
+      const int r = live ? a.members[m0 + (pair0 + p) / G] : lead, h = kvh * G + (live ? (pair0 + p) % G : 0);
+      const int t = a.rows ? a.rows[r] : r;
+      const int limit = live ? min(j_hi, a.positions[t] + 1) : j_hi;            // the first key that this row does not see
+      const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+      {
+        // the warp's 32 queries, row by row (the lanes side by side), rows of nobody and columns beyond the head as zeros
+        for (int i = 0; i < 32; ++i) {
+          const int rt = __shfl_sync(0xffffffffu, t, i), rh = __shfl_sync(0xffffffffu, h, i);
+          const bool there = q * 32 + i < pairs;
+          const bf16* from = (const bf16*)a.q + (size_t)rt * a.q_stride + (size_t)rh * a.D;
+          for (int c = lane; c < D / 8; c += 32) {
+            const uint4 v = there && c * 8 < a.D ? *(const uint4*)(from + c * 8) : make_uint4(0, 0, 0, 0);
+            const int row = q * 32 + i;
+            *(uint4*)(Qs + (c / 8) * Q_SLAB + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v;
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < n_blocks; ++i) {
+        const int j0 = j_lo + i * ST_KEYS;
+        mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.err, 0x7307);
+        float s[ST_KEYS];
+        float mx = -INFINITY;
+        if (some) {
+          tc_fence_after();
+          tmem_ld32_nowait(tmem_s + (i & 1) * ST_KEYS + lane_off, s);
+          tmem_ld32_nowait(tmem_s + (i & 1) * ST_KEYS + lane_off + 32, s + 32);
+          tmem_ld_wait();
+          tmem_ld_fence<64>(s);
+          if (map.cap1 > 0.f) {
+#pragma unroll
+            for (int c = 0; c < ST_KEYS; ++c) s[c] = capped_log2(map, s[c]);
+          }
+          if (j0 + ST_KEYS > limit) {
+#pragma unroll
+            for (int c = 0; c < ST_KEYS; ++c)
+              if (j0 + c >= limit) s[c] = -INFINITY;
+          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < ST_KEYS; c += 4) {
+            mx4[0] = fmaxf(mx4[0], s[c]); mx4[1] = fmaxf(mx4[1], s[c + 1]);
+            mx4[2] = fmaxf(mx4[2], s[c + 2]); mx4[3] = fmaxf(mx4[3], s[c + 3]);
+          }
+          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        }
+        // O += P(i-1) V(i-1) must have ended before O is rescaled and P is overwritten (a warp without pairs waits too: its
+        // arrival is one for this block)
+        if (i > 0) {
+          mbar_wait(&pv_done, (i - 1) & 1, a.err, 0x7309);
+          tc_fence_after();
+        }
+        if (some) {
+          // the exponent's reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost
+          // bfloat16 and the float32 sums nothing), so that O is rescaled once in a long while
+          float alpha = 1.f;
+          if (mx > m && (m == -INFINITY || (mx - m) * map.in > 8.f)) {
+            alpha = m == -INFINITY ? 0.f : ex2_fast((m - mx) * map.in);
+            m = mx;
+          }
+          const float ms = m == -INFINITY ? 0.f : m * map.in;
+          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32(tmem_o + lane_off + c * 32, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= alpha;
+              tmem_st32(tmem_o + lane_off + c * 32, o);
+            }
+          }
+          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < ST_KEYS; c += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              s[c + u] = ex2_fast(fmaf(s[c + u], map.in, -ms));
+              sum4[u] += s[c + u];
+            }
+          }
+          l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+          uint8_t* prow = Ps + (size_t)p * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) w[u] = s[c * 8 + u];
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) {
+              __nv_bfloat162 b[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) b[u] = __floats2bfloat162_rn(w[2 * u], w[2 * u + 1]);
+              *(uint4*)(prow + x * P_TILE + ((c ^ (p & 7)) << 4)) = *(uint4*)b;
+              if (x + 1 < TERMS) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  const float2 f = __bfloat1622float2(b[u]);
+                  w[2 * u] -= f.x;
+                  w[2 * u + 1] -= f.y;
+                }
+              }
+            }
+          }
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full);
+      }
+      // ---- this split's part: O as it is, relative to m
+      if (n_blocks > 0) {
+        mbar_wait(&pv_done, (n_blocks - 1) & 1, a.err, 0x7308);
+        tc_fence_after();
+      }
+      if (some) {
+        const size_t at = ((size_t)r * a.Hq + h) * a.slots + a.slot0 + split;
+        if (live) {
+          // (m is in the units of the raw or the capped scores: map.in takes it to base 2)
+          a.part_ml[at * 2] = m == -INFINITY ? -1e30f : m * map.in * 0.6931471805599453f;
+          a.part_ml[at * 2 + 1] = l;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (n_blocks > 0) {
+            tmem_ld32(tmem_o + lane_off + c * 32, o);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+          }
+          if (live) {
+            float* dst = a.part_o + at * a.D + c * 32;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (c * 32 + j < a.D) *(float4*)(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, st_tmem_cols<D>());
+}
+
 // The parts of one (row, head), in the order of their slots: its own keys' splits, then the shared ones'.
 __global__ void __launch_bounds__(128) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                           const int* __restrict__ rows, const int* __restrict__ group, void* out,
@@ -204,15 +507,48 @@ int launch_plain(const SharedArgs& a, int tiles, cudaStream_t s) {
   NV_RETURN_LAST();
 }
 
+template <int D, int TERMS>
+int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
+  CUtensorMap tm_k, tm_v;
+  const long long rows = (long long)a.num_pages * a.Hkv * a.page;
+  int rc = nv_tensor_map_bf16(a.kc, rows, a.D, a.D, a.page, &tm_k);
+  if (rc) return rc;
+  rc = nv_tensor_map_bf16(a.vc, rows, a.D, a.D, a.page, &tm_v);
+  if (rc) return rc;
+  constexpr int SL = D / 64;
+  constexpr size_t smem = (size_t)SL * ST_PAIRS * 128 + 3 * (size_t)SL * ST_KEYS * 128 + (size_t)TERMS * ST_PAIRS * 128 + 1024;
+  static bool attr_done = false;
+  if (!attr_done) {
+    NV_RETURN_IF(cudaFuncSetAttribute(shared_tc_kernel<D, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attr_done = true;
+  }
+  // scores go to base-2 units by map.in; capped ones are there already
+  ScoreMap map = score_map(a.scale, a.softcap);
+  if (a.softcap > 0.f) map.in = 1.f;
+  NV_RETURN_IF(launch_dep(shared_tc_kernel<D, TERMS>, dim3(tiles, a.Hkv, a.splits), dim3(ST_THREADS), smem, s, tm_k, tm_v, a, map));
+  NV_RETURN_LAST();
+}
+
+template <int TERMS>
+int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
+  return a.D <= 64 ? launch_tc<64, TERMS>(a, tiles, s) : a.D <= 128 ? launch_tc<128, TERMS>(a, tiles, s) : launch_tc<256, TERMS>(a, tiles, s);
+}
+
+// Whether the tensor-core form takes these sizes (and, with pointers, these addresses).
+bool tc_takes(int cache_dt, int D, int page) {
+  return cache_dt == NV_DT_BF16 && D >= 32 && D % 16 == 0 && (page == 16 || page == 32 || page == 64);
+}
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
 }  // namespace
 
 // Splits of the shared keys for M rows in `groups` groups whose longest prefix has `longest` positions.
-NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int longest) {
+NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
   if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
-  const int G = Hq / Hkv;
-  const long long tiles = ((long long)M * G + SP_PAIRS - 1) / SP_PAIRS + groups;
-  const long long blocks = tiles * Hkv, want = (4LL * num_multiprocessors() + blocks - 1) / blocks;
-  const long long most = (longest + 255) / 256;
+  const bool tc = tc_takes(cache_dt, D, page);
+  const int rows = tc ? ST_PAIRS : SP_PAIRS, each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4;
+  const long long tiles = ((long long)M * (Hq / Hkv) + rows - 1) / rows + groups - 1;
+  const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + 255) / 256;
   const long long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
@@ -235,7 +571,9 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   if (R == 0) return NV_OK;
   if (!scratch) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
-  const long long tiles = ((long long)M * (Hq / Hkv) + SP_PAIRS - 1) / SP_PAIRS + groups;
+  const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc) && aligned16(scratch);
+  const int per_tile = tc ? ST_PAIRS : SP_PAIRS;
+  const long long tiles = ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;         // (or fewer)
   if (shared_splits > 0 && groups > 0) {
     SharedArgs a;
     a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;
@@ -243,7 +581,8 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
     a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
     a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
     a.slots = slots; a.slot0 = own_splits; a.split_keys = 256;
-    const int rc = cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, (int)tiles, stream) : launch_plain<float>(a, (int)tiles, stream);
+    const int rc = tc ? ((float_weights || has_sink) ? launch_tc_d<3>(a, (int)tiles, stream) : launch_tc_d<1>(a, (int)tiles, stream))
+                   : cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, (int)tiles, stream) : launch_plain<float>(a, (int)tiles, stream);
     if (rc) return rc;
   }
   const int rc = nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,

@@ -517,7 +517,8 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
     L = lib()
     splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, max_context, num_sms())
-    ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, shared.longest)
+    ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache),
+                                        (1 if float_weights or sink_score is not None else 0), shared.longest)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
     _check(L.nv_attention_decode_shared(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table),
                                         block_table.shape[1], _p(row_entry), _p(positions), _p(rows), R, _p(shared.first),
