@@ -63,6 +63,9 @@ struct DecArgs {
   // hold for a (row, head)
   const int* first;
   int slots;
+  // REST: the kernel in front writes nothing that is read here, and waited itself for the kernel in front of it: this one runs
+  // beside it and waits for it where it ends, so that who waits for this kernel has waited for both
+  int beside;
   void* out;
   float* part_o;          // [rows, Hq, splits, D]
   float* part_ml;         // [rows, Hq, splits, 2]
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
     }
     mbar_fence_init();
   }
-  grid_dep_wait();              // the queries and the newest keys come from the kernel before
+  if (!REST || !a.beside) grid_dep_wait();      // the queries and the newest keys come from the kernel before
   grid_dep_launch();
   for (int i = threadIdx.x; i < ng * D; i += (WARPS + 1) * 32) {
     int g = i / D, d = i % D;
@@ -409,6 +412,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
     }
   }
   if (!REST && a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, D, (float*)dec_smem);
+  if (REST && a.beside) grid_dep_wait();
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -479,7 +483,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
   const int pb = p_lo + split * per;
   const int n_pages = max(0, min(p_hi, pb + per) - pb);
   if (n_pages == 0 && (REST || a.splits > 1)) {      // nothing for this split: say so and leave
-    grid_dep_wait();
+    if (!REST || !a.beside) grid_dep_wait();
     grid_dep_launch();
     for (int i = threadIdx.x; i < ng * a.D; i += (WARPS + 1) * 32) {
       const size_t pi = ((size_t)r * a.Hq + kvh * G + g0 + i / a.D) * (REST ? a.slots : a.splits) + split;
@@ -487,6 +491,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
       if (i % a.D == 0) { a.part_ml[pi * 2] = -1e30f; a.part_ml[pi * 2 + 1] = 0.f; }
     }
     if (!REST && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
+    if (REST && a.beside) grid_dep_wait();
     return;
   }
   const uint32_t box_bytes = (uint32_t)a.page * 128;           // one box: `page` keys x 64 elements
@@ -510,7 +515,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
   for (int i = threadIdx.x; i < min(n_pages, BT_CACHE); i += (WARPS + 1) * 32) bt_s[i] = bt[pb + i];
   __syncthreads();
   if (warp < WARPS) {
-    grid_dep_wait();
+    if (!REST || !a.beside) grid_dep_wait();
     grid_dep_launch();
     for (int i = threadIdx.x; i < TC_ROWS * D; i += WARPS * 32) {
       const int g = i / D, d = i % D;
@@ -529,7 +534,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
       const int newest = (n - 1) / a.page - pb;          // this split's page that is still being written
-      bool waited = false;
+      bool waited = REST && a.beside;
       int s = 0;                                   // stage of page i and the parity of its use, kept by counting
       uint32_t ph = 0;                             // (this one thread's instructions pace the ring)
       for (int i = 0; i < n_pages; ++i, s = (s + 1 == a.stages ? 0 : s + 1), ph ^= (s == 0)) {
@@ -766,6 +771,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
     }
   }
   if (!REST && a.splits > 1 && a.split_count) merge_when_last(a, r, t, kvh * G + g0, ng, a.D, (float*)dec_smem);
+  if (REST && a.beside) grid_dep_wait();
 }
 
 // Combines the splits of one (row, head) in split order.
@@ -926,7 +932,7 @@ int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const vo
                int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
                int* split_count, int split_count_len, int has_sink, float sink_score,
                int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
-               const float* slopes, const float* bias_table, int bias_len, const int* first, int slots, cudaStream_t stream) {
+               const float* slopes, const float* bias_table, int bias_len, const int* first, int slots, int beside, cudaStream_t stream) {
   // gate: head h's output of batch row t is multiplied by sigmoid(gate[t * gate_ld + h]) (nullptr: it is not); the
   // gates must have been written before the kernel that precedes this one on the stream.
   // softcap > 0: scaled scores are capped, s -> softcap * tanh(s / softcap).  chunk > 0: a row at position p sees the
@@ -953,7 +959,7 @@ int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const vo
   a.max_blocks = max_blocks; a.window = window; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.splits = splits;
   a.long_pages = 1; a.many_shares = 0x7fffffff; a.short_pages = a.mid_pages = 0;      // even shares
   a.part_o = scratch;
-  a.first = first; a.slots = slots;
+  a.first = first; a.slots = slots; a.beside = beside;
   a.part_ml = scratch ? scratch + (size_t)R * Hq * slots * D : nullptr;
   a.err = err;
   a.has_sink = has_sink; a.sink = sink_score;
@@ -1063,18 +1069,19 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
                                const float* slopes, const float* bias_table, int bias_len, cudaStream_t stream) {
   return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, window,
                     out, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, split_count, split_count_len, has_sink,
-                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, stream);
+                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, 0, stream);
 }
 
 // The keys from position first[r] on, as partial results (see decode_run): what attention over a shared prefix joins with it.
+// beside: the kernel in front works out the prefix (see DecArgs).
 int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                              const int* block_table, int max_blocks, const int* row_entry, const int* positions, const int* rows,
                              const int* first, int R, float scale, int out_dt, int Hq, int Hkv, int D, int page, int num_pages,
-                             int splits, int slots, float* scratch, int* err, int float_weights, float softcap, cudaStream_t stream) {
+                             int splits, int slots, float* scratch, int* err, int float_weights, float softcap, int beside, cudaStream_t stream) {
   if (!first) return NV_ERR_BAD_SIZE;
   return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, 0,
                     nullptr, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, nullptr, 0, 0, 0.f, float_weights, softcap,
-                    nullptr, 0, 0, nullptr, nullptr, 0, first, slots, stream);
+                    nullptr, 0, 0, nullptr, nullptr, 0, first, slots, beside, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

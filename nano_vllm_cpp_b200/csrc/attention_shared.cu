@@ -14,7 +14,7 @@
 int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                              const int* block_table, int max_blocks, const int* row_entry, const int* positions, const int* rows,
                              const int* first, int R, float scale, int out_dt, int Hq, int Hkv, int D, int page, int num_pages,
-                             int splits, int slots, float* scratch, int* err, int float_weights, float softcap, cudaStream_t stream);
+                             int splits, int slots, float* scratch, int* err, int float_weights, float softcap, int beside, cudaStream_t stream);
 
 namespace {
 
@@ -37,13 +37,24 @@ struct SharedArgs {
   int split_keys;           // a split has at least so many keys (a multiple of the page and of the kernel's block of keys)
 };
 
-// Which tile of `rows_per_tile` pairs of which group is tile number x?  Found by one thread; tile.x < 0: none (a launch has as many
-// tiles as there may be).
-__device__ __forceinline__ int2 find_tile(const SharedArgs& a, int x, int G, int rows_per_tile) {
-  for (int g = 0; g < a.groups; ++g) {
-    const int pairs = (a.cu[g + 1] - a.cu[g]) * G, tiles = (pairs + rows_per_tile - 1) / rows_per_tile;
-    if (x < tiles) return make_int2(g, x * rows_per_tile);
-    x -= tiles;
+// Which tile of `rows_per_tile` pairs of which group is tile number x?  A whole warp looks, 32 groups at a time; .x < 0: none (a
+// launch has as many tiles as there may be).
+__device__ __forceinline__ int2 find_tile(const SharedArgs& a, int x, int G, int rows_per_tile, int lane) {
+  for (int g0 = 0; g0 < a.groups; g0 += 32) {
+    const int g = g0 + lane;
+    const int tiles = g < a.groups ? ((a.cu[g + 1] - a.cu[g]) * G + rows_per_tile - 1) / rows_per_tile : 0;
+    int end = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += before;
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, x < end);
+    if (who) {
+      const int l = __ffs(who) - 1;
+      return make_int2(g0 + l, (x - __shfl_sync(0xffffffffu, end - tiles, l)) * rows_per_tile);
+    }
+    x -= __shfl_sync(0xffffffffu, end, 31);
   }
   return make_int2(-1, 0);
 }
@@ -63,7 +74,10 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, kvh = blockIdx.y, split = blockIdx.z, G = a.Hq / a.Hkv;
-  if (tid == 0) tile_s = find_tile(a, blockIdx.x, G, SP_PAIRS);
+  if (tid < 32) {
+    const int2 tile = find_tile(a, blockIdx.x, G, SP_PAIRS, tid);
+    if (tid == 0) tile_s = tile;
+  }
   __syncthreads();
   const int g = tile_s.x, pair0 = tile_s.y;
   if (g < 0) return;
@@ -226,7 +240,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 1) tmem_alloc(&tmem_base_s, st_tmem_cols<D>());
   grid_dep_wait();
   grid_dep_launch();
-  if (tid == 0) tile_s = find_tile(a, blockIdx.x, G, ST_PAIRS);
+  if (warp == 0) {
+    const int2 tile = find_tile(a, blockIdx.x, G, ST_PAIRS, lane);
+    if (lane == 0) tile_s = tile;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -330,15 +347,25 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int limit = live ? min(j_hi, a.positions[t] + 1) : j_hi;            // the first key that this row does not see
       const uint32_t lane_off = (uint32_t)(q * 32) << 16;
       {
-        // the warp's 32 queries, row by row (the lanes side by side), rows of nobody and columns beyond the head as zeros
-        for (int i = 0; i < 32; ++i) {
-          const int rt = __shfl_sync(0xffffffffu, t, i), rh = __shfl_sync(0xffffffffu, h, i);
-          const bool there = q * 32 + i < pairs;
-          const bf16* from = (const bf16*)a.q + (size_t)rt * a.q_stride + (size_t)rh * a.D;
-          for (int c = lane; c < D / 8; c += 32) {
-            const uint4 v = there && c * 8 < a.D ? *(const uint4*)(from + c * 8) : make_uint4(0, 0, 0, 0);
-            const int row = q * 32 + i;
-            *(uint4*)(Qs + (c / 8) * Q_SLAB + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v;
+        // the warp's 32 queries, D / 8 lanes a row and eight loads of a lane under way; rows of nobody and columns beyond the head
+        // are zeros
+        constexpr int PER = D / 8, AT_ONCE = 32 / PER;              // (PER is 8, 16 or 32)
+        const int c = lane % PER;
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += 8 * AT_ONCE) {
+          uint4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int i = (i0 + u * AT_ONCE + lane / PER) % 32;
+            const int rt = __shfl_sync(0xffffffffu, t, i), rh = __shfl_sync(0xffffffffu, h, i);
+            v[u] = q * 32 + i < pairs && c * 8 < a.D
+                       ? *(const uint4*)((const bf16*)a.q + (size_t)rt * a.q_stride + (size_t)rh * a.D + c * 8)
+                       : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int row = q * 32 + (i0 + u * AT_ONCE + lane / PER) % 32;
+            *(uint4*)(Qs + (c / 8) * Q_SLAB + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[u];
           }
         }
         fence_async_smem();
@@ -473,25 +500,44 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem_base, st_tmem_cols<D>());
 }
 
-// The parts of one (row, head), in the order of their slots: its own keys' splits, then the shared ones'.
+// The parts of one (row, head), in the order of their slots: its own keys' splits, then the shared ones'.  A warp works out what
+// the parts weigh, then every thread adds its elements up, eight loads at a time.
+constexpr int MAX_PARTS = 64;
+
 __global__ void __launch_bounds__(128) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                           const int* __restrict__ rows, const int* __restrict__ group, void* out,
                                                           int out_dt, int Hq, int D, int own, int slots, int has_sink, float sink,
                                                           HeadGate gate) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int r = blockIdx.x, h = blockIdx.y, t = rows ? rows[r] : r;
+  __shared__ float w_s[MAX_PARTS];
+  const int r = blockIdx.x, h = blockIdx.y, t = rows ? rows[r] : r, lane = threadIdx.x % 32;
   const int n = group[r] >= 0 ? slots : own;
   const size_t at = ((size_t)r * Hq + h) * slots;
-  float mm = -1e30f, ll = 0.f;
-  for (int s = 0; s < n; ++s) mm = fmaxf(mm, part_ml[(at + s) * 2]);
-  for (int s = 0; s < n; ++s) ll = fmaf(part_ml[(at + s) * 2 + 1], expf(part_ml[(at + s) * 2] - mm), ll);
-  if (has_sink) ll += expf(sink - mm);
-  const float by = (ll > 0.f ? 1.f / ll : 0.f) * head_gate_of(gate, t, h);
+  grid_dep_wait();
+  grid_dep_launch();
+  if (threadIdx.x < 32) {
+    const float2 none = make_float2(-1e30f, 0.f);
+    const float2* ml = (const float2*)part_ml + at;
+    const float2 x = lane < n ? ml[lane] : none, y = lane + 32 < n ? ml[lane + 32] : none;
+    const float mm = warp_max(fmaxf(x.x, y.x)), wx = expf(x.x - mm), wy = expf(y.x - mm);
+    float ll = warp_sum(x.y * wx + y.y * wy);
+    if (has_sink) ll += expf(sink - mm);
+    const float by = (ll > 0.f ? 1.f / ll : 0.f) * head_gate_of(gate, t, h);
+    w_s[lane] = wx * by;
+    w_s[lane + 32] = wy * by;
+  }
+  __syncthreads();
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    const float* from = part_o + at * D + d;
     float o = 0.f;
-    for (int s = 0; s < n; ++s) o = fmaf(part_o[(at + s) * D + d], expf(part_ml[(at + s) * 2] - mm), o);
-    st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, o * by);
+    for (int s0 = 0; s0 < n; s0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = s0 + i < n ? __ldg(from + (size_t)(s0 + i) * D) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < n) o = fmaf(v[i], w_s[s0 + i], o);
+    }
+    st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, o);
   }
 }
 
@@ -567,9 +613,10 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
                                       long long gate_ld, cudaStream_t stream) {
   if (!dt_ok(q_dt) || !dt_ok(cache_dt) || !dt_ok(out_dt)) return NV_ERR_BAD_DTYPE;
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || !nv_attention_shared_usable(D, page) || !(scale > 0.f)) return NV_ERR_UNSUPPORTED;
-  if (R < 0 || M < 0 || groups < 0 || own_splits < 1 || shared_splits < 0 || num_pages < 1) return NV_ERR_BAD_SIZE;
+  if (R < 0 || M < 0 || groups < 0 || own_splits < 1 || shared_splits < 0 || own_splits + shared_splits > MAX_PARTS || num_pages < 1)
+    return NV_ERR_BAD_SIZE;
   if (R == 0) return NV_OK;
-  if (!scratch) return NV_ERR_BAD_SIZE;
+  if (!scratch || ((uintptr_t)scratch & 7)) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
   const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc) && aligned16(scratch);
   const int per_tile = tc ? ST_PAIRS : SP_PAIRS;
@@ -587,7 +634,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   }
   const int rc = nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
                                           first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err,
-                                          (float_weights || has_sink) ? 1 : 0, softcap, stream);
+                                          (float_weights || has_sink) ? 1 : 0, softcap, shared_splits > 0 && groups > 0 ? 1 : 0, stream);
   if (rc) return rc;
   NV_RETURN_IF(launch_dep(shared_join_kernel, dim3(R, Hq), dim3(128), 0, stream, (const float*)scratch,
                           (const float*)scratch + (size_t)R * Hq * slots * D, rows, group, out, out_dt, Hq, D, own_splits, slots,

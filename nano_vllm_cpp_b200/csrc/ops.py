@@ -461,6 +461,7 @@ class SharedPrefix:
 
     def __init__(self, groups, rows: int, device):
         packed, self.members, self.longest = self.pack(groups, rows)
+        self.shortest = min((n for _, n in groups), default=0) if self.members == rows else 0      # what every row shares at least
         self.R, self.groups = rows, len(groups)
         self.bind(torch.tensor(packed, dtype=torch.int32).to(device))
 
@@ -516,7 +517,8 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(scale > 0 and softcap >= 0, "attention_decode_shared: the scale is positive, a cap is not negative")
     _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
     L = lib()
-    splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, max_context, num_sms())
+    own = max(1, max_context - shared.shortest // page * page)              # the most keys a row reads for itself
+    splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, own, num_sms())
     ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache),
                                         (1 if float_weights or sink_score is not None else 0), shared.longest)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
