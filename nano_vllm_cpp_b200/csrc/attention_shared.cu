@@ -29,6 +29,7 @@ struct SharedArgs {
   const int* members;       // [M] rows, group by group
   const int* cu;            // [groups + 1] into members
   const int* len;           // [groups] shared positions
+  const int* lead;          // [groups] the row whose block table is read
   float* part_o;            // [R, Hq, slots, D]
   float* part_ml;           // [R, Hq, slots, 2]
   int* err;
@@ -37,12 +38,18 @@ struct SharedArgs {
   int split_keys;           // a split has at least so many keys (a multiple of the page and of the kernel's block of keys)
 };
 
-// Which tile of `rows_per_tile` pairs of which group is tile number x?  A whole warp looks, 32 groups at a time; .x < 0: none (a
+// A block's tile: which group, its first pair and the number of pairs from there on in the group, its places in `members`, whole
+// pages of shared positions, and the leading row.
+struct Tile {
+  int group, pair0, pairs, member0, len, lead;
+};
+// Which tile of `rows_per_tile` pairs of which group is tile number x?  A whole warp looks, 32 groups at a time; group < 0: none (a
 // launch has as many tiles as there may be).
-__device__ __forceinline__ int2 find_tile(const SharedArgs& a, int x, int G, int rows_per_tile, int lane) {
+__device__ __forceinline__ Tile find_tile(const SharedArgs& a, int x, int G, int rows_per_tile, int lane) {
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
-    const int g = g0 + lane;
-    const int tiles = g < a.groups ? ((a.cu[g + 1] - a.cu[g]) * G + rows_per_tile - 1) / rows_per_tile : 0;
+    const int g = min(g0 + lane, a.groups - 1);
+    const int from = a.cu[g], to = a.cu[g + 1], len = a.len[g], lead = a.lead[g];
+    const int pairs = g0 + lane < a.groups ? (to - from) * G : 0, tiles = (pairs + rows_per_tile - 1) / rows_per_tile;
     int end = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -51,12 +58,13 @@ __device__ __forceinline__ int2 find_tile(const SharedArgs& a, int x, int G, int
     }
     const uint32_t who = __ballot_sync(0xffffffffu, x < end);
     if (who) {
-      const int l = __ffs(who) - 1;
-      return make_int2(g0 + l, (x - __shfl_sync(0xffffffffu, end - tiles, l)) * rows_per_tile);
+      const int l = __ffs(who) - 1, pair0 = (x - __shfl_sync(0xffffffffu, end - tiles, l)) * rows_per_tile;
+      return Tile{g0 + l, pair0, __shfl_sync(0xffffffffu, pairs, l) - pair0, __shfl_sync(0xffffffffu, from, l),
+                  __shfl_sync(0xffffffffu, len, l) / a.page * a.page, __shfl_sync(0xffffffffu, lead, l)};
     }
     x -= __shfl_sync(0xffffffffu, end, 31);
   }
-  return make_int2(-1, 0);
+  return Tile{-1, 0, 0, 0, 0, 0};
 }
 
 // The plain form: any type, any head size in steps of eight, float32 products.  A block takes 16 pairs of one kv head and one
@@ -70,19 +78,13 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
   float* q_s = sp_smem;                          // [SP_PAIRS][LD]
   float* kv_s = q_s + SP_PAIRS * LD;             // [SP_KEYS][LD]
   __shared__ float p_s[SP_PAIRS][SP_KEYS + 1];
-  __shared__ int2 tile_s;
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, kvh = blockIdx.y, split = blockIdx.z, G = a.Hq / a.Hkv;
-  if (tid < 32) {
-    const int2 tile = find_tile(a, blockIdx.x, G, SP_PAIRS, tid);
-    if (tid == 0) tile_s = tile;
-  }
-  __syncthreads();
-  const int g = tile_s.x, pair0 = tile_s.y;
-  if (g < 0) return;
-  const int m0 = a.cu[g], pairs = (a.cu[g + 1] - m0) * G, len = a.len[g] / a.page * a.page;
-  const int lead = a.members[m0], lead_t = a.rows ? a.rows[lead] : lead;
+  const Tile tile = find_tile(a, blockIdx.x, G, SP_PAIRS, tid % 32);
+  if (tile.group < 0) return;
+  const int m0 = tile.member0, pair0 = tile.pair0, pairs = pair0 + tile.pairs, len = tile.len;
+  const int lead = tile.lead, lead_t = a.rows ? a.rows[lead] : lead;
   const int* bt = a.block_table + (long long)a.row_entry[lead_t] * a.max_blocks;
   const int share = max(a.split_keys, ((len + a.splits - 1) / a.splits + SP_KEYS - 1) / SP_KEYS * SP_KEYS);
   const int j_lo = min(len, split * share), j_hi = min(len, j_lo + share);
@@ -195,7 +197,14 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
 // 3: the float32 weights enter the product with the values as three bfloat16 terms (all their bits) instead of one rounded.
 // Heads between the forms' sizes: the boxes reach beyond the pages' rows and are filled with zeros.
 constexpr int ST_PAIRS = 128, ST_KEYS = 64, ST_THREADS = 192;
-constexpr int ST_PAGES = 1024;           // block-table entries of a split kept in shared memory
+
+// Shared memory to global in one copy: addresses and bytes in steps of 16; the caller waits before it leaves.
+__device__ __forceinline__ void bulk_store(void* to, const void* from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(from)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_store_wait() {
+  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+}
 
 template <int D>
 constexpr int st_tmem_cols() { return 2 * ST_KEYS + D <= 256 ? 256 : 512; }
@@ -208,8 +217,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   extern __shared__ __align__(1024) uint8_t st_smem_raw[];
   __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full, pv_done;
   __shared__ uint32_t tmem_base_s;
-  __shared__ int2 tile_s;
-  __shared__ int bt_s[ST_PAGES];
 
   uint8_t* smem = (uint8_t*)(((uintptr_t)st_smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* Qs = smem;
@@ -234,49 +241,45 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     mbar_init(&pv_done, 1);
     mbar_fence_init();
   }
-  // keys of a block that are not loaded (behind the split's end) must be finite numbers: their weights are zero
-  for (int i = tid; i < (int)(3 * SL * KV_SLAB / 16); i += ST_THREADS) ((uint4*)Ks)[i] = make_uint4(0, 0, 0, 0);
-  fence_async_smem();
   if (warp == 1) tmem_alloc(&tmem_base_s, st_tmem_cols<D>());
-  grid_dep_wait();
-  grid_dep_launch();
-  if (warp == 0) {
-    const int2 tile = find_tile(a, blockIdx.x, G, ST_PAIRS, lane);
-    if (lane == 0) tile_s = tile;
-  }
+  // The groups, the tables and the positions are inputs of the whole step (as in attention_decode.cu): they are read before the
+  // kernel in front has ended, every warp for itself; queries, keys and values come after the wait.
+  const Tile tile = find_tile(a, blockIdx.x, G, ST_PAIRS, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
-  const int g = tile_s.x, pair0 = tile_s.y;
-  if (g >= 0) {
-    const int m0 = a.cu[g], pairs = min(ST_PAIRS, (a.cu[g + 1] - m0) * G - pair0), len = a.len[g] / a.page * a.page;
+  if (tile.group >= 0) {
+    const int pair0 = tile.pair0, pairs = min(ST_PAIRS, tile.pairs), len = tile.len;
     const int share = max(a.split_keys, ((len + a.splits - 1) / a.splits + ST_KEYS - 1) / ST_KEYS * ST_KEYS);
     const int j_lo = min(len, split * share), j_hi = min(len, j_lo + share);
     const int n_blocks = (j_hi - j_lo + ST_KEYS - 1) / ST_KEYS;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 2 * ST_KEYS;
-    const int lead = a.members[m0], lead_t = a.rows ? a.rows[lead] : lead;
-    const int* bt = a.block_table + (long long)a.row_entry[lead_t] * a.max_blocks;
-    const int page_shift = 31 - __clz(a.page);     // pages are 16, 32 or 64 keys
-    const int pg0 = j_lo >> page_shift, n_pg = min((j_hi - j_lo) >> page_shift, ST_PAGES);
-    for (int i = tid; i < n_pg; i += ST_THREADS) bt_s[i] = bt[pg0 + i];
-    __syncthreads();
+    const int lead_t = a.rows ? a.rows[tile.lead] : tile.lead;
+    // A block's keys behind the split's end are not loaded; their weights are zero, their values must be finite numbers.  Only a
+    // first block meets what the shared memory held before.
+    if (n_blocks == 1 && j_hi - j_lo < ST_KEYS) {
+      for (int i = tid; i < (int)(SL * KV_SLAB / 16); i += ST_THREADS) ((uint4*)Vs)[i] = make_uint4(0, 0, 0, 0);
+      fence_async_smem();
+      __syncthreads();
+    }
 
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer
+      const int page_shift = 31 - __clz(a.page);     // pages are 16, 32 or 64 keys
       const int pages = ST_KEYS >> page_shift;
       const uint32_t box = (uint32_t)a.page * 128;
       const int my_p = lane / SL, my_s = lane % SL;
-      auto load = [&](int i, bool values) {
-        const int j = j_lo + i * ST_KEYS + (my_p << page_shift);
-        int blk = -1;
-        if (my_p < pages && j < j_hi) {
-          const int pi = (j >> page_shift) - pg0;
-          blk = pi < ST_PAGES ? bt_s[pi] : bt[pg0 + pi];
-          if (blk < 0 || blk >= a.num_pages) {                           // it should be there and is not
-            atomicExch(a.err, 1 + lead_t);
-            blk = -1;
-          }
+      const int* bt = a.block_table + (long long)a.row_entry[lead_t] * a.max_blocks + (j_lo >> page_shift);
+      const int n_pages = my_p < pages ? (j_hi - j_lo) >> page_shift : 0;      // (a lane without a box has none)
+      auto page_of = [&](int i) { return i * pages + my_p < n_pages ? bt[i * pages + my_p] : -2; };
+      int blk_k = page_of(0), blk_v = blk_k, blk_next = page_of(1);            // read two blocks ahead
+      grid_dep_wait();
+      grid_dep_launch();
+      auto load = [&](int i, bool values, int blk) {
+        if (blk != -2 && (blk < 0 || blk >= a.num_pages)) {                    // it should be there and is not
+          atomicExch(a.err, 1 + lead_t);
+          blk = -1;
         }
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, blk >= 0));
         uint64_t* full = values ? &v_full : &k_full[i & 1];
@@ -291,13 +294,18 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           tma_load_2d(dst, values ? &tm_v : &tm_k, full, my_s * 64, (blk * a.Hkv + kvh) * a.page);
         }
       };
-      if (n_blocks > 0) load(0, false);
+      if (n_blocks > 0) load(0, false, blk_k);
       for (int i = 0; i < n_blocks; ++i) {         // the next keys go out before these values: they are free earlier
-        if (i + 1 < n_blocks) load(i + 1, false);
-        load(i, true);
+        blk_v = blk_k;
+        blk_k = blk_next;
+        blk_next = page_of(i + 2);
+        if (i + 1 < n_blocks) load(i + 1, false, blk_k);
+        load(i, true, blk_v);
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer
+      grid_dep_wait();
+      grid_dep_launch();
       if (lane == 0 && n_blocks > 0) {
         const uint32_t idesc_s = instr_desc(ST_KEYS), idesc_o = instr_desc_b_mn(D);
         const uint32_t q_addr = smem_u32(Qs), k_addr = smem_u32(Ks), v_addr = smem_u32(Vs), p_addr = smem_u32(Ps);
@@ -342,9 +350,11 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int q = warp % 4;                        // a warp may touch tensor-memory lanes [32q, 32q + 32) only
       const int p = q * 32 + lane;
       const bool live = p < pairs, some = q * 32 < pairs;       // (a warp without pairs only arrives where it is waited for)
-      const int r = live ? a.members[m0 + (pair0 + p) / G] : lead, h = kvh * G + (live ? (pair0 + p) % G : 0);
+      const int r = live ? a.members[tile.member0 + (pair0 + p) / G] : tile.lead, h = kvh * G + (live ? (pair0 + p) % G : 0);
       const int t = a.rows ? a.rows[r] : r;
       const int limit = live ? min(j_hi, a.positions[t] + 1) : j_hi;            // the first key that this row does not see
+      grid_dep_wait();
+      grid_dep_launch();
       const uint32_t lane_off = (uint32_t)(q * 32) << 16;
       {
         // the warp's 32 queries, D / 8 lanes a row and eight loads of a lane under way; rows of nobody and columns beyond the head
@@ -476,6 +486,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           a.part_ml[at * 2] = m == -INFINITY ? -1e30f : m * map.in * 0.6931471805599453f;
           a.part_ml[at * 2 + 1] = l;
         }
+        // A row of O goes through shared memory (all of it is free now; rows a chunk of 16 bytes further apart than they are long, so
+        // that a warp's threads write to different banks) and leaves in one copy: whole lines instead of 16 bytes in each of 32.
+        uint8_t* row = smem + (size_t)p * (D * 4 + 16);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -485,13 +498,12 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
           }
-          if (live) {
-            float* dst = a.part_o + at * a.D + c * 32;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (c * 32 + j < a.D) *(float4*)(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          }
+          for (int j = 0; j < 32; j += 4) *(float4*)(row + (c * 32 + j) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
+        fence_async_smem();
+        if (live) bulk_store(a.part_o + at * a.D, row, (uint32_t)a.D * 4);
+        bulk_store_wait();
       }
     }
   }
@@ -500,44 +512,68 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem_base, st_tmem_cols<D>());
 }
 
-// The parts of one (row, head), in the order of their slots: its own keys' splits, then the shared ones'.  A warp works out what
-// the parts weigh, then every thread adds its elements up, eight loads at a time.
-constexpr int MAX_PARTS = 64;
+// The parts of one (row, head): its own keys' splits, then the shared ones'.  Every warp works out what the parts weigh, takes every
+// fourth of them, four elements a lane and all loads under way, and the four sums are added in their order.
+constexpr int MAX_PARTS = 64, JOIN_WARPS = 4;
 
-__global__ void __launch_bounds__(128) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                                                          const int* __restrict__ rows, const int* __restrict__ group, void* out,
-                                                          int out_dt, int Hq, int D, int own, int slots, int has_sink, float sink,
-                                                          HeadGate gate) {
-  __shared__ float w_s[MAX_PARTS];
-  const int r = blockIdx.x, h = blockIdx.y, t = rows ? rows[r] : r, lane = threadIdx.x % 32;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                                      const int* __restrict__ rows, const int* __restrict__ group,
+                                                                      void* out, int out_dt, int Hq, int D, int own, int slots,
+                                                                      int has_sink, float sink, HeadGate gate) {
+  __shared__ float4 sum_s[JOIN_WARPS][64];
+  const int r = blockIdx.x, h = blockIdx.y, t = rows ? rows[r] : r, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int n = group[r] >= 0 ? slots : own;
   const size_t at = ((size_t)r * Hq + h) * slots;
   grid_dep_wait();
   grid_dep_launch();
-  if (threadIdx.x < 32) {
-    const float2 none = make_float2(-1e30f, 0.f);
-    const float2* ml = (const float2*)part_ml + at;
-    const float2 x = lane < n ? ml[lane] : none, y = lane + 32 < n ? ml[lane + 32] : none;
-    const float mm = warp_max(fmaxf(x.x, y.x)), wx = expf(x.x - mm), wy = expf(y.x - mm);
-    float ll = warp_sum(x.y * wx + y.y * wy);
-    if (has_sink) ll += expf(sink - mm);
-    const float by = (ll > 0.f ? 1.f / ll : 0.f) * head_gate_of(gate, t, h);
-    w_s[lane] = wx * by;
-    w_s[lane + 32] = wy * by;
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    const float* from = part_o + at * D + d;
-    float o = 0.f;
-    for (int s0 = 0; s0 < n; s0 += 8) {
-      float v[8];
+  const float2 none = make_float2(-1e30f, 0.f);
+  const float2* ml = (const float2*)part_ml + at;
+  const float2 x = lane < n ? ml[lane] : none, y = lane + 32 < n ? ml[lane + 32] : none;
+  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  float wx = 0.f, wy = 0.f, by = 0.f;
+  bool weighed = false;
+  for (int s0 = warp; s0 < n; s0 += 4 * JOIN_WARPS) {
+    float4 v[4][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = s0 + i < n ? __ldg(from + (size_t)(s0 + i) * D) : 0.f;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s0 + i < n) o = fmaf(v[i], w_s[s0 + i], o);
+      for (int c = 0; c < 2; ++c) {
+        const int s = s0 + i * JOIN_WARPS, d = (c * 32 + lane) * 4;
+        v[i][c] = s < n && d < D ? __ldg((const float4*)(part_o + (at + s) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    if (!weighed) {                                  // (behind the loads, which need not wait for it)
+      const float mm = warp_max(fmaxf(x.x, y.x));
+      wx = expf(x.x - mm);
+      wy = expf(y.x - mm);
+      float ll = warp_sum(x.y * wx + y.y * wy);
+      if (has_sink) ll += expf(sink - mm);
+      by = ll > 0.f ? 1.f / ll : 0.f;
+      weighed = true;
     }
-    st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * JOIN_WARPS;
+      const float w = __shfl_sync(0xffffffffu, s < 32 ? wx : wy, s % 32);
+      if (s < n) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          o[c].x = fmaf(v[i][c].x, w, o[c].x); o[c].y = fmaf(v[i][c].y, w, o[c].y);
+          o[c].z = fmaf(v[i][c].z, w, o[c].z); o[c].w = fmaf(v[i][c].w, w, o[c].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) sum_s[warp][c * 32 + lane] = o[c];
+  by = __shfl_sync(0xffffffffu, by, 0);
+  __shared__ float by_s;
+  if (threadIdx.x == 0) by_s = by * head_gate_of(gate, t, h);        // (warp 0 has a part always: a row has own keys' splits)
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += JOIN_WARPS * 32) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) v += ((const float*)&sum_s[w][0])[d];
+    st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, v * by_s);
   }
 }
 
@@ -562,7 +598,9 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
   rc = nv_tensor_map_bf16(a.vc, rows, a.D, a.D, a.page, &tm_v);
   if (rc) return rc;
   constexpr int SL = D / 64;
-  constexpr size_t smem = (size_t)SL * ST_PAIRS * 128 + 3 * (size_t)SL * ST_KEYS * 128 + (size_t)TERMS * ST_PAIRS * 128 + 1024;
+  constexpr size_t tiles_bytes = (size_t)SL * ST_PAIRS * 128 + 3 * (size_t)SL * ST_KEYS * 128 + (size_t)TERMS * ST_PAIRS * 128;
+  constexpr size_t smem = tiles_bytes + 1024;
+  static_assert(tiles_bytes >= (size_t)ST_PAIRS * (D * 4 + 16), "a row of results has its place");
   static bool attr_done = false;
   if (!attr_done) {
     NV_RETURN_IF(cudaFuncSetAttribute(shared_tc_kernel<D, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -588,6 +626,17 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
+// Splits of the rows' own keys, of which no row has more than `most`: one wave of blocks (three live on a multiprocessor, as in
+// attention_decode.cu; what a block costs beside its keys is the time here), and 128 keys a split or more.
+NV_API int nv_attention_shared_own_splits(int R, int Hq, int Hkv, int most) {
+  if (R <= 0 || Hkv <= 0 || most <= 0) return 1;
+  const int G = Hq / Hkv;
+  const long long blocks = (long long)R * Hkv * ((G + 15) / 16);
+  long long n = 3LL * num_multiprocessors() / blocks;
+  if (n > (most + 127) / 128) n = (most + 127) / 128;
+  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+}
+
 // Splits of the shared keys for M rows in `groups` groups whose longest prefix has `longest` positions.
 NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
   if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
@@ -602,12 +651,12 @@ NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D,
 NV_API int nv_attention_shared_usable(int D, int page) { return D >= 8 && D <= 256 && D % 8 == 0 && page >= 16 && page % 16 == 0; }
 
 // R rows (rows: their batch rows, nullptr: all); first [R]: positions of the row that are shared (0 without a group), group [R]: its
-// group or -1, members [M], cu [groups + 1], len [groups]: see SharedArgs.  own_splits and shared_splits parts a (row, head);
+// group or -1, members [M], cu [groups + 1], len and lead [groups]: see SharedArgs.  own_splits and shared_splits parts a (row, head);
 // scratch: R * Hq * (own_splits + shared_splits) * (D + 2) floats.
 NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                                       const int* block_table, int max_blocks, const int* row_entry, const int* positions,
                                       const int* rows, int R, const int* first, const int* group, const int* members, int M,
-                                      const int* cu, const int* len, int groups, float scale, void* out, int out_dt, int Hq, int Hkv,
+                                      const int* cu, const int* len, const int* lead, int groups, float scale, void* out, int out_dt, int Hq, int Hkv,
                                       int D, int page, int num_pages, int own_splits, int shared_splits, float* scratch, int* err,
                                       int has_sink, float sink_score, int float_weights, float softcap, const float* gate,
                                       long long gate_ld, cudaStream_t stream) {
@@ -616,15 +665,15 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   if (R < 0 || M < 0 || groups < 0 || own_splits < 1 || shared_splits < 0 || own_splits + shared_splits > MAX_PARTS || num_pages < 1)
     return NV_ERR_BAD_SIZE;
   if (R == 0) return NV_OK;
-  if (!scratch || ((uintptr_t)scratch & 7)) return NV_ERR_BAD_SIZE;
+  if (!scratch || ((uintptr_t)scratch & 15)) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
-  const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc) && aligned16(scratch);
+  const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc);
   const int per_tile = tc ? ST_PAIRS : SP_PAIRS;
   const long long tiles = ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;         // (or fewer)
   if (shared_splits > 0 && groups > 0) {
     SharedArgs a;
     a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;
-    a.members = members; a.cu = cu; a.len = len; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
+    a.members = members; a.cu = cu; a.len = len; a.lead = lead; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
     a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
     a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
     a.slots = slots; a.slot0 = own_splits; a.split_keys = 256;
@@ -636,7 +685,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
                                           first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err,
                                           (float_weights || has_sink) ? 1 : 0, softcap, shared_splits > 0 && groups > 0 ? 1 : 0, stream);
   if (rc) return rc;
-  NV_RETURN_IF(launch_dep(shared_join_kernel, dim3(R, Hq), dim3(128), 0, stream, (const float*)scratch,
+  NV_RETURN_IF(launch_dep(shared_join_kernel, dim3(R, Hq), dim3(JOIN_WARPS * 32), 0, stream, (const float*)scratch,
                           (const float*)scratch + (size_t)R * Hq * slots * D, rows, group, out, out_dt, Hq, D, own_splits, slots,
                           has_sink, sink_score, HeadGate{gate, gate_ld}));
   NV_RETURN_LAST();

@@ -468,7 +468,7 @@ class SharedPrefix:
     @staticmethod
     def pack(groups, rows: int):
         """The host's arrays in one list: per row its shared positions and its group (or -1), the groups' rows one after the
-        other (``rows`` places), where each group's start, and its positions; the number of grouped rows; the longest prefix."""
+        other (``rows`` places), where each group's start, its positions, and its first row; the number of grouped rows; the longest prefix."""
         first, group, members, cu, lens = [0] * rows, [-1] * rows, [], [0], []
         for g, (own, n) in enumerate(groups):
             _need(len(own) > 0 and n >= 0, "SharedPrefix: a group has a row at least and no negative prefix")
@@ -479,13 +479,14 @@ class SharedPrefix:
                 members.append(int(r))
             cu.append(len(members))
             lens.append(int(n))
-        return first + group + members + [0] * (rows - len(members)) + cu + lens, len(members), max(lens, default=0)
+        leads = [int(own[0]) for own, _ in groups]
+        return first + group + members + [0] * (rows - len(members)) + cu + lens + leads, len(members), max(lens, default=0)
 
     def bind(self, buf) -> None:
         R, G = self.R, self.groups
         self.buf = buf
-        self.first, self.group, self.rows_of, self.cu, self.lens = (buf[a:b] for a, b in (
-            (0, R), (R, 2 * R), (2 * R, 3 * R), (3 * R, 3 * R + G + 1), (3 * R + G + 1, 3 * R + 2 * G + 1)))
+        self.first, self.group, self.rows_of, self.cu, self.lens, self.leads = (buf[a:b] for a, b in (
+            (0, R), (R, 2 * R), (2 * R, 3 * R), (3 * R, 3 * R + G + 1), (3 * R + G + 1, 3 * R + 2 * G + 1), (3 * R + 2 * G + 1, 3 * R + 3 * G + 1)))
 
 
 def attention_decode_shared_usable(k_cache, D: int) -> bool:
@@ -518,13 +519,13 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
     L = lib()
     own = max(1, max_context - shared.shortest // page * page)              # the most keys a row reads for itself
-    splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, own, num_sms())
+    splits = L.nv_attention_shared_own_splits(R, Hq, Hkv, own)
     ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache),
                                         (1 if float_weights or sink_score is not None else 0), shared.longest)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
     _check(L.nv_attention_decode_shared(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table),
                                         block_table.shape[1], _p(row_entry), _p(positions), _p(rows), R, _p(shared.first),
-                                        _p(shared.group), _p(shared.rows_of), shared.members, _p(shared.cu), _p(shared.lens),
+                                        _p(shared.group), _p(shared.rows_of), shared.members, _p(shared.cu), _p(shared.lens), _p(shared.leads),
                                         shared.groups, scale, _p(out), dt(out), Hq, Hkv, D, page, k_cache.shape[0], splits, ours,
                                         _p(scratch), _p(err.t if err is not None else _global_err().t),
                                         (0 if sink_score is None else 1), float(sink_score or 0.0), (1 if float_weights else 0),

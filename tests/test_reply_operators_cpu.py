@@ -33,7 +33,7 @@ def test_page_copies_refuse_sizes():
 
 def shared(q_dt=1, R=1, M=0, groups=0, scale=1.0, Hq=4, Hkv=2, D=64, page=16, pages=8, own=1, ours=0):
     return ops.lib().nv_attention_decode_shared(None, q_dt, 512, None, None, 1, None, 4, None, None, None, R, None, None, None, M, None,
-                                                None, groups, scale, None, 1, Hq, Hkv, D, page, pages, own, ours, None, None, 0, 0.0,
+                                                None, None, groups, scale, None, 1, Hq, Hkv, D, page, pages, own, ours, None, None, 0, 0.0,
                                                 0, 0.0, None, 0, None)
 
 
@@ -53,7 +53,7 @@ def test_shared_prefix_packs_its_groups():
     assert packed[:6] == [0, 32, 7, 0, 32, 0]                               # shared positions of every row
     assert packed[6:12] == [-1, 0, 1, -1, 0, -1]                            # its group
     assert packed[12:15] == [4, 1, 2]                                       # the groups' rows, the leading one first
-    assert packed[18:21] == [0, 2, 3] and packed[21:] == [32, 7]
+    assert packed[18:21] == [0, 2, 3] and packed[21:23] == [32, 7] and packed[23:] == [4, 2]
     assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0, 0)
 
 
