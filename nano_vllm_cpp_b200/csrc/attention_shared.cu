@@ -68,15 +68,40 @@ __device__ __forceinline__ Tile find_tile(const SharedArgs& a, int x, int G, int
 }
 
 // The plain form: any type, any head size in steps of eight, float32 products.  A block takes 16 pairs of one kv head and one
-// split of the keys, 32 keys at a time; eight threads share a pair.
+// split of the keys, 32 keys at a time; eight threads share a pair.  The values are on their way while the scores are worked out,
+// the next keys while the values are summed.  DC: elements of a head at most.
 constexpr int SP_PAIRS = 16, SP_KEYS = 32, SP_THREADS = 128;
 
 template <typename T>
+struct Eight;                                    // eight elements as they lie in the cache
+template <>
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = __ldg((const float4*)p); b = __ldg((const float4*)p + 1); }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void put(float* to) const { *(float4*)to = a; *(float4*)(to + 4) = b; }
+};
+template <>
+struct Eight<bf16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const bf16* p) { a = __ldg((const uint4*)p); }
+  __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void put(float* to) const {
+    const __nv_bfloat162* h = (const __nv_bfloat162*)&a;
+    const float2 f0 = __bfloat1622float2(h[0]), f1 = __bfloat1622float2(h[1]), f2 = __bfloat1622float2(h[2]), f3 = __bfloat1622float2(h[3]);
+    *(float4*)to = make_float4(f0.x, f0.y, f1.x, f1.y);
+    *(float4*)(to + 4) = make_float4(f2.x, f2.y, f3.x, f3.y);
+  }
+};
+
+template <typename T, int DC>
 __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) {
+  constexpr int CHUNKS = SP_KEYS * (DC / 8) / SP_THREADS;        // pieces of eight elements a thread fetches of a block of keys
   extern __shared__ __align__(16) float sp_smem[];
   const int D = a.D, LD = D + 4;
   float* q_s = sp_smem;                          // [SP_PAIRS][LD]
-  float* kv_s = q_s + SP_PAIRS * LD;             // [SP_KEYS][LD]
+  float* k_s = q_s + SP_PAIRS * LD;              // [SP_KEYS][LD]
+  float* v_s = k_s + SP_KEYS * LD;               // [SP_KEYS][LD]
   __shared__ float p_s[SP_PAIRS][SP_KEYS + 1];
   grid_dep_wait();
   grid_dep_launch();
@@ -89,6 +114,28 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
   const int share = max(a.split_keys, ((len + a.splits - 1) / a.splits + SP_KEYS - 1) / SP_KEYS * SP_KEYS);
   const int j_lo = min(len, split * share), j_hi = min(len, j_lo + share);
 
+  Eight<T> part[CHUNKS];
+  auto fetch = [&](const void* cache, int j0) {  // zeros behind the split
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int x = tid + c * SP_THREADS, key = x / (D / 8), at = x % (D / 8), j = j0 + key;
+      part[c].zero();
+      if (key < SP_KEYS && j < j_hi) {
+        const int blk = __ldg(bt + j / a.page);
+        if (blk >= 0 && blk < a.num_pages) part[c].load((const T*)cache + (((size_t)blk * a.Hkv + kvh) * a.page + j % a.page) * D + at * 8);
+        else if (a.err) atomicExch(a.err, 1 + lead_t);
+      }
+    }
+  };
+  auto put = [&](float* to) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int x = tid + c * SP_THREADS, key = x / (D / 8), at = x % (D / 8);
+      if (key < SP_KEYS) part[c].put(to + key * LD + at * 8);
+    }
+  };
+  fetch(a.kc, j_lo);
+
   const int i = tid / 8, sub = tid % 8;          // this thread's pair of the tile, and which of its eight threads it is
   const bool live = pair0 + i < pairs;
   const int r = live ? a.members[m0 + (pair0 + i) / G] : lead, h = kvh * G + (live ? (pair0 + i) % G : 0);
@@ -96,40 +143,22 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
   const int limit = live ? min(j_hi, a.positions[t] + 1) : 0;        // the first key that this row does not see
   for (int d = sub; d < D; d += 8) q_s[i * LD + d] = live ? ld_dt(a.q, a.q_dt, (size_t)t * a.q_stride + (size_t)h * D + d) * a.scale : 0.f;
 
-  float m = -INFINITY, l = 0.f, o[8][4];
+  float m = -INFINITY, l = 0.f, o[DC / 32][4];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-  const int chunks = D / 4;
-  auto load = [&](const void* cache, int j0) {   // SP_KEYS keys (or values) as floats, zeros beyond the split
-    for (int x = tid; x < SP_KEYS * (D / 8); x += SP_THREADS) {
-      const int key = x / (D / 8), c = x % (D / 8), j = j0 + key;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (j < j_hi) {
-        const int blk = bt[j / a.page];
-        if (blk >= 0 && blk < a.num_pages) {
-          const T* p = (const T*)cache + (((size_t)blk * a.Hkv + kvh) * a.page + j % a.page) * D + c * 8;
-#pragma unroll
-          for (int u = 0; u < 8; ++u) v[u] = to_f32(p[u]);
-        } else if (a.err) {
-          atomicExch(a.err, 1 + lead_t);
-        }
-      }
-      *(float4*)&kv_s[key * LD + c * 8] = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)&kv_s[key * LD + c * 8 + 4] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  };
+  for (int c = 0; c < DC / 32; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
   for (int j0 = j_lo; j0 < j_hi; j0 += SP_KEYS) {
+    put(k_s);                                    // (the scores before these are done: every thread has been at the barrier below)
     __syncthreads();
-    load(a.kc, j0);
-    __syncthreads();
+    fetch(a.vc, j0);
     float s[SP_KEYS / 8];
 #pragma unroll
     for (int u = 0; u < SP_KEYS / 8; ++u) s[u] = 0.f;
-    for (int c = 0; c < chunks; ++c) {
+#pragma unroll 4
+    for (int c = 0; c < D / 4; ++c) {
       const float4 qv = *(const float4*)&q_s[i * LD + c * 4];
 #pragma unroll
       for (int u = 0; u < SP_KEYS / 8; ++u) {
-        const float4 kv = *(const float4*)&kv_s[(u * 8 + sub) * LD + c * 4];
+        const float4 kv = *(const float4*)&k_s[(u * 8 + sub) * LD + c * 4];
         s[u] = fmaf(qv.x, kv.x, s[u]); s[u] = fmaf(qv.y, kv.y, s[u]); s[u] = fmaf(qv.z, kv.z, s[u]); s[u] = fmaf(qv.w, kv.w, s[u]);
       }
     }
@@ -154,31 +183,32 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     l = l * alpha + sum;
+    put(v_s);                                    // (the sums before these are done: every thread has been at the barrier above)
     __syncthreads();
-    load(a.vc, j0);
-    __syncthreads();
+    fetch(a.kc, j0 + SP_KEYS);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const int at = (c * 8 + sub) * 4;
-      if (at < D) {
-        float4 acc = make_float4(o[c][0] * alpha, o[c][1] * alpha, o[c][2] * alpha, o[c][3] * alpha);
-        for (int key = 0; key < SP_KEYS; ++key) {
-          const float p = p_s[i][key];
-          const float4 v = *(const float4*)&kv_s[key * LD + at];
-          acc.x = fmaf(p, v.x, acc.x); acc.y = fmaf(p, v.y, acc.y); acc.z = fmaf(p, v.z, acc.z); acc.w = fmaf(p, v.w, acc.w);
+    for (int c = 0; c < DC / 32; ++c)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[c][u] *= alpha;
+#pragma unroll 4
+    for (int key = 0; key < SP_KEYS; ++key) {
+      const float p = p_s[i][key];
+#pragma unroll
+      for (int c = 0; c < DC / 32; ++c) {
+        const int at = (c * 8 + sub) * 4;
+        if (at < D) {
+          const float4 v = *(const float4*)&v_s[key * LD + at];
+          o[c][0] = fmaf(p, v.x, o[c][0]); o[c][1] = fmaf(p, v.y, o[c][1]); o[c][2] = fmaf(p, v.z, o[c][2]); o[c][3] = fmaf(p, v.w, o[c][3]);
         }
-        o[c][0] = acc.x; o[c][1] = acc.y; o[c][2] = acc.z; o[c][3] = acc.w;
       }
     }
   }
   if (!live) return;
   const size_t at = ((size_t)r * a.Hq + h) * a.slots + a.slot0 + split;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
+  for (int c = 0; c < DC / 32; ++c) {
     const int d = (c * 8 + sub) * 4;
-    if (d < D)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) a.part_o[at * D + d + u] = o[c][u];
+    if (d < D) *(float4*)(a.part_o + at * D + d) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
   }
   if (sub == 0) {
     a.part_ml[at * 2] = m == -INFINITY ? -1e30f : m;
@@ -352,29 +382,28 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const bool live = p < pairs, some = q * 32 < pairs;       // (a warp without pairs only arrives where it is waited for)
       const int r = live ? a.members[tile.member0 + (pair0 + p) / G] : tile.lead, h = kvh * G + (live ? (pair0 + p) % G : 0);
       const int t = a.rows ? a.rows[r] : r;
-      const int limit = live ? min(j_hi, a.positions[t] + 1) : j_hi;            // the first key that this row does not see
+      const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+      const int position = a.positions[t];
       grid_dep_wait();
       grid_dep_launch();
-      const uint32_t lane_off = (uint32_t)(q * 32) << 16;
       {
-        // the warp's 32 queries, D / 8 lanes a row and eight loads of a lane under way; rows of nobody and columns beyond the head
-        // are zeros
-        constexpr int PER = D / 8, AT_ONCE = 32 / PER;              // (PER is 8, 16 or 32)
+        // the warp's 32 queries, D / 8 lanes a row and sixteen loads of a lane under way; rows of nobody and columns beyond the
+        // head are zeros
+        constexpr int PER = D / 8, AT_ONCE = 32 / PER, LOADS = 32 / AT_ONCE < 16 ? 32 / AT_ONCE : 16;      // (PER is 8, 16 or 32)
         const int c = lane % PER;
+        const long long place = (long long)t * a.q_stride + (long long)h * a.D;
 #pragma unroll
-        for (int i0 = 0; i0 < 32; i0 += 8 * AT_ONCE) {
-          uint4 v[8];
+        for (int i0 = 0; i0 < 32; i0 += LOADS * AT_ONCE) {
+          uint4 v[LOADS];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int i = (i0 + u * AT_ONCE + lane / PER) % 32;
-            const int rt = __shfl_sync(0xffffffffu, t, i), rh = __shfl_sync(0xffffffffu, h, i);
-            v[u] = q * 32 + i < pairs && c * 8 < a.D
-                       ? *(const uint4*)((const bf16*)a.q + (size_t)rt * a.q_stride + (size_t)rh * a.D + c * 8)
-                       : make_uint4(0, 0, 0, 0);
+          for (int u = 0; u < LOADS; ++u) {
+            const int i = i0 + u * AT_ONCE + lane / PER;
+            const long long from = __shfl_sync(0xffffffffu, place, i);
+            v[u] = q * 32 + i < pairs && c * 8 < a.D ? *(const uint4*)((const bf16*)a.q + from + c * 8) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int row = q * 32 + (i0 + u * AT_ONCE + lane / PER) % 32;
+          for (int u = 0; u < LOADS; ++u) {
+            const int row = q * 32 + i0 + u * AT_ONCE + lane / PER;
             *(uint4*)(Qs + (c / 8) * Q_SLAB + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[u];
           }
         }
@@ -382,12 +411,13 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full);
       }
+      const int limit = live ? min(j_hi, position + 1) : j_hi;                  // the first key that this row does not see
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n_blocks; ++i) {
         const int j0 = j_lo + i * ST_KEYS;
         mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.err, 0x7307);
         float s[ST_KEYS];
-        float mx = -INFINITY;
+        float alpha = 1.f;
         if (some) {
           tc_fence_after();
           tmem_ld32_nowait(tmem_s + (i & 1) * ST_KEYS + lane_off, s);
@@ -403,13 +433,36 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             for (int c = 0; c < ST_KEYS; ++c)
               if (j0 + c >= limit) s[c] = -INFINITY;
           }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx4[4] = {s[0], s[1], s[2], s[3]};                       // four chains, three numbers a step
+#pragma unroll
+          for (int c = 4; c < ST_KEYS - 4; c += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(fmaxf(s[c + u], s[c + 4 + u]), mx4[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], s[ST_KEYS - 4 + u]);
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          // the exponent's reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost
+          // bfloat16 and the float32 sums nothing), so that O is rescaled once in a long while
+          if (mx > m && (m == -INFINITY || (mx - m) * map.in > 8.f)) {
+            alpha = m == -INFINITY ? 0.f : ex2_fast((m - mx) * map.in);
+            m = mx;
+          }
+          const float ms = m == -INFINITY ? 0.f : m * map.in;
+          // two elements an instruction where there is one
+          float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float2 in2 = make_float2(map.in, map.in), ms2 = make_float2(-ms, -ms);
 #pragma unroll
           for (int c = 0; c < ST_KEYS; c += 4) {
-            mx4[0] = fmaxf(mx4[0], s[c]); mx4[1] = fmaxf(mx4[1], s[c + 1]);
-            mx4[2] = fmaxf(mx4[2], s[c + 2]); mx4[3] = fmaxf(mx4[3], s[c + 3]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float2 e = fma2(make_float2(s[c + 2 * u], s[c + 2 * u + 1]), in2, ms2);
+              s[c + 2 * u] = ex2_fast(e.x);
+              s[c + 2 * u + 1] = ex2_fast(e.y);
+              sum2[u] = add2(sum2[u], make_float2(s[c + 2 * u], s[c + 2 * u + 1]));
+            }
           }
-          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
         }
         // O += P(i-1) V(i-1) must have ended before O is rescaled and P is overwritten (a warp without pairs waits too: its
         // arrival is one for this block)
@@ -418,14 +471,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           tc_fence_after();
         }
         if (some) {
-          // the exponent's reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost
-          // bfloat16 and the float32 sums nothing), so that O is rescaled once in a long while
-          float alpha = 1.f;
-          if (mx > m && (m == -INFINITY || (mx - m) * map.in > 8.f)) {
-            alpha = m == -INFINITY ? 0.f : ex2_fast((m - mx) * map.in);
-            m = mx;
-          }
-          const float ms = m == -INFINITY ? 0.f : m * map.in;
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -436,16 +481,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               tmem_st32(tmem_o + lane_off + c * 32, o);
             }
           }
-          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < ST_KEYS; c += 4) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              s[c + u] = ex2_fast(fmaf(s[c + u], map.in, -ms));
-              sum4[u] += s[c + u];
-            }
-          }
-          l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
           uint8_t* prow = Ps + (size_t)p * 128;
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -489,17 +524,21 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         // A row of O goes through shared memory (all of it is free now; rows a chunk of 16 bytes further apart than they are long, so
         // that a warp's threads write to different banks) and leaves in one copy: whole lines instead of 16 bytes in each of 32.
         uint8_t* row = smem + (size_t)p * (D * 4 + 16);
+        constexpr int W = D < 128 ? D : 128;                  // columns whose loads are under way at once
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
+        for (int c0 = 0; c0 < D; c0 += W) {
+          float o[W];
           if (n_blocks > 0) {
-            tmem_ld32(tmem_o + lane_off + c * 32, o);
+#pragma unroll
+            for (int c = 0; c < W; c += 32) tmem_ld32_nowait(tmem_o + lane_off + c0 + c, o + c);
+            tmem_ld_wait();
+            tmem_ld_fence<W>(o);
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+            for (int j = 0; j < W; ++j) o[j] = 0.f;
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *(float4*)(row + (c * 32 + j) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          for (int j = 0; j < W; j += 4) *(float4*)(row + (c0 + j) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
         fence_async_smem();
         if (live) bulk_store(a.part_o + at * a.D, row, (uint32_t)a.D * 4);
@@ -577,16 +616,21 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const floa
   }
 }
 
-template <typename T>
-int launch_plain(const SharedArgs& a, int tiles, cudaStream_t s) {
-  const size_t smem = (size_t)(SP_PAIRS + SP_KEYS) * (a.D + 4) * sizeof(float);
+template <typename T, int DC>
+int launch_plain_d(const SharedArgs& a, int tiles, cudaStream_t s) {
+  const size_t smem = (size_t)(SP_PAIRS + 2 * SP_KEYS) * (a.D + 4) * sizeof(float);
   static bool attr_done = false;
   if (!attr_done) {
-    NV_RETURN_IF(cudaFuncSetAttribute(shared_plain_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+    NV_RETURN_IF(cudaFuncSetAttribute(shared_plain_kernel<T, DC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (SP_PAIRS + 2 * SP_KEYS) * (DC + 4) * (int)sizeof(float)));
     attr_done = true;
   }
-  NV_RETURN_IF(launch_dep(shared_plain_kernel<T>, dim3(tiles, a.Hkv, a.splits), dim3(SP_THREADS), smem, s, a));
+  NV_RETURN_IF(launch_dep(shared_plain_kernel<T, DC>, dim3(tiles, a.Hkv, a.splits), dim3(SP_THREADS), smem, s, a));
   NV_RETURN_LAST();
+}
+template <typename T>
+int launch_plain(const SharedArgs& a, int tiles, cudaStream_t s) {
+  return a.D <= 128 ? launch_plain_d<T, 128>(a, tiles, s) : launch_plain_d<T, 256>(a, tiles, s);
 }
 
 template <int D, int TERMS>
@@ -618,6 +662,9 @@ int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
   return a.D <= 64 ? launch_tc<64, TERMS>(a, tiles, s) : a.D <= 128 ? launch_tc<128, TERMS>(a, tiles, s) : launch_tc<256, TERMS>(a, tiles, s);
 }
 
+// Keys of a split at least.
+constexpr int TC_SPLIT_KEYS = 256, PLAIN_SPLIT_KEYS = 64;
+
 // Whether the tensor-core form takes these sizes (and, with pointers, these addresses).
 bool tc_takes(int cache_dt, int D, int page) {
   return cache_dt == NV_DT_BF16 && D >= 32 && D % 16 == 0 && (page == 16 || page == 32 || page == 64);
@@ -641,9 +688,9 @@ NV_API int nv_attention_shared_own_splits(int R, int Hq, int Hkv, int most) {
 NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
   if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
   const bool tc = tc_takes(cache_dt, D, page);
-  const int rows = tc ? ST_PAIRS : SP_PAIRS, each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4;
+  const int rows = tc ? ST_PAIRS : SP_PAIRS, each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4, least = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
   const long long tiles = ((long long)M * (Hq / Hkv) + rows - 1) / rows + groups - 1;
-  const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + 255) / 256;
+  const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + least - 1) / least;
   const long long n = want < most ? want : most;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
@@ -665,6 +712,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   if (R < 0 || M < 0 || groups < 0 || own_splits < 1 || shared_splits < 0 || own_splits + shared_splits > MAX_PARTS || num_pages < 1)
     return NV_ERR_BAD_SIZE;
   if (R == 0) return NV_OK;
+  if (!aligned16(kc) || !aligned16(vc)) return NV_ERR_UNSUPPORTED;
   if (!scratch || ((uintptr_t)scratch & 15)) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
   const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc);
@@ -676,7 +724,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
     a.members = members; a.cu = cu; a.len = len; a.lead = lead; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
     a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
     a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
-    a.slots = slots; a.slot0 = own_splits; a.split_keys = 256;
+    a.slots = slots; a.slot0 = own_splits; a.split_keys = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
     const int rc = tc ? ((float_weights || has_sink) ? launch_tc_d<3>(a, (int)tiles, stream) : launch_tc_d<1>(a, (int)tiles, stream))
                    : cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, (int)tiles, stream) : launch_plain<float>(a, (int)tiles, stream);
     if (rc) return rc;

@@ -155,6 +155,23 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two float32 operations an instruction.
+__device__ __forceinline__ unsigned long long pair_of(float2 v) { return *(unsigned long long*)&v; }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return *(float2*)&r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return *(float2*)&r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
+  return *(float2*)&r;
+}
 // A score on its way to base-2 units in the tensor-core kernels.  cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), whose
 // absolute error is a few units of the cap's last place, as the difference's is whatever x is.
 struct ScoreMap {

@@ -39,23 +39,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {       // (fmaxf dro
   return r;
 }
 
-__device__ __forceinline__ unsigned long long pair_of(float2 v) { return *(unsigned long long*)&v; }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
-  return *(float2*)&r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
-  return *(float2*)&r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
-  return *(float2*)&r;
-}
-
 struct Stats {
   float m, n1, s, e;
 };
