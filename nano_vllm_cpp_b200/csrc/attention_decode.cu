@@ -449,12 +449,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 constexpr int TC_ROWS = 16;      // query heads per block (rows of the MMA)
 
 // D: head dimension rounded up to a multiple of 64 (compile time: it sizes the fragments); a.D: the head's own elements.
-// MOD 1: scores pass a cap and a bias by distance; they are then in base-2 units (and a.scale is 1).  MOD 2: the same with a
+// FORM 1: the rest of a row behind a shared prefix (see DecArgs), FORM 2: `clean`.  MOD 1: scores pass a cap and a bias by distance; they are then in base-2 units (and a.scale is 1).  MOD 2: the same with a
 // cap whose tangent is tanhf's (capped_log2 is off by some 2^-22 of the cap, however small the score).
-template <int D, int TERMS, int MOD, bool REST>
+template <int D, int TERMS, int MOD, int FORM>
 __global__ void __launch_bounds__((WARPS + 1) * 32, D <= 128 ? 3 : 1)
 attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                            DecArgs a) {
+  constexpr bool REST = FORM == 1;
   extern __shared__ __align__(1024) uint8_t dec_smem_raw[];
   constexpr int QLD = D + 8;                         // padded row of q in shared memory
   __shared__ __align__(16) bf16 q_s[TC_ROWS * QLD];
@@ -669,7 +670,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
         }
         // What lies behind the row's position in its newest page may be anything, infinities of an earlier holder too, and a weight
         // of zero would not keep them out of the sums.  (The values are this warp's, and no load follows them.)
-        if (REST && j0 + 15 >= n) {
+        if (FORM != 0 && j0 + 15 >= n) {
           for (int x = lane; x < (j0 + 16 - n) * (D / 8); x += 32) {
             const int key = kb * 16 + (n - j0) + x / (D / 8), c = x % (D / 8);
             *(uint4*)(dec_smem + (vbase - smem0) + (c / 8) * box_bytes + key * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
@@ -822,7 +823,7 @@ int launch_decode(const DecArgs& a, int R, int G, size_t smem, cudaStream_t s) {
   return G == 1 ? launch_decode_g<TC, CPL, 1, false>(a, R, G, smem, s) : launch_decode_g<TC, CPL, 4, false>(a, R, G, smem, s);
 }
 
-template <int D, int TERMS, int MOD, bool REST>
+template <int D, int TERMS, int MOD, int FORM>
 int launch_decode_tc(DecArgs a, int R, const void* kc, const void* vc, int num_pages, float scale, cudaStream_t s) {
   const int G = a.Hq / a.Hkv;
   CUtensorMap tm_k, tm_v;
@@ -837,26 +838,26 @@ int launch_decode_tc(DecArgs a, int R, const void* kc, const void* vc, int num_p
   const size_t smem = (ring > merge ? ring : merge) + 1024;
   static bool attr_done = false;
   if (!attr_done) {
-    cudaError_t e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          160 * 1024);
     if (e != cudaSuccess) return (int)e;
     // three CTAs with a 64 KB ring each need nearly all of a multiprocessor's shared memory
-    e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, REST>, cudaFuncAttributePreferredSharedMemoryCarveout,
+    e = cudaFuncSetAttribute(attention_decode_tc_kernel<D, TERMS, MOD, FORM>, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return (int)e;
     attr_done = true;
   }
   dim3 grid(R, a.Hkv * ((G + TC_ROWS - 1) / TC_ROWS), a.splits);
-  NV_RETURN_IF(launch_dep(attention_decode_tc_kernel<D, TERMS, MOD, REST>, grid, dim3((WARPS + 1) * 32), smem, s, tm_k, tm_v, a));
+  NV_RETURN_IF(launch_dep(attention_decode_tc_kernel<D, TERMS, MOD, FORM>, grid, dim3((WARPS + 1) * 32), smem, s, tm_k, tm_v, a));
   NV_RETURN_LAST();
 }
 
-template <int TERMS, int MOD, bool REST = false>
+template <int TERMS, int MOD, int FORM = 0>
 int launch_decode_tc_d(const DecArgs& a, int DT, int R, const void* kc, const void* vc, int num_pages, float scale, cudaStream_t s) {
-  return DT == 64 ? launch_decode_tc<64, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
-       : DT == 128 ? launch_decode_tc<128, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
-       : DT == 192 ? launch_decode_tc<192, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s)
-                   : launch_decode_tc<256, TERMS, MOD, REST>(a, R, kc, vc, num_pages, scale, s);
+  return DT == 64 ? launch_decode_tc<64, TERMS, MOD, FORM>(a, R, kc, vc, num_pages, scale, s)
+       : DT == 128 ? launch_decode_tc<128, TERMS, MOD, FORM>(a, R, kc, vc, num_pages, scale, s)
+       : DT == 192 ? launch_decode_tc<192, TERMS, MOD, FORM>(a, R, kc, vc, num_pages, scale, s)
+                   : launch_decode_tc<256, TERMS, MOD, FORM>(a, R, kc, vc, num_pages, scale, s);
 }
 
 // Stages of the page ring for a page of `page` keys of `D` elements of `esize` bytes: as many as fit in
@@ -925,6 +926,8 @@ NV_API int nv_attention_decode_splits_of(int rows, int Hq, int Hkv, int D, int m
 // first != nullptr ([R], positions): a row reads its keys from the start of that position's page on (none where that lies behind
 // its own position) and leaves partial results, slot 0 .. splits - 1 of the `slots` that scratch holds for a (row, head): [R, Hq, slots, D] sums and then
 // [R, Hq, slots, 2] pairs of maximum (natural units; -1e30: no key) and sum.  Sink and gate are then the joining kernel's.
+// clean: what lies behind a row's position in its newest page may be anything, and the tensor-core form clears it from its copy of the
+// page (the other form never takes it in); else it must be finite numbers.
 namespace {
 int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                const int* block_table, int max_blocks, const int* row_entry, const int* positions,
@@ -932,7 +935,7 @@ int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const vo
                int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
                int* split_count, int split_count_len, int has_sink, float sink_score,
                int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
-               const float* slopes, const float* bias_table, int bias_len, const int* first, int slots, int beside, cudaStream_t stream) {
+               const float* slopes, const float* bias_table, int bias_len, const int* first, int slots, int beside, int clean, cudaStream_t stream) {
   // gate: head h's output of batch row t is multiplied by sigmoid(gate[t * gate_ld + h]) (nullptr: it is not); the
   // gates must have been written before the kernel that precedes this one on the stream.
   // softcap > 0: scaled scores are capped, s -> softcap * tanh(s / softcap).  chunk > 0: a row at position p sees the
@@ -1028,12 +1031,18 @@ int decode_run(const void* qkv, int q_dt, int q_stride, const void* kc, const vo
     // tensor-core form (a page of keys per warp); its blocks take up to 16 query heads of a kv head; with
     // float_weights or a sink the weights enter the product with the values as three bfloat16 terms
     const bool mod = a.softcap > 0.f || slopes || bias_table;
+    const bool terms = float_weights || has_sink;
     if (first)                                     // (a cap by tanhf: one form for all of them)
-      rc = float_weights ? (mod ? launch_decode_tc_d<3, 2, true>(a, DT, R, kc, vc, num_pages, scale, stream)
-                                : launch_decode_tc_d<3, 0, true>(a, DT, R, kc, vc, num_pages, scale, stream))
-                         : (mod ? launch_decode_tc_d<1, 2, true>(a, DT, R, kc, vc, num_pages, scale, stream)
-                                : launch_decode_tc_d<1, 0, true>(a, DT, R, kc, vc, num_pages, scale, stream));
-    else if (float_weights || has_sink)
+      rc = terms ? (mod ? launch_decode_tc_d<3, 2, 1>(a, DT, R, kc, vc, num_pages, scale, stream)
+                        : launch_decode_tc_d<3, 0, 1>(a, DT, R, kc, vc, num_pages, scale, stream))
+                 : (mod ? launch_decode_tc_d<1, 2, 1>(a, DT, R, kc, vc, num_pages, scale, stream)
+                        : launch_decode_tc_d<1, 0, 1>(a, DT, R, kc, vc, num_pages, scale, stream));
+    else if (clean)
+      rc = terms ? (mod ? launch_decode_tc_d<3, 2, 2>(a, DT, R, kc, vc, num_pages, scale, stream)
+                        : launch_decode_tc_d<3, 0, 2>(a, DT, R, kc, vc, num_pages, scale, stream))
+                 : (mod ? launch_decode_tc_d<1, 2, 2>(a, DT, R, kc, vc, num_pages, scale, stream)
+                        : launch_decode_tc_d<1, 0, 2>(a, DT, R, kc, vc, num_pages, scale, stream));
+    else if (terms)
       rc = has_sink && a.softcap > 0.f ? launch_decode_tc_d<3, 2>(a, DT, R, kc, vc, num_pages, scale, stream)
            : mod ? launch_decode_tc_d<3, 1>(a, DT, R, kc, vc, num_pages, scale, stream)
                  : launch_decode_tc_d<3, 0>(a, DT, R, kc, vc, num_pages, scale, stream);
@@ -1069,7 +1078,20 @@ NV_API int nv_attention_decode(const void* qkv, int q_dt, int q_stride, const vo
                                const float* slopes, const float* bias_table, int bias_len, cudaStream_t stream) {
   return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, window,
                     out, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, split_count, split_count_len, has_sink,
-                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, 0, stream);
+                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, 0, 0, stream);
+}
+
+// The same with `clean` (see decode_run).
+NV_API int nv_attention_decode_clean(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
+                                           const int* block_table, int max_blocks, const int* row_entry, const int* positions,
+                                     const int* rows, int R, float scale, int window, void* out, int out_dt, int Hq,
+                                     int Hkv, int D, int page, int num_pages, int splits, float* scratch, int* err,
+                                     int* split_count, int split_count_len, int has_sink, float sink_score,
+                                     int float_weights, float softcap, const float* gate, long long gate_ld, int chunk,
+                                     const float* slopes, const float* bias_table, int bias_len, cudaStream_t stream) {
+  return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, window,
+                    out, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, split_count, split_count_len, has_sink,
+                    sink_score, float_weights, softcap, gate, gate_ld, chunk, slopes, bias_table, bias_len, nullptr, 0, 0, 1, stream);
 }
 
 // The keys from position first[r] on, as partial results (see decode_run): what attention over a shared prefix joins with it.
@@ -1081,7 +1103,7 @@ int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void
   if (!first) return NV_ERR_BAD_SIZE;
   return decode_run(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows, R, scale, 0,
                     nullptr, out_dt, Hq, Hkv, D, page, num_pages, splits, scratch, err, nullptr, 0, 0, 0.f, float_weights, softcap,
-                    nullptr, 0, 0, nullptr, nullptr, 0, first, slots, beside, stream);
+                    nullptr, 0, 0, nullptr, nullptr, 0, first, slots, beside, 0, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -673,26 +673,54 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// Splits of the rows' own keys, of which no row has more than `most`: one wave of blocks (three live on a multiprocessor, as in
-// attention_decode.cu; what a block costs beside its keys is the time here), and 128 keys a split or more.
-NV_API int nv_attention_shared_own_splits(int R, int Hq, int Hkv, int most) {
+// Tiles of pairs that M rows in `groups` groups make at most.
+namespace {
+long long shared_tiles(int M, int groups, int Hq, int Hkv, int per_tile) {
+  return ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;
+}
+}  // namespace
+
+// Splits of the shared keys for M rows in `groups` groups whose longest prefix has `longest` positions: as many blocks as live on
+// the GPU at once (two a multiprocessor, one of the larger forms), 256 keys a split or more.  (64 rows of 28 heads on 4 behind 8,192
+// positions, 18 splits: 44 us; 9: 48, 32: 51.  128 behind 16,384, 10: 67; 6: 81, 18: 77.)
+NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
+  if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
+  const bool tc = tc_takes(cache_dt, D, page);
+  const int each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4, least = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
+  const long long tiles = shared_tiles(M, groups, Hq, Hkv, tc ? ST_PAIRS : SP_PAIRS);
+  const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + least - 1) / least;
+  const long long n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+}
+
+// Splits of the rows' own keys, of which no row has more than `most`, beside shared_splits of the above: 128 keys a split or more.
+// Where the shared part leaves room, they run beside it, one block (of 76 KB) on its multiprocessors and three on the others, and a
+// second wave would come after it (eight rows of 16 heads behind 2,048: 13.9 us in one wave, 17.5 in two); where it fills the
+// GPU they come after it anyway (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own: one split 43.8, four 41.7).
+NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int shared_splits,
+                                          int most) {
   if (R <= 0 || Hkv <= 0 || most <= 0) return 1;
   const int G = Hq / Hkv;
-  const long long blocks = (long long)R * Hkv * ((G + 15) / 16);
-  long long n = 3LL * num_multiprocessors() / blocks;
+  const long long sms = num_multiprocessors(), blocks = (long long)R * Hkv * ((G + 15) / 16);
+  const long long shared = shared_splits <= 0 ? 0 : shared_tiles(M, groups, Hq, Hkv, tc_takes(cache_dt, D, page) ? ST_PAIRS : SP_PAIRS) * Hkv * shared_splits;
+  const long long room = shared <= sms ? shared + 3 * (sms - shared) : 7 * sms;
+  long long n = room / blocks;
   if (n > (most + 127) / 128) n = (most + 127) / 128;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
 
-// Splits of the shared keys for M rows in `groups` groups whose longest prefix has `longest` positions.
-NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
-  if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
-  const bool tc = tc_takes(cache_dt, D, page);
-  const int rows = tc ? ST_PAIRS : SP_PAIRS, each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4, least = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
-  const long long tiles = ((long long)M * (Hq / Hkv) + rows - 1) / rows + groups - 1;
-  const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + least - 1) / least;
-  const long long n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+// Whether `repeated` positions that need not be read again are worth a kernel more and a join (1) or not (0), in bytes of keys and
+// values.  Tensor-core form: 16 MB, some three microseconds of reading, and 32 KB for every row and kv head, whose parts are joined
+// (shared and not: four rows of 16 kv heads behind 700 positions, 17 MB, 10.3 and 9.5 us, behind 1,500, 37 MB, 11.0 and 13.2; eight
+// of 4 behind 1,000, 14 MB, 12.2 and 11.5, behind 1,500, 22 MB, 12.2 and 14.3; 64 of 16 behind 64, 33 MB, 21.8 and 20.1, behind 128,
+// 66 MB, 23.1 and 25.4).  Plain form: 256 KB for every row and kv head, since the kernel without groups is slow at few rows of these
+// types (four float32 rows of 8 heads on 2 behind 500, 3 MB, 16.2 and 21.6; 32 of 28 on 4 behind 128, 16 MB, 30.0 and 26.0, behind
+// 256, 33 MB, 34.8 and 45.0), and half a tile of pairs a group (four rows of 16 on 16 behind 1,000, 49 MB, 21.1 and 16.3).
+NV_API int nv_attention_shared_pays(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, long long repeated) {
+  if (groups <= 0 || Hkv <= 0) return 0;
+  const long long saved = repeated * Hkv * D * 2 * (cache_dt == NV_DT_BF16 ? 2 : 4), parts = (long long)R * Hkv;
+  if (tc_takes(cache_dt, D, page)) return saved >= (16LL << 20) + 32768 * parts;
+  return saved >= 262144 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
 }
 
 NV_API int nv_attention_shared_usable(int D, int page) { return D >= 8 && D <= 256 && D % 8 == 0 && page >= 16 && page % 16 == 0; }
@@ -717,7 +745,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   const int slots = own_splits + shared_splits;
   const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc);
   const int per_tile = tc ? ST_PAIRS : SP_PAIRS;
-  const long long tiles = ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;         // (or fewer)
+  const long long tiles = shared_tiles(M, groups, Hq, Hkv, per_tile);
   if (shared_splits > 0 && groups > 0) {
     SharedArgs a;
     a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;

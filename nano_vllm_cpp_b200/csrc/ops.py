@@ -422,14 +422,15 @@ def attention_decode_usable(k_cache, D: int) -> bool:
 def attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale: float, window: int, out,
                      Hq: int, Hkv: int, D: int, max_context: int, rows=None, err=None, sink_score=None,
                      float_weights: bool = False, softcap: float = 0.0, gate=None, chunk: int = 0, slopes=None,
-                     bias_table=None) -> None:
+                     bias_table=None, clean: bool = False) -> None:
     """One query row per request (``rows``: which batch rows; None = all) against its paged keys.  ``qkv``: rows
     whose first Hq * D elements are the query heads.  ``sink_score``: a further key with that score and no value
     in every softmax.  ``float_weights``: the weights keep all their bits in the product with the values, as they always
     do with a sink (the tensor-core form takes them as three bfloat16 terms instead of one rounded one; the kernel that
     gives a lane a chunk of a key, which other head sizes, float32 caches and float32 queries beside a sink go to,
     multiplies in float32).  ``softcap`` > 0: a scaled score s becomes ``softcap * tanh(s / softcap)``.  ``gate``: see
-    ``_head_gates``.  ``chunk``, ``slopes``, ``bias_table``: see ``_score_bias``."""
+    ``_head_gates``.  ``chunk``, ``slopes``, ``bias_table``: see ``_score_bias``.  ``clean``: what lies behind a row's position
+    in its newest page may be anything, infinities and NaN too (else: any finite numbers)."""
     _cuda_contig(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows)
     _i32(block_table, row_entry, positions, rows)
     R = qkv.shape[0] if rows is None else rows.numel()
@@ -441,15 +442,13 @@ def attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, s
     if splits > 1:
         scratch = torch.empty(R * Hq * splits * (D + 2), dtype=torch.float32, device=qkv.device)
         counts = _split_counts(qkv.device)
-    _check(L.nv_attention_decode(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache),
-                                 dt(k_cache), _p(block_table), block_table.shape[1], _p(row_entry),
-                                 _p(positions), _p(rows), R, scale, window, _p(out),
-                                 dt(out), Hq, Hkv, D, page, k_cache.shape[0],
-                                 splits, _p(scratch), _p(err.t if err is not None else _global_err().t),
-                                 _p(counts), (counts.numel() if counts is not None else 0),
-                                 (0 if sink_score is None else 1), float(sink_score or 0.0),
-                                 (1 if float_weights else 0), float(softcap), *_head_gates(gate, qkv.shape[0], Hq),
-                                 *_score_bias(chunk, slopes, bias_table, Hq), _stream()), "attention_decode")
+    launch = L.nv_attention_decode_clean if clean else L.nv_attention_decode
+    _check(launch(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table), block_table.shape[1],
+                  _p(row_entry), _p(positions), _p(rows), R, scale, window, _p(out), dt(out), Hq, Hkv, D, page, k_cache.shape[0],
+                  splits, _p(scratch), _p(err.t if err is not None else _global_err().t), _p(counts),
+                  (counts.numel() if counts is not None else 0), (0 if sink_score is None else 1), float(sink_score or 0.0),
+                  (1 if float_weights else 0), float(softcap), *_head_gates(gate, qkv.shape[0], Hq),
+                  *_score_bias(chunk, slopes, bias_table, Hq), _stream()), "attention_decode")
 
 
 class SharedPrefix:
@@ -461,6 +460,7 @@ class SharedPrefix:
 
     def __init__(self, groups, rows: int, device):
         packed, self.members, self.longest = self.pack(groups, rows)
+        self.repeated = sum(n * (len(own) - 1) for own, n in groups)        # positions that are read once instead of again
         self.shortest = min((n for _, n in groups), default=0) if self.members == rows else 0      # what every row shares at least
         self.R, self.groups = rows, len(groups)
         self.bind(torch.tensor(packed, dtype=torch.int32).to(device))
@@ -493,11 +493,17 @@ def attention_decode_shared_usable(k_cache, D: int) -> bool:
     return bool(lib().nv_attention_shared_usable(D, k_cache.shape[2])) and attention_decode_usable(k_cache, D)
 
 
+def attention_sharing_pays(shared: SharedPrefix, Hq: int, Hkv: int, D: int, page: int, dtype) -> bool:
+    """Whether ``attention_decode_shared`` works the shared positions out once for these sizes, or has every row read its own."""
+    return bool(lib().nv_attention_shared_pays(shared.R, shared.members, shared.groups, Hq, Hkv, D, page, _DT[dtype], shared.repeated))
+
+
 def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, positions, scale: float, out, Hq: int, Hkv: int,
                             D: int, max_context: int, shared: SharedPrefix, rows=None, err=None, sink_score=None,
                             float_weights: bool = False, softcap: float = 0.0, gate=None) -> None:
     """``attention_decode`` for rows of which some share a prefix (``shared``): a group's shared keys and values are read once
-    for all its rows, as one product of their query heads, and joined with what each row has of its own.  A row sees the
+    for all its rows, as one product of their query heads, and joined with what each row has of its own, where that pays
+    (``attention_sharing_pays``; else ``attention_decode`` runs, and every row reads its keys itself).  A row sees the
     positions up to its own, none of them masked otherwise (layers with a window, chunks or biases by distance take
     ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``,
     ``gate``: see there.  As there, the kernel in front may write the query rows and each row's newest page, nothing else that
@@ -517,11 +523,14 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(shared.R == R, f"attention_decode_shared: {R} rows, and shared prefixes for {shared.R}")
     _need(scale > 0 and softcap >= 0, "attention_decode_shared: the scale is positive, a cap is not negative")
     _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
+    if not attention_sharing_pays(shared, Hq, Hkv, D, page, k_cache.dtype):
+        return attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, 0, out, Hq, Hkv, D, max_context,
+                                rows=rows, err=err, sink_score=sink_score, float_weights=float_weights, softcap=softcap, gate=gate, clean=True)
     L = lib()
     own = max(1, max_context - shared.shortest // page * page)              # the most keys a row reads for itself
-    splits = L.nv_attention_shared_own_splits(R, Hq, Hkv, own)
-    ours = L.nv_attention_shared_splits(shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache),
-                                        (1 if float_weights or sink_score is not None else 0), shared.longest)
+    sizes = shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache)
+    ours = L.nv_attention_shared_splits(*sizes, 1 if float_weights or sink_score is not None else 0, shared.longest)
+    splits = L.nv_attention_shared_own_splits(R, *sizes, ours, own)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
     _check(L.nv_attention_decode_shared(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table),
                                         block_table.shape[1], _p(row_entry), _p(positions), _p(rows), R, _p(shared.first),

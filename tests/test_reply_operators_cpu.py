@@ -57,6 +57,14 @@ def test_shared_prefix_packs_its_groups():
     assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0, 0)
 
 
+def test_sharing_is_a_matter_of_bytes_rows_and_heads():
+    pays = lambda R, M, g, Hq, Hkv, repeated, dt=1, D=128, page=16: ops.lib().nv_attention_shared_pays(R, M, g, Hq, Hkv, D, page, dt, repeated)
+    assert not pays(4, 0, 0, 16, 16, 0) and not pays(4, 4, 1, 16, 16, 0)
+    assert pays(64, 64, 1, 28, 4, 63 * 8192) and not pays(4, 4, 1, 16, 16, 3 * 496)
+    assert pays(4, 4, 1, 16, 16, 3 * 1500) and pays(4, 4, 1, 8, 2, 3 * 500, dt=0) and not pays(4, 4, 1, 16, 16, 3 * 500, dt=0)
+    assert pays(128, 128, 1, 28, 4, 1 << 40)                                 # (some 10^15 bytes)
+
+
 @pytest.mark.parametrize("groups", [[([], 16)], [([0], -1)], [([3], 16)], [([-1], 16)], [([0, 0], 16)], [([0], 16), ([1, 0], 16)]])
 def test_shared_prefix_refuses_groups(groups):
     with pytest.raises(ops.KernelError):

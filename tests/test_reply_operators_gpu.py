@@ -259,6 +259,16 @@ def test_page_copies_refuse():
 
 
 # ------------------------------------------------------------------------------------------------ attention
+@pytest.fixture(autouse=True, params=[True, False], ids=["shared", "as pays"])
+def sharing(request, monkeypatch):
+    """The tests' prefixes are short: they are shared whether or not that pays, and once more as it does."""
+    if "attention" not in request.node.name and "together" not in request.node.name:
+        if not request.param:
+            pytest.skip("no attention here")
+    elif request.param:
+        monkeypatch.setattr(ops(), "attention_sharing_pays", lambda shared, *a: shared.groups > 0)
+
+
 class Case:
     """Rows with tables, keys and values; ``groups``: (rows, shared positions), ``lengths``: positions of every row.  The pages that
     hold shared positions only are one page for the group; a page that a prefix ends in is each row's own, with the same content
