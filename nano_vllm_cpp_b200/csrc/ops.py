@@ -223,12 +223,14 @@ def _cuda_contig(*ts) -> None:
         _need(t.is_contiguous(), "tensor is not contiguous")
 
 
-def _here(*ts) -> None:
-    """The kernels run on the current device: a tensor of another one is refused."""
-    at = torch.cuda.current_device()
+def _ours(what: str, *ts) -> None:
+    """Contiguous tensors of the current device, where the kernels run (in one pass: a small operator's checks take longer than
+    its kernel)."""
+    at = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in ts:
-        if t is not None:
-            _need(t.device.index == at, f"tensor is on {t.device}, the current device is {at}")
+        if t is not None and (t.get_device() != at or not t.is_contiguous()):
+            _cuda_contig(t)
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is {at}")
 
 
 def _i32(*ts) -> None:
@@ -434,21 +436,26 @@ def attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, s
     _cuda_contig(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows)
     _i32(block_table, row_entry, positions, rows)
     R = qkv.shape[0] if rows is None else rows.numel()
-    page = k_cache.shape[2]
-    L = lib()
     seen = min([max_context] + [n for n in (window, chunk) if n > 0])        # the most keys a row reads
-    splits = L.nv_attention_decode_splits_of(R, Hq, Hkv, D, seen, num_sms())
+    splits = lib().nv_attention_decode_splits_of(R, Hq, Hkv, D, seen, num_sms())
+    _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, window, out, Hq, Hkv, D, R, splits, rows, err,
+                   sink_score, float_weights, softcap, gate, _score_bias(chunk, slopes, bias_table, Hq), clean)
+
+
+def _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, window, out, Hq, Hkv, D, R, splits, rows, err,
+                   sink_score, float_weights, softcap, gate, bias, clean) -> None:
+    """``attention_decode`` behind its checks, with R rows in so many splits."""
     scratch = counts = None
     if splits > 1:
         scratch = torch.empty(R * Hq * splits * (D + 2), dtype=torch.float32, device=qkv.device)
         counts = _split_counts(qkv.device)
-    launch = L.nv_attention_decode_clean if clean else L.nv_attention_decode
+    launch = lib().nv_attention_decode_clean if clean else lib().nv_attention_decode
     _check(launch(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table), block_table.shape[1],
-                  _p(row_entry), _p(positions), _p(rows), R, scale, window, _p(out), dt(out), Hq, Hkv, D, page, k_cache.shape[0],
-                  splits, _p(scratch), _p(err.t if err is not None else _global_err().t), _p(counts),
+                  _p(row_entry), _p(positions), _p(rows), R, scale, window, _p(out), dt(out), Hq, Hkv, D, k_cache.shape[2],
+                  k_cache.shape[0], splits, _p(scratch), _p(err.t if err is not None else _global_err().t), _p(counts),
                   (counts.numel() if counts is not None else 0), (0 if sink_score is None else 1), float(sink_score or 0.0),
-                  (1 if float_weights else 0), float(softcap), *_head_gates(gate, qkv.shape[0], Hq),
-                  *_score_bias(chunk, slopes, bias_table, Hq), _stream()), "attention_decode")
+                  (1 if float_weights else 0), float(softcap), *_head_gates(gate, qkv.shape[0], Hq), *bias, _stream()),
+           "attention_decode")
 
 
 class SharedPrefix:
@@ -462,7 +469,7 @@ class SharedPrefix:
         packed, self.members, self.longest = self.pack(groups, rows)
         self.repeated = sum(n * (len(own) - 1) for own, n in groups)        # positions that are read once instead of again
         self.shortest = min((n for _, n in groups), default=0) if self.members == rows else 0      # what every row shares at least
-        self.R, self.groups = rows, len(groups)
+        self.R, self.groups, self._splits = rows, len(groups), {}
         self.bind(torch.tensor(packed, dtype=torch.int32).to(device))
 
     @staticmethod
@@ -483,10 +490,25 @@ class SharedPrefix:
         return first + group + members + [0] * (rows - len(members)) + cu + lens + leads, len(members), max(lens, default=0)
 
     def bind(self, buf) -> None:
-        R, G = self.R, self.groups
+        R, G, at = self.R, self.groups, buf.data_ptr()
         self.buf = buf
-        self.first, self.group, self.rows_of, self.cu, self.lens, self.leads = (buf[a:b] for a, b in (
-            (0, R), (R, 2 * R), (2 * R, 3 * R), (3 * R, 3 * R + G + 1), (3 * R + G + 1, 3 * R + 2 * G + 1), (3 * R + 2 * G + 1, 3 * R + 3 * G + 1)))
+        self.places = tuple(at + 4 * n for n in (0, R, 2 * R, 3 * R, 3 * R + G + 1, 3 * R + 2 * G + 1))
+
+    def splits(self, Hq: int, Hkv: int, D: int, k_cache, terms: int, max_context: int):
+        """How many parts a row's own keys and the shared ones are cut into for these sizes (no shared part: 0), worked out
+        once for all layers that have them."""
+        page, dtype = k_cache.shape[2], k_cache.dtype
+        key = Hq, Hkv, D, page, dtype, terms, max_context
+        if key not in self._splits:
+            _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
+            pair = lib().nv_attention_decode_splits_of(self.R, Hq, Hkv, D, max_context, num_sms()), 0
+            if attention_sharing_pays(self, Hq, Hkv, D, page, dtype):
+                sizes = self.members, self.groups, Hq, Hkv, D, page, _DT[dtype]
+                own = max(1, max_context - self.shortest // page * page)          # the most keys a row reads for itself
+                ours = lib().nv_attention_shared_splits(*sizes, terms, self.longest)
+                pair = lib().nv_attention_shared_own_splits(self.R, *sizes, ours, own), ours
+            self._splits[key] = pair
+        return self._splits[key]
 
 
 def attention_decode_shared_usable(k_cache, D: int) -> bool:
@@ -508,37 +530,35 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``,
     ``gate``: see there.  As there, the kernel in front may write the query rows and each row's newest page, nothing else that
     is read here."""
-    _cuda_contig(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
+    _ours("attention_decode_shared", qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
     _i32(block_table, row_entry, positions, rows)
-    _here(qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
-    T = qkv.shape[0]
+    T, width = qkv.shape
     R = T if rows is None else rows.numel()
-    page = k_cache.shape[2]
+    dtype, shape = k_cache.dtype, k_cache.shape
     _need(Hq > 0 and Hkv > 0 and Hq % Hkv == 0, "attention_decode_shared: query heads are a multiple of kv heads")
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == Hkv and k_cache.shape[3] == D,
+    _need(len(shape) == 4 and shape == v_cache.shape and shape[1] == Hkv and shape[3] == D,
           "attention_decode_shared: keys and values are [pages, kv heads, slots, head size]")
-    _need(qkv.dtype == k_cache.dtype == v_cache.dtype == out.dtype, "attention_decode_shared: queries, cache and result have one type")
-    _need(qkv.dim() == 2 and qkv.shape[1] >= Hq * D and out.shape == (T, Hq * D) and positions.numel() == T and row_entry.numel() == T,
+    _need(qkv.dtype == dtype and v_cache.dtype == dtype and out.dtype == dtype,
+          "attention_decode_shared: queries, cache and result have one type")
+    _need(width >= Hq * D and out.shape == (T, Hq * D) and positions.numel() == T and row_entry.numel() == T,
           "attention_decode_shared: shapes")
-    _need(shared.R == R, f"attention_decode_shared: {R} rows, and shared prefixes for {shared.R}")
+    _need(shared.R == R, "attention_decode_shared: the shared prefixes are of another number of rows")
     _need(scale > 0 and softcap >= 0, "attention_decode_shared: the scale is positive, a cap is not negative")
-    _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
-    if not attention_sharing_pays(shared, Hq, Hkv, D, page, k_cache.dtype):
-        return attention_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, 0, out, Hq, Hkv, D, max_context,
-                                rows=rows, err=err, sink_score=sink_score, float_weights=float_weights, softcap=softcap, gate=gate, clean=True)
-    L = lib()
-    own = max(1, max_context - shared.shortest // page * page)              # the most keys a row reads for itself
-    sizes = shared.members, shared.groups, Hq, Hkv, D, page, dt(k_cache)
-    ours = L.nv_attention_shared_splits(*sizes, 1 if float_weights or sink_score is not None else 0, shared.longest)
-    splits = L.nv_attention_shared_own_splits(R, *sizes, ours, own)
+    page = shape[2]
+    terms = 1 if float_weights or sink_score is not None else 0
+    splits, ours = shared.splits(Hq, Hkv, D, k_cache, terms, max_context)
+    if ours == 0:
+        return _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, 0, out, Hq, Hkv, D, R, splits, rows, err,
+                              sink_score, float_weights, softcap, gate, (0, None, None, 0), True)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
-    _check(L.nv_attention_decode_shared(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table),
-                                        block_table.shape[1], _p(row_entry), _p(positions), _p(rows), R, _p(shared.first),
-                                        _p(shared.group), _p(shared.rows_of), shared.members, _p(shared.cu), _p(shared.lens), _p(shared.leads),
-                                        shared.groups, scale, _p(out), dt(out), Hq, Hkv, D, page, k_cache.shape[0], splits, ours,
-                                        _p(scratch), _p(err.t if err is not None else _global_err().t),
-                                        (0 if sink_score is None else 1), float(sink_score or 0.0), (1 if float_weights else 0),
-                                        float(softcap), *_head_gates(gate, T, Hq), _stream()), "attention_decode_shared")
+    code, first, group, members, cu, lens, leads = _DT[dtype], *shared.places
+    _check(lib().nv_attention_decode_shared(qkv.data_ptr(), code, width, k_cache.data_ptr(), v_cache.data_ptr(), code,
+                                            block_table.data_ptr(), block_table.shape[1], row_entry.data_ptr(), positions.data_ptr(),
+                                            _p(rows), R, first, group, members, shared.members, cu, lens, leads, shared.groups,
+                                            scale, out.data_ptr(), code, Hq, Hkv, D, page, shape[0], splits, ours, scratch.data_ptr(),
+                                            _p(err.t if err is not None else _global_err().t), (0 if sink_score is None else 1),
+                                            float(sink_score or 0.0), terms, float(softcap), *_head_gates(gate, T, Hq), _stream()),
+           "attention_decode_shared")
 
 
 def _score_bias(chunk: int, slopes, table, Hq: int):
@@ -1085,39 +1105,39 @@ def copy_pages(arrays: PageArrays, src, dst, slots=None, err=None) -> None:
     (int32 on the device; ``slots`` None: whole pages).  What lies behind the slots stays as it was.  The destinations are
     distinct and none of them is a source of another copy.  A page that the arrays do not have is not copied and sets the
     error flag."""
-    _cuda_contig(src, dst, slots)
+    _ours("copy_pages", arrays.table, src, dst, slots)
     _i32(src, dst, slots)
-    _here(arrays.table, src, dst, slots)
     N = src.numel()
     _need(dst.numel() == N and (slots is None or slots.numel() == N), "copy_pages: a source, a destination and slots per copy")
+    flag = _p(err.t if err is not None else _global_err().t)
     for at in range(0, N, 32768):               # (a grid has so many rows of blocks)
-        n = min(32768, N - at)
-        _check(lib().nv_copy_pages(_p(arrays.table), len(arrays.tensors), arrays.page_bytes, _p(src[at:at + n]), _p(dst[at:at + n]),
-                                   None if slots is None else _p(slots[at:at + n]), n,
-                                   _p(err.t if err is not None else _global_err().t), _stream()), "copy_pages")
+        _check(lib().nv_copy_pages(arrays.table.data_ptr(), len(arrays.tensors), arrays.page_bytes, src.data_ptr() + 4 * at,
+                                   dst.data_ptr() + 4 * at, None if slots is None else slots.data_ptr() + 4 * at, min(32768, N - at),
+                                   flag, _stream()), "copy_pages")
 
 
-def max_top_logprobs() -> int:
-    return int(lib().nv_token_logprobs_max_top())
+MAX_TOP_LOGPROBS = 32       # (a warp's lanes: csrc/logprobs.cu keeps a row's best in one)
 
 
 def token_logprobs(logits, tokens, logprob, *, entropy=None, rank=None, top_ids=None, top_logprobs=None, err=None) -> None:
     """Per row of ``logits`` [R, V] (float32 or bfloat16, rows of unit stride any distance apart): the log probability of
     ``tokens[r]`` under the row's softmax, into ``logprob`` [R]; the distribution's ``entropy`` [R] in nats; the token's ``rank`` [R],
     how many ids come before it in the order of (logit descending, id ascending); the first K ids of that order and their log
-    probabilities, ``top_ids`` and ``top_logprobs`` [R, K] (at most ``max_top_logprobs()``).  ``tokens`` and ``logprob`` may be None
+    probabilities, ``top_ids`` and ``top_logprobs`` [R, K] (at most ``MAX_TOP_LOGPROBS``).  ``tokens`` and ``logprob`` may be None
     for the rest alone.  Log probabilities and entropies are float32, ids and ranks int32.  Masked logits (minus infinity) have no part in
     the softmax; a row with a NaN, with plus infinity or with nothing above minus infinity has NaN for its numbers.  A
     token outside the vocabulary sets the error flag and gets NaN and the rank -1."""
     _need(logits.is_cuda and logits.dim() == 2 and logits.shape[1] > 0, "token_logprobs: logits [rows, vocabulary] on a CUDA device")
     R, V = logits.shape
-    _need(V == 1 or logits.stride(1) == 1, "token_logprobs: a row's logits are one after the other")
-    stride = logits.stride(0) if R > 1 else V
+    step, unit = logits.stride()
+    stride = step if R > 1 else V
+    _need(unit == 1 or V == 1, "token_logprobs: a row's logits are one after the other")
     _need(stride >= V, "token_logprobs: rows overlap")
-    _cuda_contig(tokens, logprob, entropy, rank, top_ids, top_logprobs)
+    _ours("token_logprobs", tokens, logprob, entropy, rank, top_ids, top_logprobs)
+    _need(logits.get_device() == (_raw_device() if _raw_device is not None else torch.cuda.current_device()),
+          "token_logprobs: the logits are on another device than the current one")
     _i32(tokens, rank, top_ids)
     _f32(logprob, entropy, top_logprobs)
-    _here(logits, tokens, logprob, entropy, rank, top_ids, top_logprobs)
     _need(tokens is not None or (logprob is None and rank is None), "token_logprobs: log probabilities and ranks are of tokens")
     for t in (tokens, logprob, entropy, rank):
         _need(t is None or t.numel() == R, "token_logprobs: one entry per row")
@@ -1126,7 +1146,7 @@ def token_logprobs(logits, tokens, logprob, *, entropy=None, rank=None, top_ids=
     if top_ids is not None:
         _need(top_ids.dim() == 2 and top_ids.shape[0] == R and top_ids.shape == top_logprobs.shape, "token_logprobs: alternatives are [rows, K]")
         K = top_ids.shape[1]
-        _need(K <= min(V, max_top_logprobs()), f"token_logprobs: at most {min(V, max_top_logprobs())} alternatives, found {K}")
+        _need(K <= V and K <= MAX_TOP_LOGPROBS, "token_logprobs: more alternatives than ids, or than MAX_TOP_LOGPROBS")
     _check(lib().nv_token_logprobs(_p(logits), dt(logits), stride, R, V, _p(tokens), _p(logprob), _p(entropy), _p(rank), K,
                                    _p(top_ids) if K else None, _p(top_logprobs) if K else None,
                                    _p(err.t if err is not None else _global_err().t), _stream()), "token_logprobs")

@@ -13,6 +13,7 @@ def logprobs(dt=0, stride=100, R=1, V=100, K=0, ids=None, lps=None):
 
 
 def test_log_probabilities_refuse_sizes():
+    assert ops.lib().nv_token_logprobs_max_top() == ops.MAX_TOP_LOGPROBS
     assert logprobs(R=0) == 0
     assert logprobs(dt=2) == BAD_DTYPE
     assert logprobs(R=-1) == BAD_SIZE
@@ -20,7 +21,7 @@ def test_log_probabilities_refuse_sizes():
     assert logprobs(stride=99) == BAD_SIZE
     assert logprobs(K=-1) == BAD_SIZE
     assert logprobs(K=5) == BAD_SIZE                                        # alternatives without a place for them
-    assert logprobs(K=ops.max_top_logprobs() + 1, ids=16, lps=16) == BAD_SIZE
+    assert logprobs(K=ops.MAX_TOP_LOGPROBS + 1, ids=16, lps=16) == BAD_SIZE
     assert logprobs(V=3, stride=3, K=4, ids=16, lps=16) == BAD_SIZE         # more alternatives than ids
 
 
