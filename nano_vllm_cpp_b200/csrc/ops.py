@@ -1109,11 +1109,8 @@ def copy_pages(arrays: PageArrays, src, dst, slots=None, err=None) -> None:
     _i32(src, dst, slots)
     N = src.numel()
     _need(dst.numel() == N and (slots is None or slots.numel() == N), "copy_pages: a source, a destination and slots per copy")
-    flag = _p(err.t if err is not None else _global_err().t)
-    for at in range(0, N, 32768):               # (a grid has so many rows of blocks)
-        _check(lib().nv_copy_pages(arrays.table.data_ptr(), len(arrays.tensors), arrays.page_bytes, src.data_ptr() + 4 * at,
-                                   dst.data_ptr() + 4 * at, None if slots is None else slots.data_ptr() + 4 * at, min(32768, N - at),
-                                   flag, _stream()), "copy_pages")
+    _check(lib().nv_copy_pages(arrays.table.data_ptr(), len(arrays.tensors), arrays.page_bytes, src.data_ptr(), dst.data_ptr(), _p(slots),
+                               N, _p(err.t if err is not None else _global_err().t), _stream()), "copy_pages")
 
 
 MAX_TOP_LOGPROBS = 32       # (a warp's lanes: csrc/logprobs.cu keeps a row's best in one)

@@ -28,7 +28,7 @@ def test_log_probabilities_refuse_sizes():
 def test_page_copies_refuse_sizes():
     call = lambda A, n, N: ops.lib().nv_copy_pages(None, A, n, None, None, None, N, None, None)
     assert call(0, 0, 5) == 0 and call(5, 64, 0) == 0
-    for bad in ((-1, 0, 1), (1, 0, -1), (1, -1, 1), (70000, 64, 1), (1, 64, 70000)):
+    for bad in ((-1, 0, 1), (1, 0, -1), (1, -1, 1), (70000, 64, 1), (1, 1 << 40, 1 << 30)):
         assert call(*bad) == BAD_SIZE
 
 
