@@ -13,6 +13,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Optional
 
+import numpy as np
 import torch
 
 from ..parts.base import KVCacheSpec, StateCacheSpec, CompositeCacheSpec, SharedCacheSpec
@@ -67,6 +68,11 @@ class DeviceCache:
     def _group(self, spec: KVCacheSpec) -> int:
         return self.windows.index(_group_key(spec))
 
+    def heads_of(self, group: int):
+        """kv heads and head size of a group's first layer."""
+        leaf = next(leaf for s in self.specs for leaf in _leaves(s) if isinstance(leaf, KVCacheSpec) and self._group(leaf) == group)
+        return leaf.num_kv_heads, leaf.head_dim
+
     def bytes_per_page(self) -> list:
         """Per group: bytes of one page over all its entries."""
         item = torch.empty((), dtype=self.dtype).element_size()
@@ -89,6 +95,7 @@ class DeviceCache:
             num_pages = [num_pages] * len(self.windows)
         self.num_pages = list(num_pages)
         self.views = []
+        self._arrays = {}                          # group, or ("state", dtype) -> ops.PageArrays
         self.max_blocks = max_blocks
         self.tables = self.step_tables = None
         if max_blocks > 0:
@@ -149,6 +156,49 @@ class DeviceCache:
     @property
     def has_state(self) -> bool:
         return any(isinstance(leaf, StateCacheSpec) for s in self.specs for leaf in _leaves(s))
+
+    def copy_forks(self, forks: list, stager) -> None:
+        """Makes the copies that forked requests begin with (``CacheManager.fork``), on the current stream: part-full pages in
+        every layer of their group, and the state slots, a launch per group and per state buffer.  ``stager``: brings the
+        index arrays to the device in one copy."""
+        from ..csrc import ops
+        if not forks:
+            return
+        pages = [[p for f in forks for p in f.pages if p[0] == g] for g in range(len(self.windows))]
+        flat = [x for g in pages for k in (1, 2, 3) for x in [p[k] for p in g]]
+        flat += [f.slot_from for f in forks] + [f.slot_to for f in forks]
+        at, n = 0, len(flat)
+        dev = stager.stage(np.array(flat, dtype=np.int32))
+
+        def take(k):
+            nonlocal at
+            at += k
+            return dev[at - k:at]
+
+        for g, copies in enumerate(pages):
+            if copies:
+                src, dst, slots = take(len(copies)), take(len(copies)), take(len(copies))
+                ops.copy_pages(self._page_arrays(g), src, dst, slots=slots)
+        src, dst = take(len(forks)), take(len(forks))
+        assert at == n
+        for dt, buf in self.state_buffers.items():
+            if ("state", dt) not in self._arrays:
+                self._arrays["state", dt] = ops.PageArrays([buf])
+            ops.copy_pages(self._arrays["state", dt], src, dst)
+
+    def _page_arrays(self, group: int):
+        """The key and value arrays of a group's layers, described for ``ops.copy_pages``."""
+        from ..csrc import ops
+        if group not in self._arrays:
+            found, queue = [], [v for v in self.views if v is not None]
+            while queue:
+                v = queue.pop(0)
+                if v.parts is not None:
+                    queue += v.parts
+                elif v.kind == "kv" and v.group == group and v.write:
+                    found += [v.k] + ([v.v] if v.v is not None else [])
+            self._arrays[group] = ops.PageArrays(found)
+        return self._arrays[group]
 
     def sync_tables(self, batch) -> None:
         """Before a step runs: the block tables of its entries, in entry order, are put together on the device

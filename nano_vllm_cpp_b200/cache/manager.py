@@ -17,6 +17,7 @@ their early pages back.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import numpy as np
 
@@ -26,6 +27,14 @@ from .block_pool import BlockPool, NoFreePages
 
 class NoFreeSlot(RuntimeError):
     pass
+
+
+@dataclass
+class Fork:
+    """What a fork leaves to copy on the device: the state slot, and per copied page (group, page, page, slots of it)."""
+    slot_from: int
+    slot_to: int
+    pages: list
 
 
 class RequestCache:
@@ -165,6 +174,38 @@ class CacheManager:
         if rc:
             self._raise(rc)
         self._ids.pop(rid, None)
+
+    def fork(self, rid, new) -> "Fork":
+        """Opens ``new`` with the cache of ``rid`` as it is: full pages are shared, a page that is part full and the state slot
+        are to be copied on the device before either request's next step (``DeviceCache.copy_forks``).  Raises ``NoFreeSlot`` or
+        ``NoFreePages`` and changes nothing where one is missing."""
+        parent = self._id(rid)
+        known = new in self._ids if not isinstance(new, int) else True
+        h = self._native(new, create=True)
+        out = (ctypes.c_int * (3 + 4 * self.num_groups))()
+        rc = host.lib().nvh_fork(self._h, parent, h, out)
+        if rc:
+            if not known:
+                self._ids.pop(new, None)
+            if rc == host.ERR_STATE:
+                raise RuntimeError(f"request {new!r}: {host.last_error()}")
+            self._raise(rc)
+        return Fork(out[0], out[1], [tuple(out[3 + 4 * i:7 + 4 * i]) for i in range(out[2])])
+
+    def shared_prefixes(self, rids: list, group: int) -> list:
+        """Which of these requests begin with the same full pages of a group: (places in ``rids``, positions in common) per
+        set of two or more, in the order of their first members."""
+        S = len(rids)
+        ids = (ctypes.c_int64 * max(S, 1))(*[self._native(r) for r in rids])
+        group_of, pages = (ctypes.c_int * max(S, 1))(), (ctypes.c_int * max(S, 1))()
+        n = host.lib().nvh_shared_prefixes(self._h, S, ids, group, group_of, pages)
+        if n < 0:
+            raise RuntimeError(host.last_error())
+        out = [([], pages[k] * self.page_size) for k in range(n)]
+        for i in range(S if n else 0):
+            if group_of[i] >= 0:
+                out[group_of[i]][0].append(i)
+        return out
 
     # ------------------------------------------------------------------ pages
     def pages_needed(self, rid, start: int, end: int) -> list:

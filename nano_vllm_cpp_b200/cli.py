@@ -12,6 +12,9 @@ here.  ``--expert-budget`` is accepted and ignored: every expert stays resident 
 ``--top-p``, ``--rep-penalty`` and ``--rep-window`` are those of the reference's second command line
 (src/main_vulkan.cpp:260-298): nucleus sampling, and the scores of ids among the last W completion tokens
 divided by THETA (1.0 = off, W = 0: the whole completion).
+``--n`` draws several replies to the prompt, which runs once; ``--logprobs K`` prints every token's log probability, rank and the
+distribution's entropy, and the K likeliest ids; ``--score`` does so for the given tokens and draws none; ``--shared-prefix``
+has decoded rows that begin with the same pages read them once.
 ``temperature``, ``top_p`` and ``max_new_tokens`` of the model folder's ``generation_config.json`` are the
 defaults of the options that are not given (src/main_vulkan.cpp:360-363).
 Exit codes as the reference's: 1 usage, 2 error (src/main.cpp:432-438).
@@ -28,6 +31,8 @@ USAGE = """Usage: nanovllm <model_dir> --tokens 1,2,3 [--max-tokens N] [--temper
                    --page-size N  --prefill-chunk N  --max-num-batched-tokens N  --max-num-seqs N
                    --eos ID  --ignore-eos  --expert-budget GB (ignored)
                    --top-p P  --rep-penalty THETA  --rep-window W   (nucleus sampling and repetition penalty)
+                   --n N  (replies to the prompt)  --logprobs K  (log probabilities, K likeliest ids)  --shared-prefix
+                   --score  (log probabilities of the given tokens instead of a reply)
 """
 
 
@@ -67,7 +72,8 @@ def main(argv=None) -> int:
     opt = dict(model_dir="", prompt="", prompt_ids=[], max_tokens=64, temperature=0.6, max_model_len=4096,
                bench=False, num_seqs=4, num_kv_blocks=0, dtype="bfloat16", random_weights=False, seed=0,
                page_size=16, prefill_chunk=0, max_num_batched_tokens=16384, max_num_seqs=512, eos=-1,
-               ignore_eos=False, top_p=1.0, rep_penalty=1.0, rep_window=64, config="")
+               ignore_eos=False, top_p=1.0, rep_penalty=1.0, rep_window=64, config="", n=1, logprobs=None,
+               shared_prefix=False, score=False)
     with_value = {"--tokens": ("prompt_ids", parse_ids), "--max-tokens": ("max_tokens", int),
                   "--temperature": ("temperature", float), "--max-model-len": ("max_model_len", int),
                   "--num-kv-blocks": ("num_kv_blocks", int), "--expert-budget": (None, float),
@@ -76,7 +82,7 @@ def main(argv=None) -> int:
                   "--max-num-batched-tokens": ("max_num_batched_tokens", int),
                   "--max-num-seqs": ("max_num_seqs", int), "--eos": ("eos", int), "--top-p": ("top_p", float),
                   "--rep-penalty": ("rep_penalty", float), "--rep-window": ("rep_window", int),
-                  "--config": ("config", str)}
+                  "--config": ("config", str), "--n": ("n", int), "--logprobs": ("logprobs", int)}
     i = 0
     given = set()
     try:
@@ -94,6 +100,8 @@ def main(argv=None) -> int:
                 opt["random_weights"] = True
             elif a == "--ignore-eos":
                 opt["ignore_eos"] = True
+            elif a in ("--shared-prefix", "--score"):
+                opt[a[2:].replace("-", "_")] = True
             elif a in ("--chat", "--server", "--host", "--port"):
                 sys.stderr.write(f"Error: {a} belongs to the chat/server front ends, which this engine does not have\n")
                 return 2
@@ -148,10 +156,11 @@ def _run(opt) -> int:
     engine = LLMEngine(opt["model_dir"], opt["max_model_len"], opt["num_kv_blocks"], dtype=opt["dtype"],
                        random_weights=opt["random_weights"], seed=opt["seed"], kvcache_block_size=opt["page_size"],
                        prefill_chunk=opt["prefill_chunk"], max_num_batched_tokens=opt["max_num_batched_tokens"],
-                       max_num_seqs=opt["max_num_seqs"], eos=opt["eos"])
+                       max_num_seqs=opt["max_num_seqs"], eos=opt["eos"], shared_prefix=opt["shared_prefix"])
     sp = SamplingParams(temperature=opt["temperature"], max_tokens=opt["max_tokens"],
                         ignore_eos=opt["ignore_eos"] or opt["bench"], top_p=opt["top_p"],
-                        repetition_penalty=opt["rep_penalty"], repetition_window=opt["rep_window"])
+                        repetition_penalty=opt["rep_penalty"], repetition_window=opt["rep_window"], n=opt["n"],
+                        logprobs=opt["logprobs"])
     if opt["bench"]:
         # synthetic prompts of 64 ids, 1 + ((i*37 + t) % (V-2))  (src/main.cpp:388-412)
         import torch
@@ -178,10 +187,23 @@ def _run(opt) -> int:
         if tg_secs > 0 and gen > 0:
             print(f"decode: {gen} tokens / {tg_secs:.3f}s = {gen / tg_secs:.1f} tok/s")
         return 0
+    if opt["score"]:
+        scores = engine.score([opt["prompt_ids"]], opt["logprobs"] or 0)[0]
+        _print_scores(scores)
+        print(f"sum: {sum(s.logprob for s in scores):.6f}")
+        return 0
     outs = engine.generate([opt["prompt_ids"]], [sp])
     for o in outs:
-        print("token_ids: " + " ".join(str(t) for t in o["token_ids"]))
+        for reply in o.get("replies", [o]):
+            print("token_ids: " + " ".join(str(t) for t in reply["token_ids"]))
+            _print_scores(reply.get("logprobs", []))
     return 0
+
+
+def _print_scores(scores) -> None:
+    for s in scores:
+        top = " ".join(f"{t}:{p:.4f}" for t, p in s.top)
+        print(f"  {s.token}: {s.logprob:.6f} rank {s.rank} entropy {s.entropy:.4f}" + (f" | {top}" if top else ""))
 
 
 if __name__ == "__main__":

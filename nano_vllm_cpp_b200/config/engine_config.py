@@ -6,6 +6,9 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 
+MAX_LOGPROBS = 32       # likeliest ids per token, what the kernel keeps (csrc/logprobs.cu)
+
+
 @dataclass
 class EngineConfig:
     model: str = ""
@@ -20,6 +23,9 @@ class EngineConfig:
     seed: int = 0                         # base seed of per-request sampling streams
     prefill_chunk: int = 0                # 0 = portions limited by the token budget only
     enable_prefix_caching: bool = True
+    # decoded rows that begin with the same pages (replies to one prompt, requests behind one system prompt) read them once:
+    # bfloat16 runs, layers without a window.  Off by default: a row's sums then do not depend on its neighbours
+    shared_prefix: bool = False
     cuda_graphs: bool = True
     run_ahead: bool = True                # launch a step before the host has read the tokens of the one before
     device: str = "cuda:0"
@@ -58,6 +64,12 @@ class SamplingParams:
     top_p: float = 1.0
     repetition_penalty: float = 1.0       # scores of ids among the recent completion tokens are divided by it
     repetition_window: int = 64           # how many of the latest completion tokens count; 0 = all of them
+    # Replies to one prompt, which runs once: each further reply begins with a fork of its cache and draws from the stream
+    # of its own seed (``seed`` + its number, where a seed is given).
+    n: int = 1
+    # None: off.  Otherwise every token comes with its log probability, rank and the distribution's entropy, and with so many
+    # of the likeliest ids (0: none), under the model's distribution at temperature 1.
+    logprobs: int | None = None
 
     def validate(self) -> None:
         if self.temperature < 0:
@@ -70,3 +82,7 @@ class SamplingParams:
             raise ValueError("repetition_penalty must be at least 0.001 (1 = off)")
         if self.repetition_window < 0:
             raise ValueError("repetition_window cannot be negative (0 = the whole completion)")
+        if self.n < 1:
+            raise ValueError("n must be positive")
+        if self.logprobs is not None and not 0 <= self.logprobs <= MAX_LOGPROBS:
+            raise ValueError(f"logprobs must lie in 0 .. {MAX_LOGPROBS}")

@@ -38,6 +38,8 @@ _PROTOS = {
     "nvh_manager_num_requests": (c_int, [c_void_p]),
     "nvh_has": (c_int, [c_void_p, c_int64]),
     "nvh_open": (c_int, [c_void_p, c_int64]),
+    "nvh_fork": (c_int, [c_void_p, c_int64, c_int64, _IP]),
+    "nvh_shared_prefixes": (c_int, [c_void_p, c_int, _LP, c_int, _IP, _IP]),
     "nvh_close": (c_int, [c_void_p, c_int64]),
     "nvh_extend": (c_int, [c_void_p, c_int64, c_int, c_int]),
     "nvh_can_extend": (c_int, [c_void_p, c_int64, c_int, c_int]),
@@ -57,6 +59,7 @@ _PROTOS = {
     "nvs_create": (c_void_p, [c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "nvs_destroy": (None, [c_void_p]),
     "nvs_add": (c_int, [c_void_p, c_int64, _IP, c_int, c_int, c_int, c_int]),
+    "nvs_add_reply": (c_int, [c_void_p, c_int64, _IP, c_int, c_int, c_int, c_int]),
     "nvs_is_finished": (c_int, [c_void_p]),
     "nvs_num_preemptions": (c_int, [c_void_p]),
     "nvs_queue_sizes": (c_int, [c_void_p, _IP, _IP]),

@@ -348,6 +348,89 @@ class CacheManager {
       if (pools[0].ref_count[pages[i]] == 0) ++revived;
     return total - n + revived;
   }
+  // Another request with the cache of `parent` as it is: it shares the pages that are full and takes one of its own, in every
+  // group, for the page that is part full, whose first slots the caller copies on the device, as it copies the state slot.  out:
+  // the parent's slot, the child's slot, the number of page copies, and (group, page, page, slots) for each of them.  Nothing
+  // changes where pages or slots are missing.
+  int fork(int64_t parent, int64_t child, int* out) {
+    RequestCache* from = find(parent);
+    if (!from) return fail(ERR_STATE, "request is not open");
+    if (requests.count(child)) return fail(ERR_STATE, "request is already open");
+    if (free_slots.empty()) return fail(ERR_NO_SLOT, "no free state slot");
+    const int full = from->num_tokens / page_size, part = from->num_tokens % page_size;
+    for (size_t g = 0; g < pools.size(); ++g)
+      if (part && full < (int)from->tables[g].size() && from->tables[g][full] >= 0 && pools[g].n_free < 1)
+        return fail(ERR_NO_PAGES, "no free blocks");
+    RequestCache rc = *from;
+    rc.rid = child;
+    rc.slot = free_slots.back();
+    free_slots.pop_back();
+    rc.dirty.assign(pools.size(), 1);
+    int copies = 0;
+    for (size_t g = 0; g < pools.size(); ++g) {
+      auto& table = rc.tables[g];
+      if ((int)table.size() > full + (part ? 1 : 0)) table.resize(full + (part ? 1 : 0));      // (pages taken for rows that never ran)
+      for (int i = 0; i < (int)table.size(); ++i) {
+        if (table[i] < 0) continue;                                                          // given back
+        if (i < full) {
+          const int r = pools[g].share(table[i]);
+          if (r) return r;
+        } else {
+          const int mine = pools[g].allocate();
+          out[3 + 4 * copies] = (int)g;
+          out[4 + 4 * copies] = table[i];
+          out[5 + 4 * copies] = mine;
+          out[6 + 4 * copies] = part;
+          ++copies;
+          table[i] = mine;
+        }
+      }
+    }
+    out[0] = from->slot;
+    out[1] = rc.slot;
+    out[2] = copies;
+    requests.emplace(child, std::move(rc));
+    return OK;
+  }
+  // Which of S open requests begin with the same pages of group g?  group_of[i]: the number of entry i's group, or -1; pages[k]: how
+  // many pages the entries of group k have in common, one at least.  Returns the number of groups, each of two entries or more.
+  int shared_prefixes(int S, const int64_t* rids, int g, int* group_of, int* pages) const {
+    std::unordered_map<int, int> by_page;                    // first page -> the first entry that has it
+    std::vector<const std::vector<int>*> tables(S, nullptr);
+    std::vector<int> lead(S, -1), common(S, 0), members(S, 0);
+    for (int i = 0; i < S; ++i) {
+      group_of[i] = -1;
+      auto it = requests.find(rids[i]);
+      if (it == requests.end()) return fail(ERR_STATE, "request is not open");
+      tables[i] = &it->second.tables[g];
+      const int full = it->second.num_tokens / page_size;    // (a page that is still being written is nobody else's)
+      if (full < 1 || tables[i]->empty() || (*tables[i])[0] < 0) continue;
+      const int l = by_page.emplace((*tables[i])[0], i).first->second;
+      lead[i] = l;
+      ++members[l];
+      int n = std::min(full, (int)tables[i]->size());
+      if (l != i) {
+        n = std::min(n, common[l]);
+        const int* a = tables[l]->data();
+        const int* b = tables[i]->data();
+        int k = 0;
+        while (k < n && a[k] == b[k]) ++k;
+        n = k;
+      }
+      common[l] = n;
+    }
+    int groups = 0;
+    std::vector<int> number(S, -1);
+    for (int i = 0; i < S; ++i) {
+      if (lead[i] < 0 || members[lead[i]] < 2) continue;
+      if (number[lead[i]] < 0) {
+        pages[groups] = common[lead[i]];
+        number[lead[i]] = groups++;
+      }
+      group_of[i] = number[lead[i]];
+    }
+    return groups;
+  }
   // The device's copies of the block tables can no longer be trusted (a step was prepared but never ran): every
   // request's tables travel again with its next step.
   void touch_all() {
@@ -597,6 +680,12 @@ NVH_API int nvh_manager_free_slots(void* m) { return (int)((CacheManager*)m)->fr
 NVH_API int nvh_manager_num_requests(void* m) { return (int)((CacheManager*)m)->requests.size(); }
 NVH_API int nvh_has(void* m, int64_t rid) { return ((CacheManager*)m)->find(rid) ? 1 : 0; }
 NVH_API int nvh_open(void* m, int64_t rid) { return ((CacheManager*)m)->open(rid); }
+NVH_API int nvh_fork(void* m, int64_t parent, int64_t child, int* out) { return ((CacheManager*)m)->fork(parent, child, out); }
+NVH_API int nvh_shared_prefixes(void* m, int S, const int64_t* rids, int g, int* group_of, int* pages) {
+  CacheManager* cm = (CacheManager*)m;
+  if (g < 0 || g >= (int)cm->pools.size()) return fail(ERR_STATE, "no such cache group");
+  return cm->shared_prefixes(S, rids, g, group_of, pages);
+}
 NVH_API int nvh_close(void* m, int64_t rid) { return ((CacheManager*)m)->close(rid); }
 NVH_API int nvh_extend(void* m, int64_t rid, int start, int end) { return ((CacheManager*)m)->extend(rid, start, end); }
 NVH_API int nvh_can_extend(void* m, int64_t rid, int start, int end) {
@@ -801,6 +890,21 @@ NVH_API int nvs_add(void* s, int64_t seq_id, const int* tokens, int n, int num_p
   Seq* raw = q.get();
   sc.seqs.emplace(seq_id, std::move(q));
   sc.waiting.push_back(raw);
+  return OK;
+}
+// A further reply to a prompt that has run: its sequence (the prompt and the reply's first token) goes on where the forked request
+// `seq_id` of the manager ends, in the running queue; without one (no page or slot was free) it waits for its turn like a
+// preempted sequence and runs its prompt again.
+NVH_API int nvs_add_reply(void* s, int64_t seq_id, const int* tokens, int n, int num_prompt, int max_tokens, int ignore_eos) {
+  Scheduler& sc = ((SchedHandle*)s)->s;
+  const int rc = nvs_add(s, seq_id, tokens, n, num_prompt, max_tokens, ignore_eos);
+  if (rc) return rc;
+  Seq* q = sc.seqs[seq_id].get();
+  if (sc.m->find(seq_id)) {
+    sc.waiting.pop_back();
+    q->status = 1;
+    sc.running.push_back(q);
+  }
   return OK;
 }
 NVH_API int nvs_is_finished(void* s) { return ((SchedHandle*)s)->s.finished() ? 1 : 0; }

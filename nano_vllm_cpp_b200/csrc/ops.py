@@ -465,17 +465,25 @@ class SharedPrefix:
     values at their first so many positions, each in pages of its own or in common ones; whole pages of them are read through
     the block table of the first of them.  A row is in one group at most; the others read all their keys themselves."""
 
-    def __init__(self, groups, rows: int, device):
-        packed, self.members, self.longest = self.pack(groups, rows)
-        self.repeated = sum(n * (len(own) - 1) for own, n in groups)        # positions that are read once instead of again
-        self.shortest = min((n for _, n in groups), default=0) if self.members == rows else 0      # what every row shares at least
+    def __init__(self, groups, rows: int, device, *, facts=None, buf=None):
+        """``facts`` (longest prefix, what every row shares at least, positions that are read once instead of again): what the
+        launches go by, where other steps of the same shape are to run the same ones.  ``buf``: the packed arrays where they
+        are on the device already (``pack``)."""
+        packed, self.members = self.pack(groups, rows)
         self.R, self.groups, self._splits = rows, len(groups), {}
-        self.bind(torch.tensor(packed, dtype=torch.int32).to(device))
+        self.longest, self.shortest, self.repeated = self.facts(groups, rows) if facts is None else facts
+        self.bind(torch.tensor(packed, dtype=torch.int32).to(device) if buf is None else buf)
+
+    @staticmethod
+    def facts(groups, rows: int):
+        lens = [n for _, n in groups]
+        whole = sum(len(own) for own, _ in groups) == rows
+        return max(lens, default=0), min(lens, default=0) if whole else 0, sum(n * (len(own) - 1) for own, n in groups)
 
     @staticmethod
     def pack(groups, rows: int):
         """The host's arrays in one list: per row its shared positions and its group (or -1), the groups' rows one after the
-        other (``rows`` places), where each group's start, its positions, and its first row; the number of grouped rows; the longest prefix."""
+        other (``rows`` places), where each group's start, its positions, and its first row; and the number of grouped rows."""
         first, group, members, cu, lens = [0] * rows, [-1] * rows, [], [0], []
         for g, (own, n) in enumerate(groups):
             _need(len(own) > 0 and n >= 0, "SharedPrefix: a group has a row at least and no negative prefix")
@@ -487,7 +495,7 @@ class SharedPrefix:
             cu.append(len(members))
             lens.append(int(n))
         leads = [int(own[0]) for own, _ in groups]
-        return first + group + members + [0] * (rows - len(members)) + cu + lens + leads, len(members), max(lens, default=0)
+        return first + group + members + [0] * (rows - len(members)) + cu + lens + leads, len(members)
 
     def bind(self, buf) -> None:
         R, G, at = self.R, self.groups, buf.data_ptr()
@@ -502,7 +510,7 @@ class SharedPrefix:
         if key not in self._splits:
             _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
             pair = lib().nv_attention_decode_splits_of(self.R, Hq, Hkv, D, max_context, num_sms()), 0
-            if attention_sharing_pays(self, Hq, Hkv, D, page, dtype):
+            if attention_sharing_pays(self.R, self.members, self.groups, Hq, Hkv, D, page, dtype, self.repeated):
                 sizes = self.members, self.groups, Hq, Hkv, D, page, _DT[dtype]
                 own = max(1, max_context - self.shortest // page * page)          # the most keys a row reads for itself
                 ours = lib().nv_attention_shared_splits(*sizes, terms, self.longest)
@@ -515,9 +523,10 @@ def attention_decode_shared_usable(k_cache, D: int) -> bool:
     return bool(lib().nv_attention_shared_usable(D, k_cache.shape[2])) and attention_decode_usable(k_cache, D)
 
 
-def attention_sharing_pays(shared: SharedPrefix, Hq: int, Hkv: int, D: int, page: int, dtype) -> bool:
-    """Whether ``attention_decode_shared`` works the shared positions out once for these sizes, or has every row read its own."""
-    return bool(lib().nv_attention_shared_pays(shared.R, shared.members, shared.groups, Hq, Hkv, D, page, _DT[dtype], shared.repeated))
+def attention_sharing_pays(rows: int, members: int, groups: int, Hq: int, Hkv: int, D: int, page: int, dtype, repeated: int) -> bool:
+    """Whether ``attention_decode_shared`` works the shared positions out once, or has every row read its own: ``members`` of the
+    rows in so many groups, ``repeated`` positions that need not be read again."""
+    return bool(lib().nv_attention_shared_pays(rows, members, groups, Hq, Hkv, D, page, _DT[dtype], repeated))
 
 
 def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, positions, scale: float, out, Hq: int, Hkv: int,

@@ -53,6 +53,7 @@ class StepBatch:
     uniforms: torch.Tensor = None       # [n_want] float64
     native_ids: object = None           # the entries' request ids as the native cache manager knows them
     table_updates: list = None          # per group (src [S], len [S], rows [n, max_blocks]): see batch_layout
+    shared: object = None               # ops.SharedPrefix: which of the single rows share a prefix, where the step looks for them
 
 
 def _align4(n: int) -> int:

@@ -12,12 +12,13 @@ from __future__ import annotations
 import os
 from dataclasses import dataclass, field
 
-from ..config.engine_config import EngineConfig, SamplingParams
+from ..cache import NoFreePages, NoFreeSlot
+from ..config.engine_config import EngineConfig, MAX_LOGPROBS, SamplingParams
 from ..sampling import Sampler, uniform
 from .batch import StepEntry
 from .runner import ModelRunner
 from .scheduler import Scheduler
-from .sequence import Sequence
+from .sequence import Sequence, SequenceStatus
 
 
 @dataclass
@@ -26,6 +27,7 @@ class StepOutput:
     num_prefill_tokens: int = 0
     num_decode_tokens: int = 0
     new_tokens: list = field(default_factory=list)  # [(seq_id, token)] for every token drawn this step
+    logprobs: list = field(default_factory=list)    # [(seq_id, TokenLogprob)] where SamplingParams.logprobs asks for them
 
 
 class _Pending:
@@ -35,6 +37,8 @@ class _Pending:
         self.scheduled, self.sampled_seqs, self.handle = scheduled, sampled_seqs, handle
         self.n_prefill, self.n_decode = n_prefill, n_decode
         self.finished = []          # sequences that the stand-in bookkeeping ended (by length)
+        self.replies = []           # further replies whose first tokens this step draws, in the order of their tokens
+        self.scored = False         # the step works out log probabilities
         self.places = None          # per sampled row: index of its stand-in in the sequence's tokens, or None
 
 
@@ -57,7 +61,7 @@ class LLMEngine:
             max_requests=cfg.max_num_seqs, max_model_len=cfg.max_model_len, device=cfg.device,
             random_seed=cfg.seed if random_weights else None, norm_std=norm_std, std=std,
             gpu_memory_utilization=cfg.gpu_memory_utilization, prefix_caching=cfg.enable_prefix_caching,
-            cuda_graphs=cfg.cuda_graphs, log_stats=cfg.log_stats)
+            cuda_graphs=cfg.cuda_graphs, log_stats=cfg.log_stats, shared_prefix=cfg.shared_prefix)
         mc = self.runner.config
         max_pos = getattr(mc, "max_position_embeddings", None)
         if max_pos:                                              # include/nanovllm/config.hpp:269
@@ -73,6 +77,7 @@ class LLMEngine:
             self._warm_up()
         self._pending = None
         self._nucleus_live = set()      # ids of live requests that are sampled by the nucleus rule
+        self._to_fork = set()           # ids of requests whose further replies wait for their prompt
 
     def _warm_up(self) -> None:
         """The largest step the scheduler can ask for runs once before the first request: what its activations
@@ -115,6 +120,8 @@ class LLMEngine:
         return self.config.eos
 
     def add_request(self, prompt_ids, sampling: SamplingParams | None = None) -> int:
+        """Queues a request and returns its id.  With ``SamplingParams.n`` > 1 its further replies have the ids behind it and
+        join the running requests with the step that completes the prompt."""
         sp = sampling or SamplingParams()
         sp.validate()
         ids = [int(t) for t in prompt_ids]
@@ -125,10 +132,14 @@ class LLMEngine:
         bad = [t for t in ids if not (0 <= t < self.vocab_size)]
         if bad:
             raise ValueError(f"token id {bad[0]} is outside the vocabulary [0, {self.vocab_size})")
+        if sp.logprobs is not None and sp.logprobs > self.vocab_size:
+            raise ValueError(f"logprobs {sp.logprobs} is more than the vocabulary's {self.vocab_size} ids")
         seq = Sequence(ids, sp, base_seed=self.config.seed)
         self.scheduler.add(seq)
         if seq.nucleus_sampling:
             self._nucleus_live.add(seq.seq_id)
+        if seq.replies:
+            self._to_fork.add(seq.seq_id)
         return seq.seq_id
 
     # ------------------------------------------------------------------ one step
@@ -148,7 +159,8 @@ class LLMEngine:
         cur, nxt = self._pending, None
         # (a request under the nucleus rule needs its latest tokens on the host for the repetition penalty:
         # while one is live, steps run in the plain order)
-        if self.config.run_ahead and not self._nucleus_live:
+        # (nor from before a prompt whose replies begin with forks of its cache until their first tokens are there)
+        if self.config.run_ahead and not self._nucleus_live and not self._to_fork and not cur.replies:
             self._stand_ins(cur)
             nxt = self._launch()
         tokens = self.runner.collect(cur.handle)
@@ -161,6 +173,7 @@ class LLMEngine:
             return None
         entries, temps, us, sampled_seqs, nucleus = [], [], [], [], []
         n_prefill = n_decode = 0
+        again, replies, parents = [], [], []
         for s in scheduled:
             toks = s.seq.token_ids[s.start:s.start + s.count]
             entries.append(StepEntry(s.seq.seq_id, toks, [s.count - 1] if s.samples else []))
@@ -171,12 +184,30 @@ class LLMEngine:
                 sampled_seqs.append(s.seq)
                 nucleus.append((s.seq.top_p, s.seq.repetition_penalty, s.seq.recent_token_ids)
                                if s.seq.nucleus_sampling else None)
+                if not s.seq.forked:                                # the prompt is through: its replies draw from the same logits
+                    parents.append(s.seq)
+                    for q in s.seq.replies:
+                        again.append((len(temps) - 1, q.temperature, uniform(q.seed, 0) if q.temperature > 0 else 0.0,
+                                      (q.top_p, q.repetition_penalty, []) if q.nucleus_sampling else None))
+                        replies.append(q)
             if s.count == 1 and s.start >= s.seq.num_prompt_tokens:
                 n_decode += 1
             else:
                 n_prefill += s.count
-        handle = self.runner.launch_tokens(entries, temps, us, nucleus if any(x is not None for x in nucleus) else None)
-        return _Pending(scheduled, sampled_seqs, handle, n_prefill, n_decode)
+        asked = [q.logprobs for q in sampled_seqs + replies if q.logprobs is not None]
+        handle = self.runner.launch_tokens(entries, temps, us, nucleus if any(x is not None for x in nucleus) else None,
+                                           again=again or None, logprobs=max(asked) if asked else None)
+        pending = _Pending(scheduled, sampled_seqs, handle, n_prefill, n_decode)
+        pending.replies, pending.scored = replies, bool(asked)
+        for seq in parents:                     # the prompt is in the cache, behind what has just been queued
+            seq.forked = True
+            self._to_fork.discard(seq.seq_id)
+            for q in seq.replies:
+                try:
+                    self.runner.fork(seq.seq_id, [q.seq_id])
+                except (NoFreePages, NoFreeSlot):
+                    break                       # this reply and the others wait and run the prompt again
+        return pending
 
     def _stand_ins(self, cur) -> None:
         """The bookkeeping of a step whose tokens are not known yet: every sampled row r appends -(r + 1)."""
@@ -186,42 +217,93 @@ class LLMEngine:
         cur.places = [n if seq.num_tokens == n + 1 else None for seq, n in zip(cur.sampled_seqs, before)]
 
     def _resolve(self, cur, tokens: list) -> StepOutput:
+        scores = self.runner.collect_logprobs(cur.handle, tokens) if cur.scored else [None] * len(tokens)
+        told: list = []
+
+        def score(seq, s) -> None:
+            if seq.logprobs is not None:
+                s.top = s.top[:seq.logprobs]
+                seq.scores.append(s)
+                told.append((seq.seq_id, s))
+
         if cur.places is None:                                   # nothing was decided ahead: the plain order
+            W = len(cur.sampled_seqs)
             sampled = {seq.seq_id: tok for seq, tok in zip(cur.sampled_seqs, tokens)}
+            before = [seq.num_tokens for seq in cur.sampled_seqs]
             finished = self.scheduler.postprocess(cur.scheduled, sampled)
+            for seq, n, s in zip(cur.sampled_seqs, before, scores):
+                if seq.num_tokens > n:                           # (else it was preempted after it was scheduled)
+                    score(seq, s)
+            for seq, tok, s in zip(cur.replies, tokens[W:], scores[W:]):
+                seq.token_ids.append(tok)
+                sampled[seq.seq_id] = tok
+                score(seq, s)
+                if (tok == self.config.eos and not seq.ignore_eos) or seq.max_tokens <= 1 or seq.num_tokens >= self.config.max_model_len:
+                    if self.runner.manager.has(seq.seq_id):
+                        self.runner.close(seq.seq_id)
+                    seq.status = SequenceStatus.FINISHED
+                    finished.append(seq)
+                else:
+                    self.scheduler.add_reply(seq)
+                    if seq.nucleus_sampling:
+                        self._nucleus_live.add(seq.seq_id)
             self._nucleus_live.difference_update(q.seq_id for q in finished)
             return StepOutput([(q.seq_id, q.completion_token_ids) for q in finished], cur.n_prefill, cur.n_decode,
-                              list(sampled.items()))
+                              list(sampled.items()), told)
         finished, new = list(cur.finished), []
-        for seq, place, tok in zip(cur.sampled_seqs, cur.places, tokens):
+        for seq, place, tok, s in zip(cur.sampled_seqs, cur.places, tokens, scores):
             if place is None:                                    # preempted meanwhile, or ended a step earlier
                 continue
             self.scheduler.patch(seq, place, tok)
             new.append((seq.seq_id, tok))
+            score(seq, s)
             if tok == self.config.eos and not seq.ignore_eos and not seq.is_finished:
                 self.scheduler.finish_late(seq)
                 finished.append(seq)
         self._nucleus_live.difference_update(q.seq_id for q in finished)
-        return StepOutput([(q.seq_id, q.completion_token_ids) for q in finished], cur.n_prefill, cur.n_decode, new)
+        return StepOutput([(q.seq_id, q.completion_token_ids) for q in finished], cur.n_prefill, cur.n_decode, new, told)
 
     # ------------------------------------------------------------------ generate
     def generate(self, prompts, sampling_params=None) -> list:
-        """``prompts``: list of token-id lists.  ``sampling_params``: one for all or one per prompt."""
+        """``prompts``: list of token-id lists.  ``sampling_params``: one for all or one per prompt.  A result is
+        ``{"token_ids": [...]}``; ``SamplingParams.logprobs`` adds ``"logprobs"``, a ``TokenLogprob`` per token, and
+        ``SamplingParams.n`` > 1 ``"replies"``, the results of all replies, the first of which is the result's own."""
         if sampling_params is None or isinstance(sampling_params, SamplingParams):
             sps = [sampling_params or SamplingParams()] * len(prompts)
         else:
             sps = list(sampling_params)
             if len(sps) != len(prompts):
                 raise ValueError("prompts and sampling params size mismatch")      # src/llm_engine.cpp:107
+        families = {}
         for p, sp in zip(prompts, sps):
             if isinstance(p, str):
                 raise TypeError("this engine takes token ids; tokenize outside it")
-            self.add_request(p, sp)
-        completed = {}
+            first = self.add_request(p, sp)
+            if sp.n > 1:
+                families[first] = range(first + 1, first + sp.n)          # (ids are handed out one after the other)
+        completed, scores = {}, {}
         while not self.is_finished():
-            for seq_id, toks in self.step().finished:
-                completed[seq_id] = toks
-        return [{"token_ids": completed[k]} for k in sorted(completed)]
+            out = self.step()
+            for seq_id, s in out.logprobs:
+                scores.setdefault(seq_id, []).append(s)
+            for seq_id, toks in out.finished:
+                completed[seq_id] = {"token_ids": toks}
+                if seq_id in scores:
+                    completed[seq_id]["logprobs"] = scores.pop(seq_id)
+        for first, others in families.items():
+            completed[first]["replies"] = [dict(completed[first])] + [completed.pop(q) for q in others]
+        return [completed[k] for k in sorted(completed)]
+
+    def score(self, prompts, top: int = 0) -> list:
+        """Per sequence of token ids, a ``TokenLogprob`` for every token but the first, given the ones before it, with the
+        ``top`` likeliest ids.  Runs at once, beside whatever requests are queued (it takes a free state slot and pages)."""
+        most = min(MAX_LOGPROBS, self.vocab_size)
+        if not 0 <= top <= most:
+            raise ValueError(f"top must lie in 0 .. {most}")
+        for ids in prompts:
+            if not len(ids) or len(ids) > self.config.max_model_len:
+                raise ValueError("a sequence to score has at least one token and no more than max_model_len")
+        return [self.runner.score(ids, top, min(512, self.config.max_num_batched_tokens)) for ids in prompts]
 
 
 LLM = LLMEngine

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import gc
 import sys
+from dataclasses import dataclass
 
 import numpy as np
 import torch
@@ -38,6 +39,13 @@ MAX_DECODE_GRAPHS = 64      # captured steps of single rows only (one per batch 
 GRAPH_MAX_LOGIT_BYTES = 64 << 20
 
 
+def _to_pinned(t: torch.Tensor) -> torch.Tensor:
+    """A copy of a device tensor in pinned memory, queued on the current stream."""
+    host = torch.empty(t.shape, dtype=t.dtype, pin_memory=True)
+    host.copy_(t, non_blocking=True)
+    return host
+
+
 class _Prepared:
     """What is left of a step's preparation when nobody needs its arrays on the host side."""
     __slots__ = ("native_ids", "ends")
@@ -46,12 +54,33 @@ class _Prepared:
         self.native_ids, self.ends = native_ids, ends
 
 
+class _Launched:
+    """A step that was queued: its tokens (then the kernels' error flag) in pinned memory, valid once ``done`` has passed, with the
+    further draws and the log probabilities where they were asked for."""
+    __slots__ = ("host", "done", "W", "again", "scores")
+
+    def __init__(self, host, done, W, again, scores):
+        self.host, self.done, self.W, self.again, self.scores = host, done, W, again, scores
+
+
+@dataclass
+class TokenLogprob:
+    """How likely a token was under the model's distribution (at temperature 1, before any penalty): its log probability and
+    its rank (0: the likeliest), the distribution's entropy in nats, and the likeliest ids with their log probabilities."""
+    token: int
+    logprob: float
+    rank: int
+    entropy: float
+    top: list
+
+
 class ModelRunner:
     def __init__(self, model_dir: str, *, dtype: str = "bfloat16", page_size: int = 16, num_pages: int | None = None,
                  max_tokens: int | None = None, max_requests: int = 4, max_model_len: int | None = None,
                  device: str = "cuda:0", random_seed: int | None = None, norm_std: float = 0.0,
                  std: float | None = None, gpu_memory_utilization: float = 0.9, prefix_caching: bool = False,
-                 fast_kernels: bool = True, cuda_graphs: bool = True, log_stats: bool = False):
+                 fast_kernels: bool = True, cuda_graphs: bool = True, log_stats: bool = False,
+                 shared_prefix: bool = False):
         if not torch.cuda.is_available():
             raise StepError("no CUDA device: this engine runs on the GPU only (there is no CPU fallback)")
         if dtype not in _DTYPES:
@@ -99,6 +128,12 @@ class ModelRunner:
         self._out_ring: list = [None, None, None]     # pinned [tokens..., error flag] of the launches in flight
         self._out_at = 0
         self._seen: dict = {}
+        # the group of layers that see every earlier position, whose rows' common prefixes are looked for; a float32 run
+        # keeps the plain kernel for every row (its sums have one order however the work is cut)
+        self._whole_group = None
+        if shared_prefix and fast_kernels and self.ctx.act_dtype == torch.bfloat16 and 0 in self.cache.windows:
+            self._whole_group = self.cache.windows.index(0)
+            self._whole_heads = self.cache.heads_of(self._whole_group)
 
     def _pages_from_free_memory(self, utilization: float) -> int:
         per_page = sum(self.cache.bytes_per_page())
@@ -117,6 +152,21 @@ class ModelRunner:
 
     def close(self, rid) -> None:
         self.manager.close(rid)
+
+    def fork(self, rid, new_rids: list) -> None:
+        """Opens ``new_rids`` with the cache of ``rid`` as it is, so that each goes on from there by itself: full pages are
+        shared, part-full ones and recurrent states are copied on the device (behind whatever is queued there).  All of
+        them or none: ``NoFreeSlot`` / ``NoFreePages`` leave everything as it was."""
+        forks, opened = [], []
+        try:
+            for new in new_rids:
+                forks.append(self.manager.fork(rid, new))
+                opened.append(new)
+            self.cache.copy_forks(forks, self.stager)
+        except BaseException:
+            for new in opened:
+                self.manager.close(new)
+            raise
 
     def num_cached(self, rid) -> int:
         return self.manager.get(rid).num_tokens
@@ -225,11 +275,13 @@ class ModelRunner:
         if not entries:
             return torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
         logits = batch = None
-        key = self._graph_key(entries, None)
+        shared = self._shared_rows(entries)
+        key = self._graph_key(entries, None, shared)
         if key is not None:
-            logits, batch = self._graph_step(entries, None, key)
+            logits, batch = self._graph_step(entries, None, key, shared)
         if batch is None:
             batch = self.prepare(entries)
+            self._share(batch, shared)
             logits = self._forward(batch)
         if check:
             self.ctx.err.check("step")
@@ -247,22 +299,30 @@ class ModelRunner:
         return self.collect(self.launch_tokens(entries, temperatures, uniforms, nucleus))
 
     @torch.no_grad()
-    def launch_tokens(self, entries: list, temperatures: list, uniforms: list, nucleus: list | None = None):
+    def launch_tokens(self, entries: list, temperatures: list, uniforms: list, nucleus: list | None = None,
+                      again: list | None = None, logprobs: int | None = None):
         """Queues ``step_tokens`` and returns a handle for ``collect`` without waiting.  The tokens also stay on the
         device (``self.feed``): an entry of the *next* launch may name the token drawn for wanted row r of this
         one as ``-(r + 1)`` instead of its value, so the next step can be queued before this one has been read.
 
         ``nucleus``: per wanted row ``None`` or ``(top_p, penalty, recent ids)``: such a row's token is drawn by the
         nucleus rule with repetition penalty (``ops.sample_nucleus``) from the same logits, temperature and
-        uniform number; the other rows are untouched by it."""
+        uniform number; the other rows are untouched by it.
+
+        ``again``: (wanted row, temperature, uniform number, ``None`` or its nucleus) per further token to draw from that row's
+        logits (the first tokens of further replies to a prompt); they follow the rows' tokens in what ``collect``
+        returns.  ``logprobs``: not ``None``: ``collect_logprobs`` returns a ``TokenLogprob`` for every token, with so many of the
+        likeliest ids."""
         sampling = (temperatures, uniforms)
         batch = None
         picked = [r for r, x in enumerate(nucleus or []) if x is not None]
-        key = None if picked else self._graph_key(entries, sampling)
+        shared = self._shared_rows(entries)
+        key = None if picked else self._graph_key(entries, sampling, shared)
         if key is not None:
-            _, batch = self._graph_step(entries, sampling, key)
+            logits, batch = self._graph_step(entries, sampling, key, shared)
         if batch is None:
             batch = self.prepare(entries, sampling=sampling)
+            self._share(batch, shared)
             logits = self._forward(batch)
             self._sample_into_feed(logits, batch)
             if picked:
@@ -274,19 +334,113 @@ class ModelRunner:
             self._out_ring[k] = torch.empty(max(W + 1, self.feed.numel()), dtype=torch.int32).pin_memory()
         host = self._out_ring[k]
         host[:W + 1].copy_(self.feed[:W + 1], non_blocking=True)
+        further = self._draw_again(logits, again) if again else None
+        scores = None if logprobs is None else self._score(logits, self.feed[:W], again, further, int(logprobs))
+        if further is not None:
+            further = _to_pinned(further)
         done = torch.cuda.Event()
         done.record()
         self._commit(batch)
-        return (host, done, W)
+        return _Launched(host, done, W, further, scores)
 
     def collect(self, handle) -> list:
         """Waits for a launch and returns its tokens; raises if a kernel of the step flagged an error."""
-        host, done, W = handle
-        done.synchronize()
-        view = host.numpy()
+        handle.done.synchronize()
+        W, view = handle.W, handle.host.numpy()
         if int(view[W]):
             self.ctx.err.check("step")
-        return view[:W].tolist()
+        return view[:W].tolist() + (handle.again.tolist() if handle.again is not None else [])
+
+    def collect_logprobs(self, handle, tokens: list) -> list:
+        """The ``TokenLogprob`` of every token that ``collect`` returned for this launch."""
+        logprob, entropy, rank, ids, top = [t.tolist() if t is not None else None for t in handle.scores]
+        return [TokenLogprob(t, logprob[i], rank[i], entropy[i], list(zip(ids[i], top[i])) if ids is not None else [])
+                for i, t in enumerate(tokens)]
+
+    @torch.no_grad()
+    def score(self, tokens: list, top: int = 0, portion: int = 512) -> list:
+        """A ``TokenLogprob`` for every token of a sequence but the first, given the ones before it (for perplexities, and to
+        rank given continuations).  Takes a state slot and the sequence's pages while it runs, ``portion`` tokens a
+        step."""
+        tokens, rid = [int(t) for t in tokens], ("score", object())
+        bad = [t for t in tokens if not 0 <= t < self.vocab_size]
+        if bad:
+            raise StepError(f"token id {bad[0]} is outside the vocabulary [0, {self.vocab_size})")
+        found, last = [], len(tokens) - 1
+        try:
+            for at in range(0, last, portion):
+                end = min(last, at + portion)
+                logits = self.step([StepEntry(rid, tokens[at:end], list(range(end - at)))])
+                given = torch.tensor(tokens[at + 1:end + 1], dtype=torch.int32).to(self.device)
+                handle = _Launched(None, None, 0, None, self._score(logits, given, None, None, top))
+                torch.cuda.current_stream(self.device).synchronize()
+                found += self.collect_logprobs(handle, tokens[at + 1:end + 1])
+        finally:
+            if self.manager.has(rid):
+                self.close(rid)
+        return found
+
+    def _score(self, logits, tokens, again, further, top: int):
+        """Queues the log probabilities of the rows' tokens, and of the tokens drawn again from some of them, and their copies to
+        pinned memory: (log probabilities, entropies, ranks, likeliest ids, their log probabilities)."""
+        if again:
+            rows = torch.tensor([r for r, *_ in again], dtype=torch.int64).to(self.device, non_blocking=True)
+            logits, tokens = torch.cat([logits, logits.index_select(0, rows)]), torch.cat([tokens, further])
+        n, dev = logits.shape[0], self.device
+        logprob, entropy = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+        rank = torch.empty(n, dtype=torch.int32, device=dev)
+        ids = best = None
+        if top > 0:
+            ids = torch.empty((n, top), dtype=torch.int32, device=dev)
+            best = torch.empty((n, top), dtype=torch.float32, device=dev)
+        if n:
+            ops.token_logprobs(logits, tokens, logprob, entropy=entropy, rank=rank, top_ids=ids, top_logprobs=best, err=self.ctx.err)
+        return [None if t is None else _to_pinned(t) for t in (logprob, entropy, rank, ids, best)]
+
+    def _draw_again(self, logits, again: list):
+        """Queues further draws from wanted rows' logits; their tokens, on the device."""
+        dev, n = self.device, len(again)
+        rows = torch.tensor([r for r, *_ in again], dtype=torch.int64).to(dev, non_blocking=True)
+        picked = [i for i, (_, _, _, x) in enumerate(again) if x is not None]
+        out = torch.empty(n, dtype=torch.int32, device=dev)
+        chosen = logits.index_select(0, rows)
+        ops.sample(chosen, torch.tensor([t for _, t, _, _ in again], dtype=torch.float32).to(dev, non_blocking=True),
+                   torch.tensor([u for _, _, u, _ in again], dtype=torch.float64).to(dev, non_blocking=True), out)
+        if picked:
+            self._nucleus_rows(chosen, picked, [t for _, t, _, _ in again], [u for _, _, u, _ in again], [x for _, _, _, x in again], out)
+        return out
+
+    # ------------------------------------------------------------------ rows that share a prefix
+    def _shared_rows(self, entries: list):
+        """Which single rows of the step begin with the same pages: (groups of places among the step's single rows with the
+        positions in common, number of single rows), or ``None`` where nobody looks, nobody shares, or the layers would
+        have every row read its own keys anyway."""
+        if self._whole_group is None:
+            return None
+        single = [e for e in entries if len(e.tokens) == 1]
+        known = [i for i, e in enumerate(single) if self.manager.has(e.rid)]
+        if len(known) < 2:
+            return None
+        groups = self.manager.shared_prefixes([single[i].rid for i in known], self._whole_group)
+        groups = [([known[i] for i in members], n) for members, n in groups]
+        Hkv, D = self._whole_heads
+        repeated, members = sum(n * (len(m) - 1) for m, n in groups), sum(len(m) for m, _ in groups)
+        pays = ops.attention_sharing_pays(len(single), members, len(groups), Hkv, Hkv, D, self.page_size, torch.bfloat16, repeated)
+        return (groups, len(single)) if pays else None
+
+    @staticmethod
+    def _rounded_facts(groups, rows: int):
+        """What a captured step's launches go by: the powers of two around the step's own numbers, so that steps of about the
+        same prefixes share a capture."""
+        longest, shortest, repeated = ops.SharedPrefix.facts(groups, rows)
+        floor = lambda n: 1 << (n.bit_length() - 1) if n > 0 else 0
+        return 1 << max(0, longest - 1).bit_length(), floor(shortest), floor(repeated)
+
+    def _share(self, batch, shared) -> None:
+        if shared is not None:
+            groups, rows = shared
+            buf = self.stager.stage(np.array(ops.SharedPrefix.pack(groups, rows)[0], dtype=np.int32))
+            batch.shared = ops.SharedPrefix(groups, rows, self.device, buf=buf)
 
     def _sample_into_feed(self, logits, batch) -> None:
         """Queues the sampling kernel; tokens go to ``feed[:W]``, the kernels' error flag to ``feed[W]``."""
@@ -299,6 +453,9 @@ class ModelRunner:
 
     def _nucleus_into_feed(self, logits, picked, temperatures, uniforms, nucleus) -> None:
         """Draws the rows ``picked`` again by the nucleus rule and puts their tokens in their places of ``feed``."""
+        self._nucleus_rows(logits, picked, temperatures, uniforms, nucleus, self.feed)
+
+    def _nucleus_rows(self, logits, picked, temperatures, uniforms, nucleus, tokens) -> None:
         params, flat, off = [], [], [0]
         for r in picked:
             top_p, penalty, recent = nucleus[r]
@@ -311,10 +468,10 @@ class ModelRunner:
         ops.sample_nucleus(logits.index_select(0, rows), torch.tensor(params, dtype=torch.float64).to(dev),
                            torch.tensor(flat or [0], dtype=torch.int32).to(dev),
                            torch.tensor(off, dtype=torch.int32).to(dev), out)
-        self.feed.index_copy_(0, rows, out)
+        tokens.index_copy_(0, rows, out)
 
     # ------------------------------------------------------------------ steps as CUDA graphs
-    def _graph_key(self, entries: list, sampling):
+    def _graph_key(self, entries: list, sampling, shared=None):
         """What fixes a step's kernels and their sizes: the number of entries, of rows, of entries with a single row
         (they go to another attention kernel) and of wanted rows, and whether the sampling kernel follows.  How the
         rows are cut into entries and which rows are wanted is data: the kernels read it from the step's arrays.
@@ -327,9 +484,13 @@ class ModelRunner:
         W = sum(len(e.want) for e in entries)
         if W * self.vocab_size * 4 > GRAPH_MAX_LOGIT_BYTES:
             return None                        # (a captured step keeps its logits tensor for good)
-        return (len(entries), T, sum(1 for e in entries if len(e.tokens) == 1), W, sampling is not None)
+        key = (len(entries), T, sum(1 for e in entries if len(e.tokens) == 1), W, sampling is not None)
+        if shared is not None:                 # ... and how many groups and rows share prefixes of about which lengths
+            groups, rows = shared
+            key += (len(groups), sum(len(m) for m, _ in groups), *self._rounded_facts(groups, rows))
+        return key
 
-    def _graph_step(self, entries: list, sampling, key):
+    def _graph_step(self, entries: list, sampling, key, shared=None):
         """Two steps of the same shape (see ``_graph_key``) launch the same kernels with the same sizes; only the
         index arrays differ (every kernel takes positions, entry lengths and tables from them, on the device).  A shape
         seen for the second time is captured and replayed from then on: the arrays are copied into the buffer the
@@ -353,6 +514,12 @@ class ModelRunner:
             batch = self.prepare(entries, static_dev, sampling)
             # the split of the keys of single rows must not depend on the step
             batch.max_context = batch.max_single_context = self.max_model_len
+            shared_dev = None
+            if shared is not None:
+                groups, rows = shared
+                packed = np.array(ops.SharedPrefix.pack(groups, rows)[0], dtype=np.int32)
+                shared_dev = self.stager.stage(packed, torch.empty(len(packed), dtype=torch.int32, device=self.device))
+                batch.shared = ops.SharedPrefix(groups, rows, self.device, facts=self._rounded_facts(groups, rows), buf=shared_dev)
             logits = self._forward(batch)       # warms up; also this step's result
             if sampling is not None:
                 self._sample_into_feed(logits, batch)
@@ -373,10 +540,12 @@ class ModelRunner:
             finally:
                 if collecting:
                     gc.enable()
-            self._graphs[key] = (graph, static_dev, static_logits, ops.launch_count() - before)
+            self._graphs[key] = (graph, static_dev, static_logits, ops.launch_count() - before, shared_dev)
             return logits, batch
-        graph, static_dev, static_logits, launches = g
+        graph, static_dev, static_logits, launches, shared_dev = g
         batch = self.prepare(entries, static_dev, sampling, views=False)
+        if shared is not None:
+            self.stager.stage(np.array(ops.SharedPrefix.pack(*shared)[0], dtype=np.int32), shared_dev)
         graph.replay()
         ops.add_launches(launches)
         return static_logits, batch

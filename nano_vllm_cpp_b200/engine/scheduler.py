@@ -88,6 +88,17 @@ class Scheduler:
             raise SchedulerError(host.last_error())
         self._seqs[seq.seq_id] = seq
 
+    def add_reply(self, seq: Sequence) -> None:
+        """A further reply to a prompt that has run (its first token is drawn): it decodes on from its forked cache, or waits to
+        run its prompt again where nothing could be forked."""
+        arr, n = host.ints(seq.token_ids)
+        rc = host.lib().nvs_add_reply(self._h, seq.seq_id, arr, n, seq.num_prompt_tokens, seq.max_tokens,
+                                      1 if seq.ignore_eos else 0)
+        if rc:
+            raise SchedulerError(host.last_error())
+        self._seqs[seq.seq_id] = seq
+        self._sync(seq)
+
     def is_finished(self) -> bool:
         return bool(host.lib().nvs_is_finished(self._h))
 

@@ -16,7 +16,7 @@ class SequenceStatus(Enum):
 class Sequence:
     _counter = itertools.count()
 
-    def __init__(self, token_ids: list, sampling: SamplingParams, base_seed: int = 0):
+    def __init__(self, token_ids: list, sampling: SamplingParams, base_seed: int = 0, reply: int = 0):
         if not token_ids:
             raise ValueError("empty prompt token ids")
         self.seq_id = next(Sequence._counter)
@@ -31,7 +31,12 @@ class Sequence:
         self.repetition_penalty = float(sampling.repetition_penalty)
         self.repetition_window = int(sampling.repetition_window)
         # the request's own random stream: (seed, number of tokens drawn so far)
-        self.seed = sampling.seed if sampling.seed is not None else (base_seed * 0x9E3779B1 + self.seq_id)
+        self.seed = sampling.seed + reply if sampling.seed is not None else (base_seed * 0x9E3779B1 + self.seq_id)
+        self.logprobs = sampling.logprobs       # likeliest ids wanted beside every token; None: no log probabilities
+        self.scores: list = []                  # a TokenLogprob per completion token, where they are wanted
+        # further replies to the prompt, which join the scheduler when the prompt has run
+        self.replies = ([Sequence(token_ids, sampling, base_seed, r) for r in range(1, int(sampling.n))] if reply == 0 else [])
+        self.forked = not self.replies
         self.num_preemptions = 0
 
     @property

@@ -49,13 +49,14 @@ def test_shared_attention_refuses_sizes():
 
 
 def test_shared_prefix_packs_its_groups():
-    packed, members, longest = ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6)
-    assert members == 3 and longest == 32
+    packed, members = ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6)
+    assert members == 3 and ops.SharedPrefix.facts([([4, 1], 32), ([2], 7)], 6) == (32, 0, 32)
+    assert ops.SharedPrefix.facts([([0, 1, 2], 48), ([3], 16)], 4) == (48, 16, 96) and ops.SharedPrefix.facts([], 3) == (0, 0, 0)
     assert packed[:6] == [0, 32, 7, 0, 32, 0]                               # shared positions of every row
     assert packed[6:12] == [-1, 0, 1, -1, 0, -1]                            # its group
     assert packed[12:15] == [4, 1, 2]                                       # the groups' rows, the leading one first
     assert packed[18:21] == [0, 2, 3] and packed[21:23] == [32, 7] and packed[23:] == [4, 2]
-    assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0, 0)
+    assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0)
 
 
 def test_sharing_is_a_matter_of_bytes_rows_and_heads():

@@ -266,7 +266,7 @@ def sharing(request, monkeypatch):
         if not request.param:
             pytest.skip("no attention here")
     elif request.param:
-        monkeypatch.setattr(ops(), "attention_sharing_pays", lambda shared, *a: shared.groups > 0)
+        monkeypatch.setattr(ops(), "attention_sharing_pays", lambda rows, members, groups, *a: groups > 0)
 
 
 class Case:
