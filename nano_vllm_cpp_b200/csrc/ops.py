@@ -448,7 +448,9 @@ def _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, sca
     scratch = counts = None
     if splits > 1:
         scratch = torch.empty(R * Hq * splits * (D + 2), dtype=torch.float32, device=qkv.device)
-        counts = _split_counts(qkv.device)
+        # (``clean`` calls add their splits up in a second kernel: the counters are one array for kernels that run one after the
+        # other, and these calls may overlap, on two streams or in two captured graphs)
+        counts = None if clean else _split_counts(qkv.device)
     launch = lib().nv_attention_decode_clean if clean else lib().nv_attention_decode
     _check(launch(_p(qkv), dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), dt(k_cache), _p(block_table), block_table.shape[1],
                   _p(row_entry), _p(positions), _p(rows), R, scale, window, _p(out), dt(out), Hq, Hkv, D, k_cache.shape[2],
@@ -472,6 +474,7 @@ class SharedPrefix:
         packed, self.members = self.pack(groups, rows)
         self.R, self.groups, self._splits = rows, len(groups), {}
         self.longest, self.shortest, self.repeated = self.facts(groups, rows) if facts is None else facts
+        self.reach = max((n for _, n in groups), default=0)          # positions that the block tables must cover
         self.bind(torch.tensor(packed, dtype=torch.int32).to(device) if buf is None else buf)
 
     @staticmethod
@@ -554,6 +557,8 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(shared.R == R, "attention_decode_shared: the shared prefixes are of another number of rows")
     _need(scale > 0 and softcap >= 0, "attention_decode_shared: the scale is positive, a cap is not negative")
     page = shape[2]
+    _need(block_table.dim() == 2 and shared.reach // page <= block_table.shape[1],
+          "attention_decode_shared: a prefix reaches beyond the block tables")
     terms = 1 if float_weights or sink_score is not None else 0
     splits, ours = shared.splits(Hq, Hkv, D, k_cache, terms, max_context)
     if ours == 0:

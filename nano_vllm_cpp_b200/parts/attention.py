@@ -313,7 +313,7 @@ class PagedAttention(Mixer):
         scored = dict(softcap=self.softcap, gate=gate, chunk=self.chunk, slopes=self.slopes, bias_table=self.bias_table)
         single = batch.n_single if ops.attention_decode_usable(cache.k, P) else 0
         if single:
-            self._attend_single(q, cache, bt, batch, att, P, sink_score=self.sink_score, float_weights=self.weight_terms == 3, **scored)
+            _attend_single(self, q, cache, bt, batch, att, P, sink_score=self.sink_score, float_weights=self.weight_terms == 3, **scored)
         if single < batch.S:
             tiles = (batch.T - single) // ops.attention_prefill_tile_rows() + (batch.S - single)
             ops.attention_prefill(q, cache.k, cache.v, bt, batch.cu_rows, batch.entry_pos0, tiles, self.scale,
@@ -377,20 +377,6 @@ class PagedAttention(Mixer):
             att = back
         return linear(ctx, att, self.o_weight, torch.float32, bias=self.o_bias)
 
-    def _attend_single(self, q, cache, bt, batch, att, D, *, chunk=0, slopes=None, bias_table=None, **scored):
-        """The step's single rows: every row by itself, or, where the step says which of them share a prefix and the layer
-        sees every earlier position alike, the shared keys once for all of them."""
-        context = batch.max_context if batch.decode_only else batch.max_single_context
-        rows = None if batch.decode_only else batch.single_rows
-        alike = self.window == 0 and chunk == 0 and slopes is None and bias_table is None and self.scale > 0
-        if batch.shared is not None and alike:
-            ops.attention_decode_shared(q, cache.k, cache.v, bt, batch.row_entry, batch.positions, self.scale, att, self.Hq, self.Hkv,
-                                        D, context, batch.shared, rows=rows, err=self.ctx.err, **scored)
-        else:
-            ops.attention_decode(q, cache.k, cache.v, bt, batch.row_entry, batch.positions, self.scale, self.window, att, self.Hq,
-                                 self.Hkv, D, context, rows=rows, err=self.ctx.err, chunk=chunk, slopes=slopes,
-                                 bias_table=bias_table, **scored)
-
     def _attend(self, qkv, cache, bt, batch, att):
         """Which kernel runs which rows.  float32 runs keep the plain kernel for every row, so that their sums have
         one order however the work is cut.  bfloat16 runs send entries of one row to the split-key decode kernel and
@@ -425,10 +411,26 @@ class PagedAttention(Mixer):
             join.record(side)
         try:
             if single:
-                self._attend_single(qkv, cache, bt, batch, att, self.D)
+                _attend_single(self, qkv, cache, bt, batch, att, self.D)
         finally:                # (a refused call, too, leaves no reader of these buffers behind the main stream's back)
             if side is not None:
                 main.wait_event(join)
+
+
+def _attend_single(part, q, cache, bt, batch, att, D, *, chunk=0, slopes=None, bias_table=None, **scored):
+    """The step's single rows: every row by itself, or, where the step says which of them share a prefix and the layer
+    sees every earlier position alike, the shared keys once for all of them."""
+    context = batch.max_context if batch.decode_only else batch.max_single_context
+    rows = None if batch.decode_only else batch.single_rows
+    alike = part.window == 0 and chunk == 0 and slopes is None and bias_table is None and part.scale > 0
+    shared = getattr(batch, "shared", None)          # (a batch put together by hand may not say)
+    if shared is not None and alike:
+        ops.attention_decode_shared(q, cache.k, cache.v, bt, batch.row_entry, batch.positions, part.scale, att, part.Hq, part.Hkv,
+                                    D, context, shared, rows=rows, err=part.ctx.err, **scored)
+    else:
+        ops.attention_decode(q, cache.k, cache.v, bt, batch.row_entry, batch.positions, part.scale, part.window, att, part.Hq,
+                             part.Hkv, D, context, rows=rows, err=part.ctx.err, chunk=chunk, slopes=slopes,
+                             bias_table=bias_table, **scored)
 
 
 def distance_buckets(rows: int, far: int) -> list:

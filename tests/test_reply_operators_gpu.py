@@ -468,9 +468,44 @@ def test_attention_refuses():
     call()
     for kw in (dict(q=c.q.float()), dict(k=c.k.float()), dict(out=out.float()), dict(out=out[:, :128].contiguous()), dict(Hq=3), dict(D=32),
                dict(shared=three), dict(scale=0.0), dict(scale=-1.0), dict(softcap=-1.0), dict(q=c.q[:, :128].contiguous()),
-               dict(v=c.v[:-1]), dict(k=c.k.transpose(1, 2)), dict(Hkv=1), dict(gate=torch.zeros(2, 3, device=DEV))):
+               dict(shared=o.SharedPrefix([([0, 1], 16 * c.table.shape[1] + 16)], 2, DEV)), dict(v=c.v[:-1]), dict(k=c.k.transpose(1, 2)), dict(Hkv=1), dict(gate=torch.zeros(2, 3, device=DEV))):
         with pytest.raises(o.KernelError):
             call(**kw)
+
+
+def test_attention_of_no_rows():
+    o = ops()
+    c = Case(4, 2, 64, [40, 50], [([0, 1], 32)])
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    got = c.run(rows=none, groups=[], stale=2.0)
+    assert bool((got == 2.0).all()) and o.SharedPrefix([], 0, DEV).buf.numel() == 1
+
+
+def test_attention_captured_twice_and_replayed_side_by_side():
+    """Two captures of the operator, each with a scratch of its own, replayed on two streams at once with new queries."""
+    cases = [Case(16, 4, 64, [300 + 7 * r for r in range(6)], [(list(range(6)), 288)], seed=s) for s in (1, 2)]
+    plans, outs, graphs = [], [], []
+    for c in cases:
+        plans.append(ops().SharedPrefix(c.groups, 6, DEV))
+        outs.append(c.run(shared=plans[-1]))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run(shared=plans[-1], out=outs[-1])
+        graphs.append(g)
+    for k in range(3):
+        for i, c in enumerate(cases):
+            c.q.copy_(rnd(*c.q.shape, seed=100 + 2 * k + i, dtype=torch.bfloat16))
+        torch.cuda.synchronize()
+        streams = torch.cuda.Stream(), torch.cuda.Stream()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for c, out in zip(cases, outs):
+            want, weight, score = c.want()
+            assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score)).all())
 
 
 # ------------------------------------------------------------------------------------------------ the three together
