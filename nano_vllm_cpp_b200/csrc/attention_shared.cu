@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
 //   warp 0     fetches the pages of K (two buffers) and V as TMA boxes of one page x 64 elements, a lane a box
 //   warp 1     allocates tensor memory; one thread issues the products
 //   warps 2-5  gather the queries of the tile's pairs into shared memory (128-byte swizzle), then a thread owns a pair: it reads its
-//              row of S, keeps its maximum and sum, writes P as bfloat16 into shared memory, and at the end its row of O, undivided,
-//              with maximum and sum to the scratch
+//              row of S, keeps its maximum and sum, writes P as bfloat16 over its scores, from where the second product takes it (three
+//              terms: into shared memory), and at the end its row of O, undivided, with maximum and sum to the scratch
 // All keys of a split are seen by all pairs, but for those behind a row's own position, so there is no mask in most blocks.  TERMS =
 // 3: the float32 weights enter the product with the values as three bfloat16 terms (all their bits) instead of one rounded.
 // Heads between the forms' sizes: the boxes reach beyond the pages' rows and are filled with zeros.
@@ -239,20 +239,24 @@ __device__ __forceinline__ void bulk_store_wait() {
 template <int D>
 constexpr int st_tmem_cols() { return 2 * ST_KEYS + D <= 256 ? 256 : 512; }
 
+// Buffers of values: two, but for the largest form, whose three tiles of P leave room for one.
+template <int D, int TERMS>
+constexpr int st_v_buffers() { return D > 128 && TERMS > 1 ? 1 : 2; }
+
 template <int D, int TERMS>
 __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? 2 : 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, SharedArgs a, ScoreMap map) {
-  constexpr int SL = D / 64;
+  constexpr int SL = D / 64, VB = st_v_buffers<D, TERMS>();
   constexpr uint32_t Q_SLAB = ST_PAIRS * 128, KV_SLAB = ST_KEYS * 128, P_TILE = ST_PAIRS * 128;
   extern __shared__ __align__(1024) uint8_t st_smem_raw[];
-  __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full, pv_done;
+  __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
   __shared__ uint32_t tmem_base_s;
 
   uint8_t* smem = (uint8_t*)(((uintptr_t)st_smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* Qs = smem;
   uint8_t* Ks = Qs + SL * Q_SLAB;                  // two buffers
-  uint8_t* Vs = Ks + 2 * SL * KV_SLAB;
-  uint8_t* Ps = Vs + SL * KV_SLAB;                 // TERMS tiles of [128 pairs][64 keys]
+  uint8_t* Vs = Ks + 2 * SL * KV_SLAB;             // VB buffers
+  uint8_t* Ps = Vs + VB * SL * KV_SLAB;             // TERMS > 1: so many tiles of [128 pairs][64 keys]
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kvh = blockIdx.y, split = blockIdx.z, G = a.Hq / a.Hkv;
@@ -263,10 +267,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     for (int b = 0; b < 2; ++b) {
       mbar_init(&k_full[b], 1);
       mbar_init(&k_empty[b], 1);
+      mbar_init(&v_full[b], 1);
+      mbar_init(&v_empty[b], 1);
       mbar_init(&s_full[b], 1);
     }
-    mbar_init(&v_full, 1);
-    mbar_init(&v_empty, 1);
     mbar_init(&p_full, 4);
     mbar_init(&pv_done, 1);
     mbar_fence_init();
@@ -286,10 +290,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int n_blocks = (j_hi - j_lo + ST_KEYS - 1) / ST_KEYS;
     const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 2 * ST_KEYS;
     const int lead_t = a.rows ? a.rows[tile.lead] : tile.lead;
-    // A block's keys behind the split's end are not loaded; their weights are zero, their values must be finite numbers.  Only a
-    // first block meets what the shared memory held before.
-    if (n_blocks == 1 && j_hi - j_lo < ST_KEYS) {
-      for (int i = tid; i < (int)(SL * KV_SLAB / 16); i += ST_THREADS) ((uint4*)Vs)[i] = make_uint4(0, 0, 0, 0);
+    // A block's keys behind the split's end are not loaded; their weights are zero, their values must be finite numbers.  Only the
+    // first VB blocks meet what the shared memory held before.
+    if (n_blocks <= VB && (j_hi - j_lo) % ST_KEYS) {
+      for (int i = tid; i < (int)(VB * SL * KV_SLAB / 16); i += ST_THREADS) ((uint4*)Vs)[i] = make_uint4(0, 0, 0, 0);
       fence_async_smem();
       __syncthreads();
     }
@@ -312,15 +316,16 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           blk = -1;
         }
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, blk >= 0));
-        uint64_t* full = values ? &v_full : &k_full[i & 1];
+        const int vb = i % VB;
+        uint64_t* full = values ? &v_full[vb] : &k_full[i & 1];
         if (lane == 0) {
-          if (values) mbar_wait(&v_empty, (i & 1) ^ 1, a.err, 0x7302);
+          if (values) mbar_wait(&v_empty[vb], ((i / VB) & 1) ^ 1, a.err, 0x7302);
           else mbar_wait(&k_empty[i & 1], ((i >> 1) & 1) ^ 1, a.err, 0x7301);
           mbar_expect_tx(full, boxes * box);
         }
         __syncwarp();
         if (blk >= 0) {
-          uint8_t* dst = (values ? Vs : Ks + (i & 1) * SL * KV_SLAB) + my_s * KV_SLAB + my_p * box;
+          uint8_t* dst = (values ? Vs + vb * SL * KV_SLAB : Ks + (i & 1) * SL * KV_SLAB) + my_s * KV_SLAB + my_p * box;
           tma_load_2d(dst, values ? &tm_v : &tm_k, full, my_s * 64, (blk * a.Hkv + kvh) * a.page);
         }
       };
@@ -346,7 +351,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           dk[0][s] = smem_desc_sw128(k_addr + s * KV_SLAB);
           dk[1][s] = smem_desc_sw128(k_addr + (SL + s) * KV_SLAB);
         }
-        const uint64_t dv = smem_desc_sw128_mn(v_addr, KV_SLAB, 1024);
+        const uint64_t dv[2] = {smem_desc_sw128_mn(v_addr, KV_SLAB, 1024), smem_desc_sw128_mn(v_addr + SL * KV_SLAB, KV_SLAB, 1024)};
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) dp[t] = smem_desc_sw128(p_addr + t * P_TILE);
         auto issue_s = [&](int i) {
@@ -365,14 +370,25 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         if (n_blocks > 1) issue_s(1);
         for (int i = 0; i < n_blocks; ++i) {
           mbar_wait(&p_full, i & 1, a.err, 0x7305);  // P(i) is written, S(i) is read, O is rescaled
-          mbar_wait(&v_full, i & 1, a.err, 0x7306);
+          mbar_wait(&v_full[i % VB], (i / VB) & 1, a.err, 0x7306);
           tc_fence_after();
-          // 16 keys per product: 32 bytes (2 units) along P's rows, two 8-key groups (2,048 bytes = 128 units) of V
+          // 16 keys per product: eight columns of P in tensor memory, or 32 bytes (2 units) along its rows in shared memory, and two
+          // 8-key groups (2,048 bytes = 128 units) of V
+          const uint64_t v = i % VB ? dv[1] : dv[0];
+          if (TERMS == 1) {
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t) umma_bf16_x4s(tmem_o, dp[t], dv, idesc_o, (i || t) ? 1u : 0u, 2, 128);
-          umma_commit(&v_empty);
+            for (int k = 0; k < ST_KEYS / 16; ++k)
+              umma_bf16_ts(tmem_o, tmem_s + (i & 1) * ST_KEYS + k * 8, v + k * 128, idesc_o, (i || k) ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) umma_bf16_x4s(tmem_o, dp[t], v, idesc_o, (i || t) ? 1u : 0u, 2, 128);
+          }
+          umma_commit(&v_empty[i % VB]);
           umma_commit(&pv_done);
-          if (i + 2 < n_blocks) issue_s(i + 2);      // into the buffer that S(i) has left
+          if (i + 2 < n_blocks) {                    // into the buffer that S(i) has left, and P(i), which took its place
+            if (TERMS == 1) mbar_wait(&pv_done, i & 1, a.err, 0x7310);
+            issue_s(i + 2);
+          }
         }
       }
     } else {
@@ -481,30 +497,41 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               tmem_st32(tmem_o + lane_off + c * 32, o);
             }
           }
-          uint8_t* prow = Ps + (size_t)p * 128;
+          if (TERMS == 1) {
+            // the row's weights over its scores, two in a column
+            uint32_t w[ST_KEYS / 2];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float w[8];
+            for (int c = 0; c < ST_KEYS / 2; ++c) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(s[2 * c], s[2 * c + 1]);
+              w[c] = *(const uint32_t*)&b;
+            }
+            tmem_st32_u32(tmem_s + (i & 1) * ST_KEYS + lane_off, w);
+          } else {
+            uint8_t* prow = Ps + (size_t)p * 128;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) w[u] = s[c * 8 + u];
+            for (int c = 0; c < 8; ++c) {
+              float w[8];
 #pragma unroll
-            for (int x = 0; x < TERMS; ++x) {
-              __nv_bfloat162 b[4];
+              for (int u = 0; u < 8; ++u) w[u] = s[c * 8 + u];
 #pragma unroll
-              for (int u = 0; u < 4; ++u) b[u] = __floats2bfloat162_rn(w[2 * u], w[2 * u + 1]);
-              *(uint4*)(prow + x * P_TILE + ((c ^ (p & 7)) << 4)) = *(uint4*)b;
-              if (x + 1 < TERMS) {
+              for (int x = 0; x < TERMS; ++x) {
+                __nv_bfloat162 b[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  const float2 f = __bfloat1622float2(b[u]);
-                  w[2 * u] -= f.x;
-                  w[2 * u + 1] -= f.y;
+                for (int u = 0; u < 4; ++u) b[u] = __floats2bfloat162_rn(w[2 * u], w[2 * u + 1]);
+                *(uint4*)(prow + x * P_TILE + ((c ^ (p & 7)) << 4)) = *(uint4*)b;
+                if (x + 1 < TERMS) {
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) {
+                    const float2 f = __bfloat1622float2(b[u]);
+                    w[2 * u] -= f.x;
+                    w[2 * u + 1] -= f.y;
+                  }
                 }
               }
             }
+            fence_async_smem();
           }
         }
-        fence_async_smem();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full);
@@ -642,7 +669,7 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
   rc = nv_tensor_map_bf16(a.vc, rows, a.D, a.D, a.page, &tm_v);
   if (rc) return rc;
   constexpr int SL = D / 64;
-  constexpr size_t tiles_bytes = (size_t)SL * ST_PAIRS * 128 + 3 * (size_t)SL * ST_KEYS * 128 + (size_t)TERMS * ST_PAIRS * 128;
+  constexpr size_t tiles_bytes = (size_t)SL * ST_PAIRS * 128 + (2 + st_v_buffers<D, TERMS>()) * (size_t)SL * ST_KEYS * 128 + (TERMS > 1 ? (size_t)TERMS * ST_PAIRS * 128 : 0);
   constexpr size_t smem = tiles_bytes + 1024;
   static_assert(tiles_bytes >= (size_t)ST_PAIRS * (D * 4 + 16), "a row of results has its place");
   static bool attr_done = false;
