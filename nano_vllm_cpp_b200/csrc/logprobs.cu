@@ -2,8 +2,9 @@
 //
 //   m = max x,  Z = sum e^(x - m),  logprob(t) = x_t - m - log Z,  entropy = log Z - sum e^(x - m) (x - m) / Z
 //
-// What bounds it: the logits, read once.  2,048 rows of 151,936 float32 take 204 us, 6.1 TB/s; a handful of rows takes the latency
-// of a launch, of two or three tiles and of a cluster's exchange (one row: 6 us above an empty kernel, with five alternatives 10).
+// What bounds it: the logits, read once.  2,048 rows of 151,936 float32 take 184 us, 6.8 TB/s (226 with five alternatives each); a
+// handful of rows takes the latency of a launch, of a tile or two and of the cluster's exchange: one row 5.3 us, with five
+// alternatives 9.4.
 //
 // One pass keeps m, n1 (how many logits equal m), s (the sum of the others' e^(x - m)) and e (the sum of e^(x - m) (x - m)):
 // log Z = log n1 + log1p(s / n1).  The largest term is never added to the small ones, so the logarithm of an all but certain
@@ -70,7 +71,8 @@ struct LpArgs {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int LP_E = 16;               // elements a thread takes at a time: four (bfloat16: two) 16-byte pieces
 constexpr int LP_STAGES = 4;           // tiles under way: a thread copies its own pieces into shared memory, three tiles ahead
-constexpr int LP_LIST = 1024;          // candidates a block has room for (and at least 512 beside a bound that a tile may bring)
+constexpr int MAX_CLUSTER = 16;        // blocks a row
+constexpr int LP_LIST = 512;           // candidates a block has room for
 constexpr int LP_LONG = 256;           // ... and from how many on they are thinned out to the best K
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -96,29 +98,15 @@ struct Vec<bf16> {
   }
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t of_rank(const void* p, uint32_t rank) {    // the address of block `rank`'s copy of a shared variable
+// The blocks of a cluster leave what they have with the first one: its copy of a shared variable, as they address it.
+__device__ __forceinline__ uint32_t of_first(const void* p) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)));
   return a;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ Key ld_cluster_key(uint32_t a) {
-  Key v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
-}
+__device__ __forceinline__ void put_first(uint32_t a, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ void put_first(uint32_t a, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void put_first(uint32_t a, Key v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
 
 // The K largest of the n keys in list[] come to its front and to best[], in descending order (fewer keys: zeros behind them); every
 // thread of the block calls, between two barriers.  A key's place is the number of larger ones.
@@ -172,23 +160,29 @@ __device__ void collect_slowly(const T* x, int i0, int i1, int K, Key* list, Key
 // A cluster of blocks takes a row, each block a run of its 16-byte pieces; a warp has a maximum, its threads their sums, which are
 // rescaled when it moves.  Alternatives: the first tile gives a bound that at least K of its logits reach (the K-th largest among
 // every full warp's few largest thread maxima), what lies above it goes into a list, and behind 2, 4, 8 ... tiles the list is thinned
-// out to its K best, which raises the bound.  The first block of
-// the cluster joins the sums and lists.
-template <typename T>
+// out to its K best, which raises the bound.  Every block leaves its
+// warps' sums and its list with the first one of the cluster, which joins them.
+// TOP: with alternatives (K > 0).
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprobs_kernel(LpArgs a) {
   constexpr int N = Vec<T>::N, NV = LP_E / N, TILE = THREADS * NV;     // (a tile in pieces)
-  extern __shared__ __align__(16) uint4 ring[];                       // [LP_STAGES][NV][THREADS]
+  extern __shared__ __align__(16) uint4 ring[];                       // [LP_STAGES][NV][THREADS], and behind them:
   __shared__ Key list_s[LP_LIST];
   __shared__ Key best_s[32];
-  __shared__ Stats st_s[WARPS], mine_s;
   __shared__ uint32_t most_s[64];
-  __shared__ int rank_s, n_s;
+  __shared__ int n_s;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int cluster = (int)gridDim.x / a.R, row = blockIdx.x / cluster, part = blockIdx.x % cluster;
-  if (tid == 0) rank_s = n_s = 0;
+  // what every warp and block of the cluster has, in the first one (join_bytes)
+  Stats* const all_s = (Stats*)(ring + LP_STAGES * TILE);             // [cluster * WARPS]
+  Key* const join_s = (Key*)(all_s + cluster * WARPS);                // [cluster * K]
+  int* const ahead_s = (int*)(join_s + cluster * a.K);                // [cluster * WARPS]
+  if (tid == 0) n_s = 0;
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");        // (this block runs)
   grid_dep_wait();
   grid_dep_launch();
   const T* x = (const T*)a.logits + (long long)row * a.stride;
+  const int token = a.tokens ? a.tokens[row] : -1;
   const int off = (int)(((uintptr_t)x / sizeof(T)) % N);              // elements between the 16-byte boundary below and the row
   const int pieces = (int)(((long long)a.V + off + N - 1) / N), per = (pieces + cluster - 1) / cluster;
   const int q0 = min(pieces, part * per), q1 = min(pieces, q0 + per);
@@ -210,14 +204,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprob
   };
 #pragma unroll
   for (int t = 0; t < LP_STAGES - 1; ++t) fetch(t);
-  const int token = a.tokens ? a.tokens[row] : -1;
-  const bool known = token >= 0 && token < a.V;
+  // the given token: its logit arrives while the first tile does
+  const bool known = token >= 0 && token < a.V, ranked = known && a.rank;
   const float xt = known ? to_f32(x[token]) : 0.f;
-  // places are found by comparing numbers, those of a NaN or minus infinity by keys; the next number below xt
   const bool by_key = !(xt > -INFINITY);
   const uint32_t xt_order = order_of(xt);
   const float xt_below = below_of(xt_order);
-  const bool ranked = known && a.rank;
   for (int q = q0; q < q1; q += TILE, ++tile) {
     asm volatile("cp.async.wait_group %0;" ::"n"(LP_STAGES - 2) : "memory");
     float v[LP_E];
@@ -256,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprob
         for (int i = 0; i < LP_E; ++i) ahead += v[i] > over;
       }
     }
-    if (a.K > 0 && !lost) {
+    if (TOP && !lost) {
       const int full = min(WARPS, (q1 - q) / 32);                     // warps all of whose threads have elements
       if (!bounded && full > 0) {
         const int each = min(32, min((a.K + full - 1) / full + 1, 64 / full));       // (K <= 32: enough, with one to spare where there is room)
@@ -341,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprob
     st.e = by.x + by.y;
   }
   const int first = max(0, q0 * N - off), last = min(a.V, q1 * N - off);          // this block's elements
-  if (a.K > 0) {
+  if (TOP) {
     __syncthreads();
     const int n = n_s;
     if (n > LP_LIST || n < min(a.K, last - first)) collect_slowly<T>(x, first, last, a.K, list_s, best_s, &n_s);
@@ -350,75 +342,85 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4) token_logprob
   st.n1 = warp_sum(st.n1);
   st.s = warp_sum(st.s);
   st.e = warp_sum(st.e);
-  if (lane == 0) st_s[warp] = st;
-  if (ranked) {
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    if (lane == 0 && ahead) atomicAdd(&rank_s, ahead);
+  if (ranked) ahead = __reduce_add_sync(0xffffffffu, ahead);
+  if (cluster > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");                 // (the first block runs)
+  if (cluster > 1) {
+    if (lane == 0) {
+      const uint32_t to = of_first(&all_s[part * WARPS + warp]);
+      put_first(to, st.m);
+      put_first(to + 4, st.n1);
+      put_first(to + 8, st.s);
+      put_first(to + 12, st.e);
+      put_first(of_first(&ahead_s[part * WARPS + warp]), ahead);
+    }
+    if (TOP && tid < a.K) put_first(of_first(&join_s[part * a.K + tid]), best_s[tid]);
+  } else if (lane == 0) {
+    all_s[warp] = st;
+    ahead_s[warp] = ahead;
   }
-  __syncthreads();
+  if (cluster > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (part != 0) return;                                            // (nobody reads from this block)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  if (TOP && cluster > 1) keep_best(join_s, cluster * a.K, a.K, best_s);
+  if (warp != 0) return;
   const Stats none = {-INFINITY, 0.f, 0.f, 0.f};
-  if (warp == 0) {
-    st = join(lane < WARPS ? st_s[lane] : none);
-    if (lane == 0) mine_s = st;
+  st = none;
+  ahead = 0;
+  for (int i = lane; i < cluster * WARPS; i += 32) {                  // at most four of a lane's own, then the lanes'
+    const Stats other = all_s[i], hi = st.m >= other.m ? st : other, lo = st.m >= other.m ? other : st;
+    const bool same = hi.m == lo.m;
+    const float d = lo.m - hi.m, c = same ? 1.f : expf(d), all = lo.n1 + lo.s;
+    st.m = hi.m;
+    st.n1 = hi.n1 + (same ? lo.n1 : 0.f);
+    st.s = hi.s + (same ? lo.s : c * all);
+    st.e = hi.e + (same ? lo.e : c > 0.f ? c * (lo.e + d * all) : 0.f);
+    ahead += ahead_s[i];
   }
-  if (cluster > 1) cluster_sync_all();
-  else __syncthreads();
-  if (part == 0) {
-    // every warp for itself: the sums are needed by all that write
-    st = lane == 0 ? mine_s : none;
-    ahead = lane == 0 ? rank_s : 0;
-    if (lane > 0 && lane < cluster) {
-      const uint32_t at = of_rank(&mine_s, lane);
-      st = Stats{ld_cluster_f32(at), ld_cluster_f32(at + 4), ld_cluster_f32(at + 8), ld_cluster_f32(at + 12)};
-      ahead = __float_as_int(ld_cluster_f32(of_rank(&rank_s, lane)));
+  st = join(st);
+  ahead = __reduce_add_sync(0xffffffffu, ahead);
+  const bool proper = fabsf(st.m) < INFINITY;
+  const float log_z = proper ? logf(st.n1) + log1pf(st.s / st.n1) : NAN;
+  if (lane == 0) {
+    if (a.tokens) {
+      if (!known && a.err) atomicExch(a.err, 1 + row);
+      if (a.logprob) a.logprob[row] = known ? (xt - st.m) - log_z : NAN;
+      if (a.rank) a.rank[row] = known ? ahead : -1;
     }
-    if (a.K > 0 && cluster > 1) {                                     // every block's best behind this one's
-      const int n = cluster * a.K;
-      for (int i = a.K + tid; i < n; i += THREADS) list_s[i] = ld_cluster_key(of_rank(&best_s[i % a.K], i / a.K));
-    }
-    st = join(st);
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    const bool proper = fabsf(st.m) < INFINITY;
-    const float log_z = proper ? logf(st.n1) + log1pf(st.s / st.n1) : NAN;
-    if (tid == 0) {
-      if (a.tokens) {
-        if (!known && a.err) atomicExch(a.err, 1 + row);
-        if (a.logprob) a.logprob[row] = known ? (xt - st.m) - log_z : NAN;
-        if (a.rank) a.rank[row] = known ? ahead : -1;
-      }
-      if (a.entropy) a.entropy[row] = log_z - st.e / (st.n1 + st.s);
-    }
-    if (a.K > 0) {
-      if (cluster > 1) {
-        __syncthreads();
-        keep_best(list_s, cluster * a.K, a.K, best_s);
-      }
-      if (tid < a.K) {
-        const Key k = best_s[tid];
-        a.top_ids[(long long)row * a.K + tid] = id_of(k);
-        a.top_logprobs[(long long)row * a.K + tid] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
-      }
-    }
+    if (a.entropy) a.entropy[row] = log_z - st.e / (st.n1 + st.s);
   }
-  if (cluster > 1) cluster_sync_all();                                // nobody leaves while its lists are read
+  if (TOP && lane < a.K) {
+    const Key k = best_s[lane];
+    a.top_ids[(long long)row * a.K + lane] = id_of(k);
+    a.top_logprobs[(long long)row * a.K + lane] = (float_of((uint32_t)(k >> 32)) - st.m) - log_z;
+  }
 }
 
-// Blocks a row: a cluster of them while that leaves two or so a multiprocessor, each with a tile at least.  One row of 151,936 logits,
-// five alternatives, on 1 / 2 / 4 / 8 / 16 blocks: 38 / 27 / 21 / 18 / 16 us (with an event's 6); 16 rows 37 / 29 / 23 / 21 / 21; 64
-// rows, twenty: 45 / 33 / 31 / 43 / 76; 150 rows, five: 45 / 39 / 49; 512: 97 / 92 / 117; 2,048: 244 / 291.
-template <typename T>
+constexpr size_t join_bytes(int cluster, int K) { return (size_t)cluster * (WARPS * (sizeof(Stats) + sizeof(int)) + K * sizeof(Key)); }
+
+// Blocks a row: a cluster of them while that leaves two or so a multiprocessor, each with half a tile at least.  On 1 / 2 / 4 / 8 /
+// 16 blocks: one row of 151,936 logits, five alternatives, 29.8 / 19.7 / 15.0 / 11.1 / 9.4 us; 32 rows 31.5 / 21.9 / 17.0 / 16.9 /
+// 20.6; 64 rows, twenty, 37.9 / 26.7 / 22.6 / 33.6; 150 rows, five, 39.2 / 34.2 / 40.2; 2,048 rows 226 / 276 / 380.
+template <typename T, bool TOP>
 int run_logprobs(const LpArgs& a, cudaStream_t s) {
-  constexpr size_t smem = (size_t)LP_STAGES * THREADS * LP_E * sizeof(T);
+  constexpr size_t ring = (size_t)LP_STAGES * THREADS * LP_E * sizeof(T), most = ring + join_bytes(MAX_CLUSTER, 32) > 80 * 1024 ? ring + join_bytes(MAX_CLUSTER, 32) : 80 * 1024;
   static bool attr_done = false;
   if (!attr_done) {
-    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    NV_RETURN_IF(cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_done = true;
   }
   const long long sms = num_multiprocessors();
   unsigned cluster = 1;
-  while (cluster < 16 && a.R * (long long)cluster * 8 <= sms * 9 && a.V / (int)(2 * cluster) >= THREADS * LP_E) cluster *= 2;
-  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T>, dim3(a.R * cluster), dim3(THREADS), smem, s, a));
+  while (cluster < MAX_CLUSTER && a.R * (long long)cluster * 8 <= sms * 9 && a.V / (int)(2 * cluster) >= THREADS * LP_E / 2) cluster *= 2;
+  // Two blocks a multiprocessor at most ask for more than a third of its memory, so that three do not share one while others
+  // have none (64 rows, twenty alternatives: 27.5 and 22.6 us).  Larger clusters have too few places then (32 rows: 16.9 and 19.0).
+  size_t smem = ring + join_bytes(cluster, a.K);
+  if (cluster <= 4 && a.R * (long long)cluster <= 2 * sms && smem < 80 * 1024) smem = 80 * 1024;
+  NV_RETURN_IF(launch_dep_clusters(cluster, token_logprobs_kernel<T, TOP>, dim3(a.R * cluster), dim3(THREADS), smem, s, a));
   NV_RETURN_LAST();
 }
 
@@ -436,5 +438,6 @@ NV_API int nv_token_logprobs(const void* logits, int dt, long long stride, int R
   if (K > 0 && (!top_ids || !top_logprobs)) return NV_ERR_BAD_SIZE;
   if (R == 0) return NV_OK;
   const LpArgs a = {logits, stride, tokens, logprob, entropy, rank, top_ids, top_logprobs, err, R, V, K};
-  return dt == NV_DT_F32 ? run_logprobs<float>(a, s) : run_logprobs<bf16>(a, s);
+  if (K > 0) return dt == NV_DT_F32 ? run_logprobs<float, true>(a, s) : run_logprobs<bf16, true>(a, s);
+  return dt == NV_DT_F32 ? run_logprobs<float, false>(a, s) : run_logprobs<bf16, false>(a, s);
 }
