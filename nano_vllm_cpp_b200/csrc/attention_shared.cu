@@ -793,3 +793,18 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
                           has_sink, sink_score, HeadGate{gate, gate_ld}));
   NV_RETURN_LAST();
 }
+
+// The same with what a step's layers have in common in one array on the host (fewer arguments to convert a call): type of queries,
+// cache and result; Hq, Hkv, D, page; R, first, group, members, M, cu, len, lead, groups; own_splits, shared_splits, float_weights.
+NV_API int nv_attention_decode_shared_plan(const long long* plan, const void* qkv, int q_stride, const void* kc, const void* vc,
+                                           const int* block_table, int max_blocks, const int* row_entry, const int* positions,
+                                           const int* rows, float scale, void* out, int num_pages, float* scratch, int* err,
+                                           int has_sink, float sink_score, float softcap, const float* gate, long long gate_ld,
+                                           cudaStream_t stream) {
+  const int dt = (int)plan[0];
+  return nv_attention_decode_shared(qkv, dt, q_stride, kc, vc, dt, block_table, max_blocks, row_entry, positions, rows, (int)plan[5],
+                                    (const int*)plan[6], (const int*)plan[7], (const int*)plan[8], (int)plan[9], (const int*)plan[10],
+                                    (const int*)plan[11], (const int*)plan[12], (int)plan[13], scale, out, dt, (int)plan[1],
+                                    (int)plan[2], (int)plan[3], (int)plan[4], num_pages, (int)plan[14], (int)plan[15], scratch, err,
+                                    has_sink, sink_score, (int)plan[16], softcap, gate, gate_ld, stream);
+}

@@ -506,18 +506,21 @@ class SharedPrefix:
         self.places = tuple(at + 4 * n for n in (0, R, 2 * R, 3 * R, 3 * R + G + 1, 3 * R + 2 * G + 1))
 
     def splits(self, Hq: int, Hkv: int, D: int, k_cache, terms: int, max_context: int):
-        """How many parts a row's own keys and the shared ones are cut into for these sizes (no shared part: 0), worked out
-        once for all layers that have them."""
+        """How many parts a row's own keys and the shared ones are cut into for these sizes (no shared part: 0), and what the
+        launcher takes for a plan, worked out once for all layers that have them."""
         page, dtype = k_cache.shape[2], k_cache.dtype
         key = Hq, Hkv, D, page, dtype, terms, max_context
         if key not in self._splits:
             _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
-            pair = lib().nv_attention_decode_splits_of(self.R, Hq, Hkv, D, max_context, num_sms()), 0
+            pair = lib().nv_attention_decode_splits_of(self.R, Hq, Hkv, D, max_context, num_sms()), 0, None
             if attention_sharing_pays(self.R, self.members, self.groups, Hq, Hkv, D, page, dtype, self.repeated):
                 sizes = self.members, self.groups, Hq, Hkv, D, page, _DT[dtype]
                 own = max(1, max_context - self.shortest // page * page)          # the most keys a row reads for itself
                 ours = lib().nv_attention_shared_splits(*sizes, terms, self.longest)
-                pair = lib().nv_attention_shared_own_splits(self.R, *sizes, ours, own), ours
+                splits = lib().nv_attention_shared_own_splits(self.R, *sizes, ours, own)
+                first, group, members, cu, lens, leads = self.places
+                pair = splits, ours, (ctypes.c_longlong * 17)(_DT[dtype], Hq, Hkv, D, page, self.R, first, group, members, self.members, cu,
+                                                              lens, leads, self.groups, splits, ours, terms)
             self._splits[key] = pair
         return self._splits[key]
 
@@ -560,18 +563,16 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     _need(block_table.dim() == 2 and shared.reach // page <= block_table.shape[1],
           "attention_decode_shared: a prefix reaches beyond the block tables")
     terms = 1 if float_weights or sink_score is not None else 0
-    splits, ours = shared.splits(Hq, Hkv, D, k_cache, terms, max_context)
+    splits, ours, plan = shared.splits(Hq, Hkv, D, k_cache, terms, max_context)
     if ours == 0:
         return _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, 0, out, Hq, Hkv, D, R, splits, rows, err,
                               sink_score, float_weights, softcap, gate, (0, None, None, 0), True)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)
-    code, first, group, members, cu, lens, leads = _DT[dtype], *shared.places
-    _check(lib().nv_attention_decode_shared(qkv.data_ptr(), code, width, k_cache.data_ptr(), v_cache.data_ptr(), code,
-                                            block_table.data_ptr(), block_table.shape[1], row_entry.data_ptr(), positions.data_ptr(),
-                                            _p(rows), R, first, group, members, shared.members, cu, lens, leads, shared.groups,
-                                            scale, out.data_ptr(), code, Hq, Hkv, D, page, shape[0], splits, ours, scratch.data_ptr(),
-                                            _p(err.t if err is not None else _global_err().t), (0 if sink_score is None else 1),
-                                            float(sink_score or 0.0), terms, float(softcap), *_head_gates(gate, T, Hq), _stream()),
+    _check(lib().nv_attention_decode_shared_plan(ctypes.addressof(plan), qkv.data_ptr(), width, k_cache.data_ptr(), v_cache.data_ptr(),
+                                                 block_table.data_ptr(), block_table.shape[1], row_entry.data_ptr(),
+                                                 positions.data_ptr(), _p(rows), scale, out.data_ptr(), shape[0], scratch.data_ptr(),
+                                                 _p(err.t if err is not None else _global_err().t), (0 if sink_score is None else 1),
+                                                 float(sink_score or 0.0), float(softcap), *_head_gates(gate, T, Hq), _stream()),
            "attention_decode_shared")
 
 
