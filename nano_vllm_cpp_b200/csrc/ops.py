@@ -465,14 +465,17 @@ class SharedPrefix:
 
     ``groups``: (rows, positions) pairs: the rows (places among the ``rows`` rows that the call takes) hold the same keys and
     values at their first so many positions, each in pages of its own or in common ones; whole pages of them are read through
-    the block table of the first of them.  A row is in one group at most; the others read all their keys themselves."""
+    the block table of the first of them.  A row is in one group at most; the others read all their keys themselves.  A row may end
+    inside its prefix; the values there are finite numbers, also behind its end (its group's other rows see them)."""
 
-    def __init__(self, groups, rows: int, device, *, facts=None, buf=None):
-        """``facts`` (longest prefix, what every row shares at least, positions that are read once instead of again): what the
-        launches go by, where other steps of the same shape are to run the same ones.  ``buf``: the packed arrays where they
-        are on the device already (``pack``)."""
-        packed, self.members = self.pack(groups, rows)
-        self.R, self.groups, self._splits = rows, len(groups), {}
+    def __init__(self, groups, rows: int, device, *, facts=None, room=None, buf=None):
+        """``facts`` (longest prefix, what every row shares at least, positions that are read once instead of again) and ``room``
+        (grouped rows and groups, at least as many as there are): what the launches go by, where other steps of the same shape
+        are to run the same ones.  ``buf``: the packed arrays where they are on the device already (``pack``)."""
+        packed, members = self.pack(groups, rows, room[1] if room else 0)
+        self.members, self.groups = room or (members, len(groups))
+        _need(members <= self.members <= rows, "SharedPrefix: room for the grouped rows, and no more than there are rows")
+        self.R = rows
         self.longest, self.shortest, self.repeated = self.facts(groups, rows) if facts is None else facts
         self.reach = max((n for _, n in groups), default=0)          # positions that the block tables must cover
         self.bind(torch.tensor(packed, dtype=torch.int32).to(device) if buf is None else buf)
@@ -484,9 +487,12 @@ class SharedPrefix:
         return max(lens, default=0), min(lens, default=0) if whole else 0, sum(n * (len(own) - 1) for own, n in groups)
 
     @staticmethod
-    def pack(groups, rows: int):
+    def pack(groups, rows: int, room: int = 0):
         """The host's arrays in one list: per row its shared positions and its group (or -1), the groups' rows one after the
-        other (``rows`` places), where each group's start, its positions, and its first row; and the number of grouped rows."""
+        other (``rows`` places), where each group's start, its positions, and its first row; and the number of grouped rows.
+        ``room``: groups without rows follow, up to so many."""
+        _need(room == 0 or room >= len(groups), "SharedPrefix: room for fewer groups than there are")
+        empty = max(0, room - len(groups))
         first, group, members, cu, lens = [0] * rows, [-1] * rows, [], [0], []
         for g, (own, n) in enumerate(groups):
             _need(len(own) > 0 and n >= 0, "SharedPrefix: a group has a row at least and no negative prefix")
@@ -498,11 +504,14 @@ class SharedPrefix:
             cu.append(len(members))
             lens.append(int(n))
         leads = [int(own[0]) for own, _ in groups]
-        return first + group + members + [0] * (rows - len(members)) + cu + lens + leads, len(members)
+        none = [0] * empty
+        return first + group + members + [0] * (rows - len(members)) + cu + [cu[-1]] * empty + lens + none + leads + none, len(members)
 
     def bind(self, buf) -> None:
+        """Has the calls read the packed arrays ``buf``, of as many rows and groups as these."""
         R, G, at = self.R, self.groups, buf.data_ptr()
-        self.buf = buf
+        _need(buf.dtype == torch.int32 and buf.numel() >= 3 * R + 3 * G + 1, "SharedPrefix: the packed arrays are int32, of these rows and groups")
+        self.buf, self._splits = buf, {}                             # (what the launcher takes for a plan has their addresses)
         self.places = tuple(at + 4 * n for n in (0, R, 2 * R, 3 * R, 3 * R + G + 1, 3 * R + 2 * G + 1))
 
     def splits(self, Hq: int, Hkv: int, D: int, k_cache, terms: int, max_context: int):
@@ -542,9 +551,9 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
     for all its rows, as one product of their query heads, and joined with what each row has of its own, where that pays
     (``attention_sharing_pays``; else ``attention_decode`` runs, and every row reads its keys itself).  A row sees the
     positions up to its own, none of them masked otherwise (layers with a window, chunks or biases by distance take
-    ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``,
-    ``gate``: see there.  As there, the kernel in front may write the query rows and each row's newest page, nothing else that
-    is read here."""
+    ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have
+    one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``, ``gate``: see there.  As there, the kernel
+    in front may write the query rows and each row's newest page, nothing else that is read here."""
     _ours("attention_decode_shared", qkv, k_cache, v_cache, block_table, row_entry, positions, out, rows, shared.buf)
     _i32(block_table, row_entry, positions, rows)
     T, width = qkv.shape

@@ -36,6 +36,7 @@ class StepError(RuntimeError):
 GRAPH_MAX_TOKENS = 1024
 MAX_GRAPHS = 48             # captured steps with a portion among their entries; further such shapes run launch by launch
 MAX_DECODE_GRAPHS = 64      # captured steps of single rows only (one per batch size, with and without sampling)
+MAX_SHARED_GRAPHS = 32      # ... and of either kind whose rows share prefixes; further such shapes run as if they shared nothing
 GRAPH_MAX_LOGIT_BYTES = 64 << 20
 
 
@@ -275,8 +276,7 @@ class ModelRunner:
         if not entries:
             return torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
         logits = batch = None
-        shared = self._shared_rows(entries)
-        key = self._graph_key(entries, None, shared)
+        key, shared = self._captured_form(entries, None, self._shared_rows(entries))
         if key is not None:
             logits, batch = self._graph_step(entries, None, key, shared)
         if batch is None:
@@ -317,7 +317,9 @@ class ModelRunner:
         batch = None
         picked = [r for r, x in enumerate(nucleus or []) if x is not None]
         shared = self._shared_rows(entries)
-        key = None if picked else self._graph_key(entries, sampling, shared)
+        key = None
+        if not picked:
+            key, shared = self._captured_form(entries, sampling, shared)
         if key is not None:
             logits, batch = self._graph_step(entries, sampling, key, shared)
         if batch is None:
@@ -430,16 +432,34 @@ class ModelRunner:
 
     @staticmethod
     def _rounded_facts(groups, rows: int):
-        """What a captured step's launches go by: the powers of two around the step's own numbers, so that steps of about the
-        same prefixes share a capture."""
+        """What a captured step's launches go by, so that steps of about the same prefixes share a capture: the powers of two
+        around the prefixes' lengths, and room for some more grouped rows and groups (up to a quarter)."""
         longest, shortest, repeated = ops.SharedPrefix.facts(groups, rows)
         floor = lambda n: 1 << (n.bit_length() - 1) if n > 0 else 0
-        return 1 << max(0, longest - 1).bit_length(), floor(shortest), floor(repeated)
+
+        def room(n):
+            step = 1 << max(0, (n - 1).bit_length() - 3)
+            return (n + step - 1) // step * step
+
+        members = min(rows, room(sum(len(own) for own, _ in groups)))
+        return (1 << max(0, longest - 1).bit_length(), floor(shortest), floor(repeated)), (members, room(len(groups)))
+
+    def _captured_form(self, entries: list, sampling, shared):
+        """The step's ``_graph_key``, and its groups: none, where they would take one capture too many."""
+        key = self._graph_key(entries, sampling, shared)
+        if shared is not None and key is not None and key not in self._graphs and \
+                sum(1 for g in self._graphs.values() if g[-1] is not None) >= MAX_SHARED_GRAPHS:
+            return self._graph_key(entries, sampling), None
+        return key, shared
+
+    @staticmethod
+    def _packed(groups, rows: int, room: int = 0):
+        return np.array(ops.SharedPrefix.pack(groups, rows, room)[0], dtype=np.int32)
 
     def _share(self, batch, shared) -> None:
         if shared is not None:
             groups, rows = shared
-            buf = self.stager.stage(np.array(ops.SharedPrefix.pack(groups, rows)[0], dtype=np.int32))
+            buf = self.stager.stage(self._packed(groups, rows))
             batch.shared = ops.SharedPrefix(groups, rows, self.device, buf=buf)
 
     def _sample_into_feed(self, logits, batch) -> None:
@@ -486,8 +506,7 @@ class ModelRunner:
             return None                        # (a captured step keeps its logits tensor for good)
         key = (len(entries), T, sum(1 for e in entries if len(e.tokens) == 1), W, sampling is not None)
         if shared is not None:                 # ... and how many groups and rows share prefixes of about which lengths
-            groups, rows = shared
-            key += (len(groups), sum(len(m) for m, _ in groups), *self._rounded_facts(groups, rows))
+            key += self._rounded_facts(*shared)
         return key
 
     def _graph_step(self, entries: list, sampling, key, shared=None):
@@ -505,8 +524,8 @@ class ModelRunner:
                 self._seen.pop(next(iter(self._seen)))
             self._seen[key] = seen
             decode = key[2] == key[0]
-            kept = sum(1 for k in self._graphs if (k[2] == k[0]) == decode)
-            if seen < 2 or kept >= (MAX_DECODE_GRAPHS if decode else MAX_GRAPHS):
+            kept = sum(1 for k, g in self._graphs.items() if (k[2] == k[0]) == decode and g[-1] is None)
+            if seen < 2 or (shared is None and kept >= (MAX_DECODE_GRAPHS if decode else MAX_GRAPHS)):
                 return None, None          # a shape seen once is not worth a capture
             T, W = key[1], key[3]
             seg, total = batch_layout(S, T, W, len(self.manager.pools), self.max_blocks, sampling is not None)
@@ -516,10 +535,10 @@ class ModelRunner:
             batch.max_context = batch.max_single_context = self.max_model_len
             shared_dev = None
             if shared is not None:
-                groups, rows = shared
-                packed = np.array(ops.SharedPrefix.pack(groups, rows)[0], dtype=np.int32)
+                facts, room = self._rounded_facts(*shared)
+                packed = self._packed(*shared, room[1])
                 shared_dev = self.stager.stage(packed, torch.empty(len(packed), dtype=torch.int32, device=self.device))
-                batch.shared = ops.SharedPrefix(groups, rows, self.device, facts=self._rounded_facts(groups, rows), buf=shared_dev)
+                batch.shared = ops.SharedPrefix(*shared, self.device, facts=facts, room=room, buf=shared_dev)
             logits = self._forward(batch)       # warms up; also this step's result
             if sampling is not None:
                 self._sample_into_feed(logits, batch)
@@ -545,7 +564,7 @@ class ModelRunner:
         graph, static_dev, static_logits, launches, shared_dev = g
         batch = self.prepare(entries, static_dev, sampling, views=False)
         if shared is not None:
-            self.stager.stage(np.array(ops.SharedPrefix.pack(*shared)[0], dtype=np.int32), shared_dev)
+            self.stager.stage(self._packed(*shared, key[-1][1]), shared_dev)
         graph.replay()
         ops.add_launches(launches)
         return static_logits, batch

@@ -257,6 +257,35 @@ def test_steps_whose_rows_share_prefixes(graphs, folders, always_shared):
     assert shared[-1] == ([([0, 4], 64), ([1, 3, 5], 144)], 6)
 
 
+@pytest.mark.parametrize("limit", [32, 1, 0])
+def test_captured_steps_whose_families_change_size(limit, folders, always_shared, monkeypatch):
+    """Ten replies and a lone request, then nine and two: one captured shape.  Shapes beyond the limit run as if nothing was shared.
+    The results are those of a run that launches the same operators (another operator's rounding may turn a router's near tie)."""
+    from nano_vllm_cpp_b200.engine import runner
+    monkeypatch.setattr(runner, "MAX_SHARED_GRAPHS", limit)
+    runners = [make_runner(folders["D"], "bfloat16", shared_prefix=s, cuda_graphs=g) for s, g in ((True, True), (limit > 0, False))]
+    for r in runners:
+        r.step([entry("a0", ids_for("D", 70, salt=1), []), entry("c0", ids_for("D", 40, salt=3), [])])
+        r.fork("a0", [f"a{i}" for i in range(1, 10)])
+    live = ["c0"] + [f"a{i}" for i in range(10)]
+    for k in range(9):
+        if k == 3:
+            for r in runners:
+                r.close("a4")
+                r.step([entry("c1", ids_for("D", 33, salt=7), [])])
+            live[live.index("a4")] = "c1"
+        if k == 6:
+            for r in runners:
+                r.close("c1")
+                r.fork("c0", ["c2"])
+            live[live.index("c1")] = "c2"                # (two groups: another shape)
+        step = [entry(x, [ids_for("D", 9, salt=20 + i)[k]]) for i, x in enumerate(live)]
+        got, want = (r.step(step).double().cpu() for r in runners)
+        assert float((got - want).abs().max()) <= 2e-2 + 3e-2 * float(want.abs().max())
+    captured = [g[-1] is not None for g in runners[0]._graphs.values()]
+    assert captured == {32: [True, True], 1: [True, False], 0: [False]}[limit]
+
+
 @pytest.mark.parametrize("case", ["C", "R"])
 def test_models_with_windows_and_states_share_what_they_can(case, folders, always_shared):
     """Layers with a window keep to themselves; layers that read another's keys share as it does."""

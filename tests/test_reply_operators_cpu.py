@@ -59,6 +59,34 @@ def test_shared_prefix_packs_its_groups():
     assert ops.SharedPrefix.pack([], 2) == ([0, 0, -1, -1, 0, 0, 0], 0)
 
 
+def test_shared_prefix_packs_room_for_more_groups():
+    packed, members = ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6, 4)
+    assert members == 3 and packed[:18] == ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6)[0][:18]
+    assert packed[18:23] == [0, 2, 3, 3, 3] and packed[23:27] == [32, 7, 0, 0] and packed[27:] == [4, 2, 0, 0]
+    with pytest.raises(ops.KernelError):
+        ops.SharedPrefix.pack([([4, 1], 32), ([2], 7)], 6, 1)
+
+
+def test_shared_prefix_refuses_arrays_and_room_that_do_not_fit():
+    groups = [([0, 1], 32)]
+    buf = torch.zeros(13, dtype=torch.int32)                                # 3 rows, 1 group
+    ops.SharedPrefix(groups, 3, "cpu", buf=buf)
+    for kw in (dict(buf=buf[:12]), dict(buf=buf.long()), dict(room=(1, 1)), dict(room=(4, 1)), dict(room=(3, 2), buf=buf)):
+        with pytest.raises(ops.KernelError):
+            ops.SharedPrefix(groups, 3, "cpu", **kw)
+
+
+def test_steps_of_about_the_same_prefixes_share_a_capture():
+    from nano_vllm_cpp_b200.engine.runner import ModelRunner
+    rounded = lambda sizes, n, rows: ModelRunner._rounded_facts([([0] * s, n) for s in sizes], rows)
+    assert rounded([8], 2048, 8) == ((2048, 2048, 8192), (8, 1)) and rounded([8], 2049, 8) == ((4096, 2048, 8192), (8, 1))
+    assert rounded([3, 2], 100, 6) == ((128, 0, 256), (5, 2)) and rounded([33], 64, 64)[1] == (40, 1) and rounded([33], 64, 34)[1] == (34, 1)
+    for rows in range(2, 70):
+        for k in range(2, rows + 1):
+            members, groups = rounded([k] * 9, 16, 9 * rows)[1]
+            assert 9 * k <= members <= min(9 * rows, 9 * k * 5 // 4 + 1) and groups == 10
+
+
 def test_sharing_is_a_matter_of_bytes_rows_and_heads():
     pays = lambda R, M, g, Hq, Hkv, repeated, dt=1, D=128, page=16: ops.lib().nv_attention_shared_pays(R, M, g, Hq, Hkv, D, page, dt, repeated)
     assert not pays(4, 0, 0, 16, 16, 0) and not pays(4, 4, 1, 16, 16, 0)

@@ -139,6 +139,15 @@ def test_log_probabilities_of_tokens_outside_the_vocabulary():
         err.check("logprobs")
 
 
+def test_log_probabilities_of_rows_far_apart():
+    """Rows that begin beyond 2^32 bytes, and beyond 2^31 elements."""
+    gap = (1 << 31) + 8
+    pool = torch.empty(2 * gap + 5000, dtype=torch.bfloat16, device=DEV)                   # 8.6 GB
+    x = pool.as_strided((3, 5000), (gap, 1))
+    x.copy_(rnd(3, 5000, seed=12))
+    check_logprobs(x, i32([0, 4999, 77]), 6)
+
+
 def test_log_probabilities_give_the_same_bits_twice():
     x = rnd(300, 20011, seed=5) * 3
     tokens = torch.arange(300, dtype=torch.int32, device=DEV)
@@ -443,6 +452,34 @@ def test_attention_on_two_streams_at_once():
                 got.append((x is d, x.run()))
     torch.cuda.synchronize()
     assert all(torch.equal(out, alone[which]) for which, out in got)
+
+
+def test_attention_by_arrays_with_room_for_more_rows_and_groups():
+    """One object whose arrays are replaced by those of other groups, as steps of a captured shape replace them."""
+    o = ops()
+    groups, lengths = GROUPS[0]
+    c = Case(8, 2, 64, lengths, groups)
+    facts = o.SharedPrefix.facts(groups, 10)
+    pack = lambda g: i32(o.SharedPrefix.pack(g, 10, 7)[0])
+    shared = o.SharedPrefix(groups[:1], 10, DEV, facts=facts, room=(10, 7), buf=pack(groups[:1]))
+    want, weight, score = c.want()
+    for g in (groups[:1], groups, groups[1:3]):
+        shared.bind(pack(g))
+        shared.reach = 300
+        got = c.run(shared=shared, stale=NAN)
+        assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_far_into_a_cache(dtype):
+    """Pages whose bytes lie beyond 2^32."""
+    c = Case(8, 2, 128, [70, 81, 66, 90], [([0, 1, 2], 64)], 16, dtype)
+    n = (1 << 32) // (2 * 16 * 128 * c.k.element_size()) + 50
+    far = torch.arange(c.k.shape[0], device=DEV) * 3 + n - 3 * c.k.shape[0]
+    k, v = (torch.zeros((n, 2, 16, 128), dtype=dtype, device=DEV) for _ in range(2))
+    k[far], v[far] = c.k, c.v
+    c.k, c.v, c.table = k, v, torch.where(c.table >= 0, far[c.table.clamp(min=0).long()].to(torch.int32), c.table)
+    c.check()
 
 
 def test_attention_reports_a_missing_page():
