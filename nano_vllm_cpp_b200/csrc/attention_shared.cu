@@ -1,14 +1,20 @@
 // Decode attention for rows that share a prefix: several replies to one prompt, or requests behind one system prompt.
 //
 // The rows of a group hold the same keys and values at their first len[g] positions.  The whole pages of these are read once,
-// through the block table of the group's first row; a page that the prefix ends in every row reads for itself.  A row's softmax over all its keys is put together from parts with sums of their own,
+// through the block table of the group's first row; a page that the prefix ends in every row reads for itself.  A row's softmax
+// over all its keys is put together from parts with sums of their own,
 //
 //   m = max over the part of s_j,  l = sum e^(s_j - m),  o = sum e^(s_j - m) v_j;      out = sum_p e^(m_p - M) o_p / sum_p e^(m_p - M) l_p
 //
 // so the shared part can be worked out for all rows of the group at once, its keys and values read once instead of once a
 // row: per kv head it is a matrix product of the (row, query head) pairs that read it.  Three launches: the shared parts (here),
-// every row's own keys, from the page on that holds position len[g] (the split-key kernel of attention_decode.cu), and their join (here).  A row that
-// belongs to no group has no shared part; of a group's keys a row sees those up to its own position.
+// every row's own keys, from the page on that holds position len[g] (the split-key kernel of attention_decode.cu), and their join
+// (here).  A row that belongs to no group has no shared part; of a group's keys a row sees those up to its own position.
+//
+// What bounds it (bfloat16, heads of 128): 64 rows of 28 heads on 4 behind 8,192 positions, 16 to 512 of their own, take 38.4 us
+// (each row by itself: 221), 18 of it the shared part, 13 the rows' own keys, 5 to 7 the join of up to 20 parts.  128 rows behind
+// 16,384 take 61 (673), 40 of it the shared part: 64 keys of two blocks of 128 pairs in 1.1 us a multiprocessor, where its
+// exponentials alone take 0.6, the products 0.8 (those of different shapes do not overlap), and the 64 KB of keys and values from L2 0.9.
 #include "tcgen05.cuh"
 
 int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
@@ -217,12 +223,13 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
 }
 
 // The tensor-core form, for bfloat16 and head sizes in steps of 16 from 32 on: a CTA takes 128 pairs of one kv head and one split
-// of the keys, 64 keys at a time.  S = Q K^T and O += P V are tcgen05.mma with S (two buffers) and O in tensor memory:
+// of the keys, 64 keys at a time.  S = Q K^T and O += P V are tcgen05.mma with S, P (two buffers) and O in tensor memory:
 //   warp 0     fetches the pages of K (two buffers) and V as TMA boxes of one page x 64 elements, a lane a box
-//   warp 1     allocates tensor memory; one thread issues the products
-//   warps 2-5  gather the queries of the tile's pairs into shared memory (128-byte swizzle), then a thread owns a pair: it reads its
-//              row of S, keeps its maximum and sum, writes P as bfloat16 over its scores, from where the second product takes it (three
-//              terms: into shared memory), and at the end its row of O, undivided, with maximum and sum to the scratch
+//   warp 1     allocates tensor memory; issues the products, a lane of it elected
+//   warps 2-5  gather the queries of the tile's pairs into shared memory (128-byte swizzle), then a thread owns a pair: it takes its
+//              row of S into registers, whereupon the next product may write S, keeps the row's maximum and sum, writes P as bfloat16
+//              to where the second product takes it (three terms: into shared memory), and at the end its row of O, undivided, with
+//              maximum and sum to the scratch
 // All keys of a split are seen by all pairs, but for those behind a row's own position, so there is no mask in most blocks.  TERMS =
 // 3: the float32 weights enter the product with the values as three bfloat16 terms (all their bits) instead of one rounded.
 // Heads between the forms' sizes: the boxes reach beyond the pages' rows and are filled with zeros.
@@ -234,6 +241,130 @@ __device__ __forceinline__ void bulk_store(void* to, const void* from, uint32_t 
 }
 __device__ __forceinline__ void bulk_store_wait() {
   asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// A warp's 32 queries of a tile of `pairs` pairs (lane's: batch row t, head h) into shared memory, D / 8 lanes a row and sixteen loads of a
+// lane under way; rows of nobody and columns beyond the head are zeros.  q: the warp's quarter of the tile.
+template <int D>
+__device__ __forceinline__ void gather_queries(const SharedArgs& a, uint8_t* Qs, int q, int lane, int pairs, int t, int h) {
+  constexpr int PER = D / 8, AT_ONCE = 32 / PER, LOADS = 32 / AT_ONCE < 16 ? 32 / AT_ONCE : 16;      // (PER is 8, 16 or 32)
+  const int c = lane % PER;
+  const long long place = (long long)t * a.q_stride + (long long)h * a.D;
+#pragma unroll
+  for (int i0 = 0; i0 < 32; i0 += LOADS * AT_ONCE) {
+    uint4 v[LOADS];
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int i = i0 + u * AT_ONCE + lane / PER;
+      const long long from = __shfl_sync(0xffffffffu, place, i);
+      v[u] = q * 32 + i < pairs && c * 8 < a.D ? *(const uint4*)((const bf16*)a.q + from + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int row = q * 32 + i0 + u * AT_ONCE + lane / PER;
+      *(uint4*)(Qs + (c / 8) * (ST_PAIRS * 128) + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[u];
+    }
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+// A pair's next block of scores, from key j on, becomes weights against its reference m; returns the sum of its weights, l among them.
+// The reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost bfloat16 and the float32
+// sums nothing), so that O is rescaled, by alpha, once in a long while.
+__device__ __forceinline__ float softmax_step(const ScoreMap& map, float* s, int j, int limit, float& m, float& alpha, float l) {
+  if (map.cap1 > 0.f) {
+#pragma unroll
+    for (int c = 0; c < ST_KEYS; ++c) s[c] = capped_log2(map, s[c]);
+  }
+  if (j + ST_KEYS > limit) {
+#pragma unroll
+    for (int c = 0; c < ST_KEYS; ++c)
+      if (j + c >= limit) s[c] = -INFINITY;
+  }
+  float mx4[4] = {s[0], s[1], s[2], s[3]};                       // four chains, three numbers a step
+#pragma unroll
+  for (int c = 4; c < ST_KEYS - 4; c += 8) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(fmaxf(s[c + u], s[c + 4 + u]), mx4[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], s[ST_KEYS - 4 + u]);
+  const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+  if (mx > m && (m == -INFINITY || (mx - m) * map.in > 8.f)) {
+    alpha = m == -INFINITY ? 0.f : ex2_fast((m - mx) * map.in);
+    m = mx;
+  }
+  const float ms = m == -INFINITY ? 0.f : m * map.in;
+  // two elements an instruction where there is one
+  float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 in2 = make_float2(map.in, map.in), ms2 = make_float2(-ms, -ms);
+#pragma unroll
+  for (int c = 0; c < ST_KEYS; c += 4) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float2 e = fma2(make_float2(s[c + 2 * u], s[c + 2 * u + 1]), in2, ms2);
+      s[c + 2 * u] = ex2_fast(e.x);
+      s[c + 2 * u + 1] = ex2_fast(e.y);
+      sum2[u] = add2(sum2[u], make_float2(s[c + 2 * u], s[c + 2 * u + 1]));
+    }
+  }
+  return l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+}
+// A row's weights as bfloat16 into tensor memory, two in a column.
+__device__ __forceinline__ void put_weights(uint32_t to, const float* s) {
+  uint32_t w[ST_KEYS / 2];
+#pragma unroll
+  for (int c = 0; c < ST_KEYS / 2; ++c) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(s[2 * c], s[2 * c + 1]);
+    w[c] = *(const uint32_t*)&b;
+  }
+  tmem_st32_u32(to, w);
+}
+// The warp's rows of O, where any of them is to be rescaled.
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t tmem_o, float alpha) {
+  if (!__any_sync(0xffffffffu, alpha != 1.f)) return;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    float o[32];
+    tmem_ld32(tmem_o + c * 32, o);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) o[j] *= alpha;
+    tmem_st32(tmem_o + c * 32, o);
+  }
+}
+
+// A pair's part: its row of O as it is (some: a product has written it; else zeros), relative to m, with maximum and sum.  The row
+// goes through shared memory (all of it is free now; rows a chunk of 16 bytes further apart than they are long, so that a warp's
+// threads write to different banks) and leaves in one copy: whole lines instead of 16 bytes in each of 32.
+template <int D>
+__device__ __forceinline__ void leave_part(const SharedArgs& a, uint8_t* row, uint32_t tmem_o, bool some, bool live, size_t at, float m,
+                                           float l, float in) {
+  if (live) {
+    // (m is in the units of the raw or the capped scores: `in` takes it to base 2)
+    a.part_ml[at * 2] = m == -INFINITY ? -1e30f : m * in * 0.6931471805599453f;
+    a.part_ml[at * 2 + 1] = l;
+  }
+  constexpr int W = D < 128 ? D : 128;                  // columns whose loads are under way at once
+#pragma unroll
+  for (int c0 = 0; c0 < D; c0 += W) {
+    float o[W];
+    if (some) {
+#pragma unroll
+      for (int c = 0; c < W; c += 32) tmem_ld32_nowait(tmem_o + c0 + c, o + c);
+      tmem_ld_wait();
+      tmem_ld_fence<W>(o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) o[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < W; j += 4) *(float4*)(row + (c0 + j) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+  }
+  fence_async_smem();
+  if (live) bulk_store(a.part_o + at * a.D, row, (uint32_t)a.D * 4);
+  bulk_store_wait();
 }
 
 template <int D>
@@ -249,7 +380,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   constexpr int SL = D / 64, VB = st_v_buffers<D, TERMS>();
   constexpr uint32_t Q_SLAB = ST_PAIRS * 128, KV_SLAB = ST_KEYS * 128, P_TILE = ST_PAIRS * 128;
   extern __shared__ __align__(1024) uint8_t st_smem_raw[];
-  __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full, pv_done;
+  __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_free, p_full, pv_done;
   __shared__ uint32_t tmem_base_s;
 
   uint8_t* smem = (uint8_t*)(((uintptr_t)st_smem_raw + 1023) & ~(uintptr_t)1023);
@@ -269,8 +400,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       mbar_init(&k_empty[b], 1);
       mbar_init(&v_full[b], 1);
       mbar_init(&v_empty[b], 1);
-      mbar_init(&s_full[b], 1);
     }
+    mbar_init(&s_full, 1);
+    mbar_init(&s_free, 4);
     mbar_init(&p_full, 4);
     mbar_init(&pv_done, 1);
     mbar_fence_init();
@@ -288,7 +420,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int share = max(a.split_keys, ((len + a.splits - 1) / a.splits + ST_KEYS - 1) / ST_KEYS * ST_KEYS);
     const int j_lo = min(len, split * share), j_hi = min(len, j_lo + share);
     const int n_blocks = (j_hi - j_lo + ST_KEYS - 1) / ST_KEYS;
-    const uint32_t tmem_s = tmem_base, tmem_o = tmem_base + 2 * ST_KEYS;
+    const uint32_t tmem_s = tmem_base, tmem_p = tmem_base + ST_KEYS, tmem_o = tmem_base + 2 * ST_KEYS;      // (P: two buffers)
     const int lead_t = a.rows ? a.rows[tile.lead] : tile.lead;
     // A block's keys behind the split's end are not loaded; their weights are zero, their values must be finite numbers.  Only the
     // first VB blocks meet what the shared memory held before.
@@ -341,7 +473,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       // ---------------------------------------------------------------- MMA issuer
       grid_dep_wait();
       grid_dep_launch();
-      if (lane == 0 && n_blocks > 0) {
+      const int n = __shfl_sync(0xffffffffu, n_blocks, 0);
+      const uint32_t tmem_s = __shfl_sync(0xffffffffu, tmem_base, 0), tmem_p = tmem_s + ST_KEYS, tmem_o = tmem_s + 2 * ST_KEYS;
+      if (n > 0) {
         const uint32_t idesc_s = instr_desc(ST_KEYS), idesc_o = instr_desc_b_mn(D);
         const uint32_t q_addr = smem_u32(Qs), k_addr = smem_u32(Ks), v_addr = smem_u32(Vs), p_addr = smem_u32(Ps);
         uint64_t dq[SL], dk[2][SL], dp[TERMS];
@@ -360,16 +494,21 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           tc_fence_after();
 #pragma unroll
           for (int s = 0; s < SL; ++s)
-            umma_bf16_x4(tmem_s + b * ST_KEYS, dq[s], b ? dk[1][s] : dk[0][s], idesc_s, s ? 1u : 0u);
-          umma_commit(&k_empty[b]);
-          umma_commit(&s_full[b]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_warp(tmem_s, dq[s] + k * 2, (b ? dk[1][s] : dk[0][s]) + k * 2, idesc_s, (s || k) ? 1u : 0u);
+          umma_commit_warp(&k_empty[b]);
+          umma_commit_warp(&s_full);
         };
         mbar_wait(&q_full, 0, a.err, 0x7304);
         tc_fence_after();
         issue_s(0);
-        if (n_blocks > 1) issue_s(1);
-        for (int i = 0; i < n_blocks; ++i) {
-          mbar_wait(&p_full, i & 1, a.err, 0x7305);  // P(i) is written, S(i) is read, O is rescaled
+        for (int i = 0; i < n; ++i) {
+          if (i + 1 < n) {                             // S(i) is in the threads' registers
+            mbar_wait(&s_free, i & 1, a.err, 0x7310);
+            issue_s(i + 1);
+          }
+          mbar_wait(&p_full, i & 1, a.err, 0x7305);    // P(i) is written, O is rescaled
           mbar_wait(&v_full[i % VB], (i / VB) & 1, a.err, 0x7306);
           tc_fence_after();
           // 16 keys per product: eight columns of P in tensor memory, or 32 bytes (2 units) along its rows in shared memory, and two
@@ -378,17 +517,15 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           if (TERMS == 1) {
 #pragma unroll
             for (int k = 0; k < ST_KEYS / 16; ++k)
-              umma_bf16_ts(tmem_o, tmem_s + (i & 1) * ST_KEYS + k * 8, v + k * 128, idesc_o, (i || k) ? 1u : 0u);
+              umma_bf16_ts_warp(tmem_o, tmem_p + (i & 1) * (ST_KEYS / 2) + k * 8, v + k * 128, idesc_o, (i || k) ? 1u : 0u);
           } else {
 #pragma unroll
-            for (int t = 0; t < TERMS; ++t) umma_bf16_x4s(tmem_o, dp[t], v, idesc_o, (i || t) ? 1u : 0u, 2, 128);
+            for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+              for (int k = 0; k < ST_KEYS / 16; ++k) umma_bf16_warp(tmem_o, dp[t] + k * 2, v + k * 128, idesc_o, (i || t || k) ? 1u : 0u);
           }
-          umma_commit(&v_empty[i % VB]);
-          umma_commit(&pv_done);
-          if (i + 2 < n_blocks) {                    // into the buffer that S(i) has left, and P(i), which took its place
-            if (TERMS == 1) mbar_wait(&pv_done, i & 1, a.err, 0x7310);
-            issue_s(i + 2);
-          }
+          umma_commit_warp(&v_empty[i % VB]);
+          umma_commit_warp(&pv_done);
         }
       }
     } else {
@@ -402,83 +539,27 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int position = a.positions[t];
       grid_dep_wait();
       grid_dep_launch();
-      {
-        // the warp's 32 queries, D / 8 lanes a row and sixteen loads of a lane under way; rows of nobody and columns beyond the
-        // head are zeros
-        constexpr int PER = D / 8, AT_ONCE = 32 / PER, LOADS = 32 / AT_ONCE < 16 ? 32 / AT_ONCE : 16;      // (PER is 8, 16 or 32)
-        const int c = lane % PER;
-        const long long place = (long long)t * a.q_stride + (long long)h * a.D;
-#pragma unroll
-        for (int i0 = 0; i0 < 32; i0 += LOADS * AT_ONCE) {
-          uint4 v[LOADS];
-#pragma unroll
-          for (int u = 0; u < LOADS; ++u) {
-            const int i = i0 + u * AT_ONCE + lane / PER;
-            const long long from = __shfl_sync(0xffffffffu, place, i);
-            v[u] = q * 32 + i < pairs && c * 8 < a.D ? *(const uint4*)((const bf16*)a.q + from + c * 8) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int u = 0; u < LOADS; ++u) {
-            const int row = q * 32 + i0 + u * AT_ONCE + lane / PER;
-            *(uint4*)(Qs + (c / 8) * Q_SLAB + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = v[u];
-          }
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full);
-      }
+      gather_queries<D>(a, Qs, q, lane, pairs, t, h);
+      if (lane == 0) mbar_arrive(&q_full);
       const int limit = live ? min(j_hi, position + 1) : j_hi;                  // the first key that this row does not see
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n_blocks; ++i) {
         const int j0 = j_lo + i * ST_KEYS;
-        mbar_wait(&s_full[i & 1], (i >> 1) & 1, a.err, 0x7307);
+        mbar_wait(&s_full, i & 1, a.err, 0x7307);
         float s[ST_KEYS];
         float alpha = 1.f;
         if (some) {
           tc_fence_after();
-          tmem_ld32_nowait(tmem_s + (i & 1) * ST_KEYS + lane_off, s);
-          tmem_ld32_nowait(tmem_s + (i & 1) * ST_KEYS + lane_off + 32, s + 32);
+          tmem_ld32_nowait(tmem_s + lane_off, s);
+          tmem_ld32_nowait(tmem_s + lane_off + 32, s + 32);
           tmem_ld_wait();
           tmem_ld_fence<64>(s);
-          if (map.cap1 > 0.f) {
-#pragma unroll
-            for (int c = 0; c < ST_KEYS; ++c) s[c] = capped_log2(map, s[c]);
-          }
-          if (j0 + ST_KEYS > limit) {
-#pragma unroll
-            for (int c = 0; c < ST_KEYS; ++c)
-              if (j0 + c >= limit) s[c] = -INFINITY;
-          }
-          float mx4[4] = {s[0], s[1], s[2], s[3]};                       // four chains, three numbers a step
-#pragma unroll
-          for (int c = 4; c < ST_KEYS - 4; c += 8) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(fmaxf(s[c + u], s[c + 4 + u]), mx4[u]);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], s[ST_KEYS - 4 + u]);
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          // the exponent's reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost
-          // bfloat16 and the float32 sums nothing), so that O is rescaled once in a long while
-          if (mx > m && (m == -INFINITY || (mx - m) * map.in > 8.f)) {
-            alpha = m == -INFINITY ? 0.f : ex2_fast((m - mx) * map.in);
-            m = mx;
-          }
-          const float ms = m == -INFINITY ? 0.f : m * map.in;
-          // two elements an instruction where there is one
-          float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float2 in2 = make_float2(map.in, map.in), ms2 = make_float2(-ms, -ms);
-#pragma unroll
-          for (int c = 0; c < ST_KEYS; c += 4) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float2 e = fma2(make_float2(s[c + 2 * u], s[c + 2 * u + 1]), in2, ms2);
-              s[c + 2 * u] = ex2_fast(e.x);
-              s[c + 2 * u + 1] = ex2_fast(e.y);
-              sum2[u] = add2(sum2[u], make_float2(s[c + 2 * u], s[c + 2 * u + 1]));
-            }
-          }
-          l = l * alpha + ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y));
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free);
+        if (some) {
+          l = softmax_step(map, s, j0, limit, m, alpha, l);
         }
         // O += P(i-1) V(i-1) must have ended before O is rescaled and P is overwritten (a warp without pairs waits too: its
         // arrival is one for this block)
@@ -487,25 +568,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           tc_fence_after();
         }
         if (some) {
-          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32(tmem_o + lane_off + c * 32, o);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] *= alpha;
-              tmem_st32(tmem_o + lane_off + c * 32, o);
-            }
-          }
+          if (i > 0) rescale<D>(tmem_o + lane_off, alpha);
           if (TERMS == 1) {
-            // the row's weights over its scores, two in a column
-            uint32_t w[ST_KEYS / 2];
-#pragma unroll
-            for (int c = 0; c < ST_KEYS / 2; ++c) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(s[2 * c], s[2 * c + 1]);
-              w[c] = *(const uint32_t*)&b;
-            }
-            tmem_st32_u32(tmem_s + (i & 1) * ST_KEYS + lane_off, w);
+            put_weights(tmem_p + (i & 1) * (ST_KEYS / 2) + lane_off, s);
           } else {
             uint8_t* prow = Ps + (size_t)p * 128;
 #pragma unroll
@@ -541,36 +606,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         mbar_wait(&pv_done, (n_blocks - 1) & 1, a.err, 0x7308);
         tc_fence_after();
       }
-      if (some) {
-        const size_t at = ((size_t)r * a.Hq + h) * a.slots + a.slot0 + split;
-        if (live) {
-          // (m is in the units of the raw or the capped scores: map.in takes it to base 2)
-          a.part_ml[at * 2] = m == -INFINITY ? -1e30f : m * map.in * 0.6931471805599453f;
-          a.part_ml[at * 2 + 1] = l;
-        }
-        // A row of O goes through shared memory (all of it is free now; rows a chunk of 16 bytes further apart than they are long, so
-        // that a warp's threads write to different banks) and leaves in one copy: whole lines instead of 16 bytes in each of 32.
-        uint8_t* row = smem + (size_t)p * (D * 4 + 16);
-        constexpr int W = D < 128 ? D : 128;                  // columns whose loads are under way at once
-#pragma unroll
-        for (int c0 = 0; c0 < D; c0 += W) {
-          float o[W];
-          if (n_blocks > 0) {
-#pragma unroll
-            for (int c = 0; c < W; c += 32) tmem_ld32_nowait(tmem_o + lane_off + c0 + c, o + c);
-            tmem_ld_wait();
-            tmem_ld_fence<W>(o);
-          } else {
-#pragma unroll
-            for (int j = 0; j < W; ++j) o[j] = 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < W; j += 4) *(float4*)(row + (c0 + j) * 4) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-        }
-        fence_async_smem();
-        if (live) bulk_store(a.part_o + at * a.D, row, (uint32_t)a.D * 4);
-        bulk_store_wait();
-      }
+      if (some)
+        leave_part<D>(a, smem + (size_t)p * (D * 4 + 16), tmem_o + lane_off, n_blocks > 0, live, ((size_t)r * a.Hq + h) * a.slots + a.slot0 + split, m, l, map.in);
     }
   }
   tc_fence_before();
@@ -698,10 +735,7 @@ bool tc_takes(int cache_dt, int D, int page) {
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-}  // namespace
-
 // Tiles of pairs that M rows in `groups` groups make at most.
-namespace {
 long long shared_tiles(int M, int groups, int Hq, int Hkv, int per_tile) {
   return ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;
 }
@@ -709,21 +743,23 @@ long long shared_tiles(int M, int groups, int Hq, int Hkv, int per_tile) {
 
 // Splits of the shared keys for M rows in `groups` groups whose longest prefix has `longest` positions: as many blocks as live on
 // the GPU at once (two a multiprocessor, one of the larger forms), 256 keys a split or more.  (64 rows of 28 heads on 4 behind 8,192
-// positions, 18 splits: 44 us; 9: 48, 32: 51.  128 behind 16,384, 10: 67; 6: 81, 18: 77.)
+// positions, 16 splits: 38.4 us; 9: 44.0, 32: 46.3.  128 behind 16,384, 10: 61; 6: 74, 18: 70.)
 NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int float_weights, int longest) {
   if (M <= 0 || groups <= 0 || longest <= 0 || Hkv <= 0) return 0;
   const bool tc = tc_takes(cache_dt, D, page);
   const int each = tc ? (D <= 128 && !float_weights ? 2 : 1) : 4, least = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
   const long long tiles = shared_tiles(M, groups, Hq, Hkv, tc ? ST_PAIRS : SP_PAIRS);
   const long long want = (long long)each * num_multiprocessors() / (tiles * Hkv), most = (longest + least - 1) / least;
-  const long long n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+  long long n = want < most ? want : most;
+  n = n < 1 ? 1 : n > 32 ? 32 : n;
+  const long long block = tc ? ST_KEYS : SP_KEYS, share = ((longest + n - 1) / n + block - 1) / block * block;
+  return (int)((longest + share - 1) / share);                       // (no split without keys)
 }
 
 // Splits of the rows' own keys, of which no row has more than `most`, beside shared_splits of the above: 128 keys a split or more.
 // Where the shared part leaves room, they run beside it, one block (of 76 KB) on its multiprocessors and three on the others, and a
-// second wave would come after it (eight rows of 16 heads behind 2,048: 13.9 us in one wave, 17.5 in two); where it fills the
-// GPU they come after it anyway (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own: one split 43.8, four 41.7).
+// second wave would come after it (eight rows of 16 heads behind 2,048: 13.6 us in one wave, 16.4 in two); where it fills the
+// GPU they come after it anyway (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own: one split 40.1, four 38.4).
 NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int shared_splits,
                                           int most) {
   if (R <= 0 || Hkv <= 0 || most <= 0) return 1;
@@ -738,16 +774,16 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
 
 // Whether `repeated` positions that need not be read again are worth a kernel more and a join (1) or not (0), in bytes of keys and
 // values.  Tensor-core form: 16 MB, some three microseconds of reading, and 32 KB for every row and kv head, whose parts are joined
-// (shared and not: four rows of 16 kv heads behind 700 positions, 17 MB, 10.3 and 9.5 us, behind 1,500, 37 MB, 11.0 and 13.2; eight
-// of 4 behind 1,000, 14 MB, 12.2 and 11.5, behind 1,500, 22 MB, 12.2 and 14.3; 64 of 16 behind 64, 33 MB, 21.8 and 20.1, behind 128,
-// 66 MB, 23.1 and 25.4).  Plain form: 256 KB for every row and kv head, since the kernel without groups is slow at few rows of these
-// types (four float32 rows of 8 heads on 2 behind 500, 3 MB, 16.2 and 21.6; 32 of 28 on 4 behind 128, 16 MB, 30.0 and 26.0, behind
-// 256, 33 MB, 34.8 and 45.0), and half a tile of pairs a group (four rows of 16 on 16 behind 1,000, 49 MB, 21.1 and 16.3).
+// (shared and not: four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37 MB, 10.3 and 14.0; eight
+// of 4 behind 1,000, 14 MB, 11.5 and 11.1, behind 1,500, 22 MB, 11.6 and 14.3; 64 of 16 behind 64, 33 MB, 19.0 and 18.7, behind 128,
+// 66 MB, 19.9 and 23.8).  Plain form: 192 KB for every row and kv head, since the kernel without groups is slow at few rows of these
+// types (four float32 rows of 8 heads on 2 behind 500, 3 MB, 15.6 and 21.5; 32 of 28 on 4 behind 128, 16 MB, 30.1 and 25.9, behind
+// 256, 33 MB, 34.8 and 44.6), and half a tile of pairs a group (four rows of 16 on 16 behind 1,000, 49 MB, 21.1 and 15.1).
 NV_API int nv_attention_shared_pays(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, long long repeated) {
   if (groups <= 0 || Hkv <= 0) return 0;
   const long long saved = repeated * Hkv * D * 2 * (cache_dt == NV_DT_BF16 ? 2 : 4), parts = (long long)R * Hkv;
   if (tc_takes(cache_dt, D, page)) return saved >= (16LL << 20) + 32768 * parts;
-  return saved >= 262144 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
+  return saved >= 196608 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
 }
 
 NV_API int nv_attention_shared_usable(int D, int page) { return D >= 8 && D <= 256 && D % 8 == 0 && page >= 16 && page % 16 == 0; }
@@ -771,17 +807,16 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   if (!scratch || ((uintptr_t)scratch & 15)) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
   const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc);
-  const int per_tile = tc ? ST_PAIRS : SP_PAIRS;
-  const long long tiles = shared_tiles(M, groups, Hq, Hkv, per_tile);
   if (shared_splits > 0 && groups > 0) {
+    const int tiles = (int)shared_tiles(M, groups, Hq, Hkv, tc ? ST_PAIRS : SP_PAIRS);
     SharedArgs a;
     a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;
     a.members = members; a.cu = cu; a.len = len; a.lead = lead; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
     a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
     a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
     a.slots = slots; a.slot0 = own_splits; a.split_keys = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
-    const int rc = tc ? ((float_weights || has_sink) ? launch_tc_d<3>(a, (int)tiles, stream) : launch_tc_d<1>(a, (int)tiles, stream))
-                   : cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, (int)tiles, stream) : launch_plain<float>(a, (int)tiles, stream);
+    const int rc = !tc ? (cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, tiles, stream) : launch_plain<float>(a, tiles, stream))
+                   : (float_weights || has_sink) ? launch_tc_d<3>(a, tiles, stream) : launch_tc_d<1>(a, tiles, stream);
     if (rc) return rc;
   }
   const int rc = nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
