@@ -8,13 +8,13 @@
 //
 // so the shared part can be worked out for all rows of the group at once, its keys and values read once instead of once a
 // row: per kv head it is a matrix product of the (row, query head) pairs that read it.  Three launches: the shared parts (here),
-// every row's own keys, from the page on that holds position len[g] (the split-key kernel of attention_decode.cu), and their join
+// every row's own keys, from the page on that holds position len[g] (here, or the split-key kernel of attention_decode.cu), and their join
 // (here).  A row that belongs to no group has no shared part; of a group's keys a row sees those up to its own position.
 //
-// What bounds it (bfloat16, heads of 128): 64 rows of 28 heads on 4 behind 8,192 positions, 16 to 512 of their own, take 38.4 us
-// (each row by itself: 221), 18 of it the shared part, 13 the rows' own keys, 5 to 7 the join of up to 20 parts.  128 rows behind
-// 16,384 take 61 (673), 40 of it the shared part: 64 keys of two blocks of 128 pairs in 1.1 us a multiprocessor, where its
-// exponentials alone take 0.6, the products 0.8 (those of different shapes do not overlap), and the 64 KB of keys and values from L2 0.9.
+// What bounds it (bfloat16, heads of 128): 64 rows of 28 heads on 4 behind 8,192 positions, 16 to 512 of their own, take 34 us (each
+// row by itself: 221), 18 of it the shared part, 10 the rows' own keys, 5 the join of up to 18 parts.  128 rows behind 16,384 take 51
+// (673), 40 of it the shared part: 64 keys of two blocks of 128 pairs in 1.1 us a multiprocessor, where its exponentials alone take
+// 0.6, the products 0.8 (those of different shapes do not overlap), and the 64 KB of keys and values from L2 0.9.
 #include "tcgen05.cuh"
 
 int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
@@ -615,33 +615,233 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem_base, st_tmem_cols<D>());
 }
 
-// The parts of one (row, head): its own keys' splits, then the shared ones'.  Every warp works out what the parts weigh, takes every
-// fourth of them, four elements a lane and all loads under way, and the four sums are added in their order.
+// Every row's own keys, from the page on that the prefix ends in, for bfloat16, heads of 64, 96 or 128 elements: eight query heads of
+// a kv head and one split of the keys a block, whose four warps take 16 keys in turn.  A row has few keys of its own, so that a block's
+// time is its latency; there is no ring of pages, no copy into shared memory and no order among the warps until their sums are joined: keys
+// and values come as 16-byte loads to where the products want them.  S^T = K Q^T and O^T = V^T P^T (mma.sync, 16 keys or dimensions by 8
+// heads): a product does not care which of the head's elements it calls its k-th, so a lane's piece of eight elements is two or four of
+// its places in four products of S^T, and row g of product j of O^T is element 8 g + j of the first 64, row g + 8 the same of the others.
+constexpr int OW_WARPS = 4, OW_HEADS = 8;
+
+__device__ __forceinline__ void mma_16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {        // 8 x 8 elements over a warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int D, int TERMS>
+__global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a, const int* __restrict__ first, int own_splits, ScoreMap map,
+                                                                int beside) {
+  constexpr int KC = D / 32, MORE = (D - 64) / 16;                   // 16-byte pieces of a key a lane; registers of a value behind the first 64
+  __shared__ float o_s[OW_WARPS][OW_HEADS][D + 4], m_s[OW_WARPS][OW_HEADS], l_s[OW_WARPS][OW_HEADS];
+  const int r = blockIdx.x, t = a.rows ? a.rows[r] : r, G = a.Hq / a.Hkv, parts = (G + OW_HEADS - 1) / OW_HEADS;
+  const int kvh = blockIdx.y / parts, h0 = kvh * G + blockIdx.y % parts * OW_HEADS, heads = min(OW_HEADS, (kvh + 1) * G - h0), split = blockIdx.z;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4;
+  const int n = a.positions[t] + 1, lo = first[r] / a.page * a.page;
+  const int units = max(0, (n - lo + 15) / 16), per = (units + own_splits - 1) / own_splits;
+  const int u0 = split * per, u1 = min(units, u0 + per);
+  const int* bt = a.block_table + (long long)a.row_entry[t] * a.max_blocks;
+  // (beside the shared part, which has waited for what wrote the queries and the newest page, and whose results are not read here)
+  if (!beside) grid_dep_wait();
+  grid_dep_launch();
+  uint4 q[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c)
+    q[c] = g < heads ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8) : make_uint4(0, 0, 0, 0);
+
+  float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  uint4 ka[KC], kb[KC], v[4];                                        // keys g and g + 8; values of keys 2 tq, 2 tq + 1, and 8 behind
+  uint32_t w[4][MORE > 0 ? MORE : 1];
+  int pages = -2;                                                    // lane i: where this warp's unit i of 32 lies
+  auto place_of = [&](int i) {                                       // the unit's first key, in rows of the cache; -1: not there
+    const int u = u0 + warp + i * OW_WARPS;
+    if (i % 32 == 0) {
+      const int mine = u + lane * OW_WARPS;
+      pages = mine < u1 ? bt[(lo + mine * 16) / a.page] : -2;
+    }
+    const int blk = __shfl_sync(0xffffffffu, pages, i % 32);
+    if (blk == -2) return -1LL;
+    if (blk < 0 || blk >= a.num_pages) {
+      if (lane == 0 && a.err) atomicExch(a.err, 1 + t);
+      return -1LL;
+    }
+    return ((long long)blk * a.Hkv + kvh) * a.page + (lo + u * 16) % a.page;
+  };
+  auto fetch_keys = [&](long long at) {
+    if (at < 0) return;
+    const bf16* x = (const bf16*)a.kc + (at + g) * D + tq * 8;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      ka[c] = __ldg((const uint4*)(x + c * 32));
+      kb[c] = __ldg((const uint4*)(x + 8 * D + c * 32));
+    }
+  };
+  auto fetch_values = [&](long long at, int left) {                  // zeros behind the row's position
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 2 * tq + (i & 1) + (i >> 1) * 8;
+      const bf16* x = (const bf16*)a.vc + (at + key) * D;
+      const bool there = at >= 0 && key < left;
+      v[i] = there ? __ldg((const uint4*)(x + g * 8)) : make_uint4(0, 0, 0, 0);
+      if (MORE == 4) {
+        const uint4 y = there ? __ldg((const uint4*)(x + 64 + g * 8)) : make_uint4(0, 0, 0, 0);
+        w[i][0] = y.x; w[i][MORE > 1 ? 1 : 0] = y.y; w[i][MORE > 2 ? 2 : 0] = y.z; w[i][MORE > 3 ? 3 : 0] = y.w;
+      }
+      if (MORE == 2) {
+        const uint2 y = there ? __ldg((const uint2*)(x + 64 + g * 4)) : make_uint2(0, 0);
+        w[i][0] = y.x; w[i][MORE > 1 ? 1 : 0] = y.y;
+      }
+    }
+  };
+  const int rounds = u0 + warp < u1 ? (u1 - u0 - warp + OW_WARPS - 1) / OW_WARPS : 0;
+  long long at = rounds > 0 ? place_of(0) : -1;
+  fetch_keys(at);
+  fetch_values(at, n - lo - (u0 + warp) * 16);
+  for (int i = 0; i < rounds; ++i) {
+    const int left = n - lo - (u0 + warp + i * OW_WARPS) * 16;       // keys from the unit's first on
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      mma_16x8(s, ka[c].x, kb[c].x, ka[c].y, kb[c].y, q[c].x, q[c].y);
+      mma_16x8(s, ka[c].z, kb[c].z, ka[c].w, kb[c].w, q[c].z, q[c].w);
+    }
+    const bool here = at >= 0;
+    at = i + 1 < rounds ? place_of(i + 1) : -1;
+    fetch_keys(at);
+    // s: keys g (heads 2 tq, 2 tq + 1) and g + 8, in base-2 units from here on
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      s[x] = map.cap1 > 0.f ? capped_log2(map, s[x]) : s[x] * map.in;
+      if (!here || g + (x >> 1) * 8 >= left) s[x] = -INFINITY;
+    }
+    float alpha[2], ref[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float mx = fmaxf(s[x], s[x + 2]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      mx = fmaxf(mx, m[x]);
+      ref[x] = mx == -INFINITY ? 0.f : mx;
+      alpha[x] = ex2_fast(m[x] - ref[x]);
+      m[x] = mx;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) s[x] = ex2_fast(s[x] - ref[x & 1]);
+    l[0] = l[0] * alpha[0] + (s[0] + s[2]);
+    l[1] = l[1] * alpha[1] + (s[1] + s[3]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o[j][0] *= alpha[0]; o[j][1] *= alpha[1]; o[j][2] *= alpha[0]; o[j][3] *= alpha[1];
+    }
+    uint32_t b[TERMS][2];                                            // the weights: rounded once, or as three terms with all their bits
+#pragma unroll
+    for (int x = 0; x < TERMS; ++x) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(s[2 * k], s[2 * k + 1]);
+        b[x][k] = transposed(*(const uint32_t*)&p);
+        if (x + 1 < TERMS) {
+          const float2 f = __bfloat1622float2(p);
+          s[2 * k] -= f.x;
+          s[2 * k + 1] -= f.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t sel = j % 2 ? 0x7632 : 0x5410;
+      auto word = [&](const uint4& x, int k) { return k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w; };
+      const uint32_t a0 = __byte_perm(word(v[0], j / 2), word(v[1], j / 2), sel), a2 = __byte_perm(word(v[2], j / 2), word(v[3], j / 2), sel);
+      uint32_t a1 = 0, a3 = 0;
+      if (j / 2 < MORE) {
+        a1 = __byte_perm(w[0][j / 2 < MORE ? j / 2 : 0], w[1][j / 2 < MORE ? j / 2 : 0], sel);
+        a3 = __byte_perm(w[2][j / 2 < MORE ? j / 2 : 0], w[3][j / 2 < MORE ? j / 2 : 0], sel);
+      }
+#pragma unroll
+      for (int x = 0; x < TERMS; ++x) mma_16x8(o[j], a0, a1, a2, a3, b[x][0], b[x][1]);
+    }
+    fetch_values(at, left - 16 * OW_WARPS);
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
+    if (g == 0) {
+      m_s[warp][2 * tq + x] = m[x];
+      l_s[warp][2 * tq + x] = l[x];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o_s[warp][2 * tq + x][g * 8 + j] = o[j][x];
+      if (j / 2 < MORE) o_s[warp][2 * tq + x][64 + g * (MORE * 2) + j] = o[j][2 + x];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (D / 4); i += OW_WARPS * 32) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float mm = m_s[0][h];
+#pragma unroll
+    for (int x = 1; x < OW_WARPS; ++x) mm = fmaxf(mm, m_s[x][h]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < OW_WARPS; ++x) {
+      const float c = ex2_fast(m_s[x][h] - ref);
+      const float4 y = *(const float4*)&o_s[x][h][d];
+      ll = fmaf(l_s[x][h], c, ll);
+      sum.x = fmaf(y.x, c, sum.x); sum.y = fmaf(y.y, c, sum.y); sum.z = fmaf(y.z, c, sum.z); sum.w = fmaf(y.w, c, sum.w);
+    }
+    const size_t at_p = ((size_t)r * a.Hq + h0 + h) * a.slots + split;
+    *(float4*)(a.part_o + at_p * D + d) = sum;
+    if (d == 0) {
+      a.part_ml[at_p * 2] = mm == -INFINITY ? -1e30f : mm * 0.6931471805599453f;
+      a.part_ml[at_p * 2 + 1] = ll;
+    }
+  }
+  if (beside) grid_dep_wait();
+}
+
+// The parts of one (row, head): its own keys' splits, then the shared ones'.  W warps of a block take it, each every W-th part, eight
+// loads of a lane under way, and add their sums in their order.  WIDE: heads of more than 128 elements.
 constexpr int MAX_PARTS = 64, JOIN_WARPS = 4;
 
+template <int W, bool WIDE>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                                       const int* __restrict__ rows, const int* __restrict__ group,
-                                                                      void* out, int out_dt, int Hq, int D, int own, int slots,
-                                                                      int has_sink, float sink, HeadGate gate) {
-  __shared__ float4 sum_s[JOIN_WARPS][64];
-  const int r = blockIdx.x, h = blockIdx.y, t = rows ? rows[r] : r, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+                                                                      void* out, int out_dt, int pairs, int Hq, int D, int own, int slots,
+                                                                      int has_sink, float sink, HeadGate gate, int whole) {
+  constexpr int C = WIDE ? 2 : 1, AT_ONCE = 8;
+  __shared__ float4 sum_s[W > 1 ? JOIN_WARPS : 1][C * 32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = warp % W;
+  const int pair = min((int)blockIdx.x * (JOIN_WARPS / W) + warp / W, pairs - 1), r = pair / Hq, h = pair % Hq, t = rows ? rows[r] : r;
   const int n = group[r] >= 0 ? slots : own;
-  const size_t at = ((size_t)r * Hq + h) * slots;
+  const size_t at = (size_t)pair * slots;
   grid_dep_wait();
   grid_dep_launch();
   const float2 none = make_float2(-1e30f, 0.f);
   const float2* ml = (const float2*)part_ml + at;
   const float2 x = lane < n ? ml[lane] : none, y = lane + 32 < n ? ml[lane + 32] : none;
-  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  float4 o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   float wx = 0.f, wy = 0.f, by = 0.f;
   bool weighed = false;
-  for (int s0 = warp; s0 < n; s0 += 4 * JOIN_WARPS) {
-    float4 v[4][2];
+  for (int s0 = sub; s0 < n || !weighed; s0 += AT_ONCE * W) {
+    float4 v[AT_ONCE][C];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AT_ONCE; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int s = s0 + i * JOIN_WARPS, d = (c * 32 + lane) * 4;
+      for (int c = 0; c < C; ++c) {
+        const int s = s0 + i * W, d = (c * 32 + lane) * 4;
         v[i][c] = s < n && d < D ? __ldg((const float4*)(part_o + (at + s) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     if (!weighed) {                                  // (behind the loads, which need not wait for it)
@@ -650,33 +850,51 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const floa
       wy = expf(y.x - mm);
       float ll = warp_sum(x.y * wx + y.y * wy);
       if (has_sink) ll += expf(sink - mm);
-      by = ll > 0.f ? 1.f / ll : 0.f;
+      by = (ll > 0.f ? 1.f / ll : 0.f) * head_gate_of(gate, t, h);
       weighed = true;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = s0 + i * JOIN_WARPS;
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int s = s0 + i * W;
       const float w = __shfl_sync(0xffffffffu, s < 32 ? wx : wy, s % 32);
       if (s < n) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < C; ++c) {
           o[c].x = fmaf(v[i][c].x, w, o[c].x); o[c].y = fmaf(v[i][c].y, w, o[c].y);
           o[c].z = fmaf(v[i][c].z, w, o[c].z); o[c].w = fmaf(v[i][c].w, w, o[c].w);
         }
       }
     }
   }
+  if (W > 1) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) sum_s[warp][c * 32 + lane] = o[c];
-  by = __shfl_sync(0xffffffffu, by, 0);
-  __shared__ float by_s;
-  if (threadIdx.x == 0) by_s = by * head_gate_of(gate, t, h);        // (warp 0 has a part always: a row has own keys' splits)
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += JOIN_WARPS * 32) {
-    float v = 0.f;
+    for (int c = 0; c < C; ++c) sum_s[warp][c * 32 + lane] = o[c];
+    __syncthreads();
+    if (sub) return;
 #pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) v += ((const float*)&sum_s[w][0])[d];
-    st_dt(out, out_dt, ((size_t)t * Hq + h) * D + d, v * by_s);
+    for (int u = 1; u < W; ++u)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float4 p = sum_s[warp + u][c * 32 + lane];
+        o[c].x += p.x; o[c].y += p.y; o[c].z += p.z; o[c].w += p.w;
+      }
+  }
+  if ((int)blockIdx.x * (JOIN_WARPS / W) + warp / W >= pairs) return;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = (c * 32 + lane) * 4;
+    if (d >= D) continue;
+    const size_t to = ((size_t)t * Hq + h) * D + d;
+    const float z[4] = {o[c].x * by, o[c].y * by, o[c].z * by, o[c].w * by};
+    if (whole && out_dt == NV_DT_BF16) {
+      const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(z[0], z[1]), __floats2bfloat162_rn(z[2], z[3])};
+      *(uint2*)((bf16*)out + to) = *(const uint2*)b;
+    } else if (whole) {
+      *(float4*)((float*)out + to) = make_float4(z[0], z[1], z[2], z[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st_dt(out, out_dt, to + i, z[i]);
+    }
   }
 }
 
@@ -721,6 +939,14 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
   NV_RETURN_LAST();
 }
 
+template <int D, int TERMS>
+int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int beside, cudaStream_t s) {
+  const int parts = (a.Hq / a.Hkv + OW_HEADS - 1) / OW_HEADS;
+  NV_RETURN_IF(launch_dep(own_keys_kernel<D, TERMS>, dim3(R, a.Hkv * parts, own_splits), dim3(OW_WARPS * 32), 0, s, a, first, own_splits,
+                          score_map(a.scale, a.softcap), beside));
+  NV_RETURN_LAST();
+}
+
 template <int TERMS>
 int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
   return a.D <= 64 ? launch_tc<64, TERMS>(a, tiles, s) : a.D <= 128 ? launch_tc<128, TERMS>(a, tiles, s) : launch_tc<256, TERMS>(a, tiles, s);
@@ -733,11 +959,27 @@ constexpr int TC_SPLIT_KEYS = 256, PLAIN_SPLIT_KEYS = 64;
 bool tc_takes(int cache_dt, int D, int page) {
   return cache_dt == NV_DT_BF16 && D >= 32 && D % 16 == 0 && (page == 16 || page == 32 || page == 64);
 }
+bool own_takes(int D) { return D == 64 || D == 96 || D == 128; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Tiles of pairs that M rows in `groups` groups make at most.
 long long shared_tiles(int M, int groups, int Hq, int Hkv, int per_tile) {
   return ((long long)M * (Hq / Hkv) + per_tile - 1) / per_tile + groups - 1;
+}
+}  // namespace
+
+namespace {
+template <int W>
+int launch_join(const float* part_o, const float* part_ml, const int* rows, const int* group, void* out, int out_dt, int R, int Hq, int D,
+                int own, int slots, int has_sink, float sink, const HeadGate& gate, cudaStream_t s) {
+  const long long pairs = (long long)R * Hq, blocks = (pairs * W + JOIN_WARPS - 1) / JOIN_WARPS;
+  if (pairs > 0x7fffffffLL) return NV_ERR_BAD_SIZE;
+  const int whole = ((uintptr_t)out & 15) == 0;                      // (four elements in one store)
+  NV_RETURN_IF(D > 128 ? launch_dep(shared_join_kernel<W, true>, dim3((unsigned)blocks), dim3(JOIN_WARPS * 32), 0, s, part_o, part_ml, rows, group,
+                                    out, out_dt, (int)pairs, Hq, D, own, slots, has_sink, sink, gate, whole)
+                       : launch_dep(shared_join_kernel<W, false>, dim3((unsigned)blocks), dim3(JOIN_WARPS * 32), 0, s, part_o, part_ml, rows, group,
+                                    out, out_dt, (int)pairs, Hq, D, own, slots, has_sink, sink, gate, whole));
+  NV_RETURN_LAST();
 }
 }  // namespace
 
@@ -756,10 +998,11 @@ NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D,
   return (int)((longest + share - 1) / share);                       // (no split without keys)
 }
 
-// Splits of the rows' own keys, of which no row has more than `most`, beside shared_splits of the above: 128 keys a split or more.
-// Where the shared part leaves room, they run beside it, one block (of 76 KB) on its multiprocessors and three on the others, and a
-// second wave would come after it (eight rows of 16 heads behind 2,048: 13.6 us in one wave, 16.4 in two); where it fills the
-// GPU they come after it anyway (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own: one split 40.1, four 38.4).
+// Splits of the rows' own keys, of which no row has more than `most`, beside shared_splits of the above.  Where the shared part leaves
+// room, they run beside it, one block on its multiprocessors and three on the others, 128 keys a split or more, and a second wave
+// would come after it (eight rows of 16 heads behind 2,048: 11.8 us in one wave, 15.3 in two); where it fills the GPU they come
+// after it anyway, 256 keys a split or more unless 128 make one wave (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own:
+// one split 38.5, two 34.1, four 36.2; up to 1,000: 49.1, 39.0, 38.1; four of 16 behind 16,384, up to 200: 33.2, two 31.1).
 NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int shared_splits,
                                           int most) {
   if (R <= 0 || Hkv <= 0 || most <= 0) return 1;
@@ -768,7 +1011,8 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
   const long long shared = shared_splits <= 0 ? 0 : shared_tiles(M, groups, Hq, Hkv, tc_takes(cache_dt, D, page) ? ST_PAIRS : SP_PAIRS) * Hkv * shared_splits;
   const long long room = shared <= sms ? shared + 3 * (sms - shared) : 7 * sms;
   long long n = room / blocks;
-  if (n > (most + 127) / 128) n = (most + 127) / 128;
+  const long long least = shared <= sms || blocks * ((most + 127) / 128) <= 3 * sms ? 128 : 256;
+  if (n > (most + least - 1) / least) n = (most + least - 1) / least;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
 
@@ -807,26 +1051,32 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
   if (!scratch || ((uintptr_t)scratch & 15)) return NV_ERR_BAD_SIZE;
   const int slots = own_splits + shared_splits;
   const bool tc = tc_takes(cache_dt, D, page) && q_dt == NV_DT_BF16 && q_stride % 8 == 0 && aligned16(qkv) && aligned16(kc) && aligned16(vc);
-  if (shared_splits > 0 && groups > 0) {
+  const int exact = (float_weights || has_sink) ? 1 : 0, beside = shared_splits > 0 && groups > 0 ? 1 : 0;
+  SharedArgs a;
+  a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;
+  a.members = members; a.cu = cu; a.len = len; a.lead = lead; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
+  a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
+  a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
+  a.slots = slots; a.slot0 = own_splits; a.split_keys = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
+  if (beside) {
     const int tiles = (int)shared_tiles(M, groups, Hq, Hkv, tc ? ST_PAIRS : SP_PAIRS);
-    SharedArgs a;
-    a.q = qkv; a.kc = kc; a.vc = vc; a.block_table = block_table; a.row_entry = row_entry; a.positions = positions; a.rows = rows;
-    a.members = members; a.cu = cu; a.len = len; a.lead = lead; a.part_o = scratch; a.part_ml = scratch + (size_t)R * Hq * slots * D; a.err = err;
-    a.scale = scale; a.softcap = softcap > 0.f ? softcap : 0.f; a.q_dt = q_dt; a.q_stride = q_stride; a.max_blocks = max_blocks;
-    a.num_pages = num_pages; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.page = page; a.groups = groups; a.splits = shared_splits;
-    a.slots = slots; a.slot0 = own_splits; a.split_keys = tc ? TC_SPLIT_KEYS : PLAIN_SPLIT_KEYS;
     const int rc = !tc ? (cache_dt == NV_DT_BF16 ? launch_plain<bf16>(a, tiles, stream) : launch_plain<float>(a, tiles, stream))
-                   : (float_weights || has_sink) ? launch_tc_d<3>(a, tiles, stream) : launch_tc_d<1>(a, tiles, stream);
+                   : exact ? launch_tc_d<3>(a, tiles, stream) : launch_tc_d<1>(a, tiles, stream);
     if (rc) return rc;
   }
-  const int rc = nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
-                                          first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err,
-                                          (float_weights || has_sink) ? 1 : 0, softcap, shared_splits > 0 && groups > 0 ? 1 : 0, stream);
+  const int rc = tc && own_takes(D) ? (D == 64 ? (exact ? launch_own<64, 3>(a, first, R, own_splits, beside, stream) : launch_own<64, 1>(a, first, R, own_splits, beside, stream))
+                                       : D == 96 ? (exact ? launch_own<96, 3>(a, first, R, own_splits, beside, stream) : launch_own<96, 1>(a, first, R, own_splits, beside, stream))
+                                                 : (exact ? launch_own<128, 3>(a, first, R, own_splits, beside, stream) : launch_own<128, 1>(a, first, R, own_splits, beside, stream)))
+                 : nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
+                                            first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err, exact,
+                                            softcap, beside, stream);
   if (rc) return rc;
-  NV_RETURN_IF(launch_dep(shared_join_kernel, dim3(R, Hq), dim3(JOIN_WARPS * 32), 0, stream, (const float*)scratch,
-                          (const float*)scratch + (size_t)R * Hq * slots * D, rows, group, out, out_dt, Hq, D, own_splits, slots,
-                          has_sink, sink_score, HeadGate{gate, gate_ld}));
-  NV_RETURN_LAST();
+  const HeadGate gated{gate, gate_ld};
+  // A warp a pair where there are many with few parts, else two (128 rows of 28 heads, 11 parts: 51.4 and 52.2 us; 64 rows, 18: 35.1 and
+  // 34.0; 50 of 24, three terms, 9: 17.9 and 16.9).
+  return slots <= 12 && (long long)R * Hq >= 2048
+             ? launch_join<1>(a.part_o, a.part_ml, rows, group, out, out_dt, R, Hq, D, own_splits, slots, has_sink, sink_score, gated, stream)
+             : launch_join<2>(a.part_o, a.part_ml, rows, group, out, out_dt, R, Hq, D, own_splits, slots, has_sink, sink_score, gated, stream);
 }
 
 // The same with what a step's layers have in common in one array on the host (fewer arguments to convert a call): type of queries,
