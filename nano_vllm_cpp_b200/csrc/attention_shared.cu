@@ -615,12 +615,15 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem_base, st_tmem_cols<D>());
 }
 
-// Every row's own keys, from the page on that the prefix ends in, for bfloat16, heads of 64, 96 or 128 elements: eight query heads of
-// a kv head and one split of the keys a block, whose four warps take 16 keys in turn.  A row has few keys of its own, so that a block's
-// time is its latency; there is no ring of pages, no copy into shared memory and no order among the warps until their sums are joined: keys
-// and values come as 16-byte loads to where the products want them.  S^T = K Q^T and O^T = V^T P^T (mma.sync, 16 keys or dimensions by 8
-// heads): a product does not care which of the head's elements it calls its k-th, so a lane's piece of eight elements is two or four of
-// its places in four products of S^T, and row g of product j of O^T is element 8 g + j of the first 64, row g + 8 the same of the others.
+// Every row's own keys, from the page on that the prefix ends in, for bfloat16, heads of 64, 80, 96, 128 or 256 elements: eight query heads
+// of a kv head and one split of the keys a block, whose four warps take 16 keys in turn.  A row has few keys of its own, so that a
+// block's time is its latency; there is no ring of pages, no copy into shared memory and no order among the warps until their sums are
+// joined: keys and values come as 16-byte loads to where the products want them.  S^T = K Q^T and O^T = V^T P^T (mma.sync, 16 keys or
+// dimensions by 8 heads): a product does not care which of the head's elements it calls its k-th, so a lane's piece of eight elements is
+// four of its places in two products of S^T; row g of product 8 i + j of O^T is element 128 i + 8 g + j, row g + 8 the same of the 64
+// behind.  (Whole calls with this kernel and with the split-key kernel, whose ring has eight pages of 16 and two of 32 x 256: 64 rows of 28
+// heads on 4 behind 8,192 positions 33.9 and 38.4 us, 44 of 16 heads of 256 on 1 in pages of 32 27.8 and 92.9.  Four blocks a
+// multiprocessor, for which registers are spilled, 58.6 us where three take 55.7.)
 constexpr int OW_WARPS = 4, OW_HEADS = 8;
 
 __device__ __forceinline__ void mma_16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -634,9 +637,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {        // 8 x 8 ele
 }
 
 template <int D, int TERMS>
-__global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a, const int* __restrict__ first, int own_splits, ScoreMap map,
+__global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kernel(SharedArgs a, const int* __restrict__ first, int own_splits, ScoreMap map,
                                                                 int beside) {
-  constexpr int KC = D / 32, MORE = (D - 64) / 16;                   // 16-byte pieces of a key a lane; registers of a value behind the first 64
+  // 16-byte pieces of a key a lane; runs of 128 elements; registers of a value behind a run's first 64
+  constexpr int KC = (D + 31) / 32, RUNS = (D + 127) / 128, MORE = D < 128 ? (D - 64) / 16 : 4;
   __shared__ float o_s[OW_WARPS][OW_HEADS][D + 4], m_s[OW_WARPS][OW_HEADS], l_s[OW_WARPS][OW_HEADS];
   const int r = blockIdx.x, t = a.rows ? a.rows[r] : r, G = a.Hq / a.Hkv, parts = (G + OW_HEADS - 1) / OW_HEADS;
   const int kvh = blockIdx.y / parts, h0 = kvh * G + blockIdx.y % parts * OW_HEADS, heads = min(OW_HEADS, (kvh + 1) * G - h0), split = blockIdx.z;
@@ -651,13 +655,13 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
   uint4 q[KC];
 #pragma unroll
   for (int c = 0; c < KC; ++c)
-    q[c] = g < heads ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8) : make_uint4(0, 0, 0, 0);
+    q[c] = g < heads && c * 32 + tq * 8 < D ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8) : make_uint4(0, 0, 0, 0);
 
-  float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[8 * RUNS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  uint4 ka[KC], kb[KC], v[4];                                        // keys g and g + 8; values of keys 2 tq, 2 tq + 1, and 8 behind
-  uint32_t w[4][MORE > 0 ? MORE : 1];
+  for (int j = 0; j < 8 * RUNS; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  uint4 ka[KC], kb[KC], v[RUNS][4];                                  // keys g and g + 8; values of keys 2 tq, 2 tq + 1, and 8 behind
+  uint32_t w[RUNS][4][MORE > 0 ? MORE : 1];
   int pages = -2;                                                    // lane i: where this warp's unit i of 32 lies
   auto place_of = [&](int i) {                                       // the unit's first key, in rows of the cache; -1: not there
     const int u = u0 + warp + i * OW_WARPS;
@@ -678,8 +682,9 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
     const bf16* x = (const bf16*)a.kc + (at + g) * D + tq * 8;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      ka[c] = __ldg((const uint4*)(x + c * 32));
-      kb[c] = __ldg((const uint4*)(x + 8 * D + c * 32));
+      const bool in = c * 32 + tq * 8 < D;
+      ka[c] = in ? __ldg((const uint4*)(x + c * 32)) : make_uint4(0, 0, 0, 0);
+      kb[c] = in ? __ldg((const uint4*)(x + 8 * D + c * 32)) : make_uint4(0, 0, 0, 0);
     }
   };
   auto fetch_values = [&](long long at, int left) {                  // zeros behind the row's position
@@ -688,14 +693,18 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
       const int key = 2 * tq + (i & 1) + (i >> 1) * 8;
       const bf16* x = (const bf16*)a.vc + (at + key) * D;
       const bool there = at >= 0 && key < left;
-      v[i] = there ? __ldg((const uint4*)(x + g * 8)) : make_uint4(0, 0, 0, 0);
-      if (MORE == 4) {
-        const uint4 y = there ? __ldg((const uint4*)(x + 64 + g * 8)) : make_uint4(0, 0, 0, 0);
-        w[i][0] = y.x; w[i][MORE > 1 ? 1 : 0] = y.y; w[i][MORE > 2 ? 2 : 0] = y.z; w[i][MORE > 3 ? 3 : 0] = y.w;
-      }
-      if (MORE == 2) {
-        const uint2 y = there ? __ldg((const uint2*)(x + 64 + g * 4)) : make_uint2(0, 0);
-        w[i][0] = y.x; w[i][MORE > 1 ? 1 : 0] = y.y;
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u) {
+        v[u][i] = there ? __ldg((const uint4*)(x + u * 128 + g * 8)) : make_uint4(0, 0, 0, 0);
+        if (MORE == 4) {
+          const uint4 y = there ? __ldg((const uint4*)(x + u * 128 + 64 + g * 8)) : make_uint4(0, 0, 0, 0);
+          w[u][i][0] = y.x; w[u][i][MORE > 1 ? 1 : 0] = y.y; w[u][i][MORE > 2 ? 2 : 0] = y.z; w[u][i][MORE > 3 ? 3 : 0] = y.w;
+        }
+        if (MORE == 2) {
+          const uint2 y = there ? __ldg((const uint2*)(x + 64 + g * 4)) : make_uint2(0, 0);
+          w[u][i][0] = y.x; w[u][i][MORE > 1 ? 1 : 0] = y.y;
+        }
+        if (MORE == 1) w[u][i][0] = there ? __ldg((const uint32_t*)(x + 64 + g * 2)) : 0u;
       }
     }
   };
@@ -737,7 +746,7 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
     l[0] = l[0] * alpha[0] + (s[0] + s[2]);
     l[1] = l[1] * alpha[1] + (s[1] + s[3]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 8 * RUNS; ++j) {
       o[j][0] *= alpha[0]; o[j][1] *= alpha[1]; o[j][2] *= alpha[0]; o[j][3] *= alpha[1];
     }
     uint32_t b[TERMS][2];                                            // the weights: rounded once, or as three terms with all their bits
@@ -755,17 +764,15 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int jj = 0; jj < 8 * RUNS; ++jj) {
+      const int u = jj / 8, j = jj % 8, k = j / 2 < MORE ? j / 2 : 0;
       const uint32_t sel = j % 2 ? 0x7632 : 0x5410;
-      auto word = [&](const uint4& x, int k) { return k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w; };
-      const uint32_t a0 = __byte_perm(word(v[0], j / 2), word(v[1], j / 2), sel), a2 = __byte_perm(word(v[2], j / 2), word(v[3], j / 2), sel);
-      uint32_t a1 = 0, a3 = 0;
-      if (j / 2 < MORE) {
-        a1 = __byte_perm(w[0][j / 2 < MORE ? j / 2 : 0], w[1][j / 2 < MORE ? j / 2 : 0], sel);
-        a3 = __byte_perm(w[2][j / 2 < MORE ? j / 2 : 0], w[3][j / 2 < MORE ? j / 2 : 0], sel);
-      }
+      auto word = [&](const uint4& x) { return j / 2 == 0 ? x.x : j / 2 == 1 ? x.y : j / 2 == 2 ? x.z : x.w; };
+      const uint32_t a0 = __byte_perm(word(v[u][0]), word(v[u][1]), sel), a2 = __byte_perm(word(v[u][2]), word(v[u][3]), sel);
+      const uint32_t a1 = j / 2 < MORE ? __byte_perm(w[u][0][k], w[u][1][k], sel) : 0u;
+      const uint32_t a3 = j / 2 < MORE ? __byte_perm(w[u][2][k], w[u][3][k], sel) : 0u;
 #pragma unroll
-      for (int x = 0; x < TERMS; ++x) mma_16x8(o[j], a0, a1, a2, a3, b[x][0], b[x][1]);
+      for (int x = 0; x < TERMS; ++x) mma_16x8(o[jj], a0, a1, a2, a3, b[x][0], b[x][1]);
     }
     fetch_values(at, left - 16 * OW_WARPS);
   }
@@ -779,9 +786,10 @@ __global__ void __launch_bounds__(OW_WARPS * 32, 3) own_keys_kernel(SharedArgs a
       l_s[warp][2 * tq + x] = l[x];
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o_s[warp][2 * tq + x][g * 8 + j] = o[j][x];
-      if (j / 2 < MORE) o_s[warp][2 * tq + x][64 + g * (MORE * 2) + j] = o[j][2 + x];
+    for (int jj = 0; jj < 8 * RUNS; ++jj) {
+      const int u = jj / 8, j = jj % 8;
+      o_s[warp][2 * tq + x][u * 128 + g * 8 + j] = o[jj][x];
+      if (j / 2 < MORE) o_s[warp][2 * tq + x][u * 128 + 64 + g * (MORE * 2) + j] = o[jj][2 + x];
     }
   }
   __syncthreads();
@@ -948,6 +956,11 @@ int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int
 }
 
 template <int TERMS>
+int launch_own_d(const SharedArgs& a, const int* first, int R, int own_splits, int beside, cudaStream_t s) {
+  return a.D == 64 ? launch_own<64, TERMS>(a, first, R, own_splits, beside, s) : a.D == 80 ? launch_own<80, TERMS>(a, first, R, own_splits, beside, s)
+         : a.D == 96 ? launch_own<96, TERMS>(a, first, R, own_splits, beside, s) : a.D == 128 ? launch_own<128, TERMS>(a, first, R, own_splits, beside, s) : launch_own<256, TERMS>(a, first, R, own_splits, beside, s);
+}
+template <int TERMS>
 int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
   return a.D <= 64 ? launch_tc<64, TERMS>(a, tiles, s) : a.D <= 128 ? launch_tc<128, TERMS>(a, tiles, s) : launch_tc<256, TERMS>(a, tiles, s);
 }
@@ -959,7 +972,7 @@ constexpr int TC_SPLIT_KEYS = 256, PLAIN_SPLIT_KEYS = 64;
 bool tc_takes(int cache_dt, int D, int page) {
   return cache_dt == NV_DT_BF16 && D >= 32 && D % 16 == 0 && (page == 16 || page == 32 || page == 64);
 }
-bool own_takes(int D) { return D == 64 || D == 96 || D == 128; }
+bool own_takes(int D) { return D == 64 || D == 80 || D == 96 || D == 128 || D == 256; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Tiles of pairs that M rows in `groups` groups make at most.
@@ -1064,9 +1077,7 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
                    : exact ? launch_tc_d<3>(a, tiles, stream) : launch_tc_d<1>(a, tiles, stream);
     if (rc) return rc;
   }
-  const int rc = tc && own_takes(D) ? (D == 64 ? (exact ? launch_own<64, 3>(a, first, R, own_splits, beside, stream) : launch_own<64, 1>(a, first, R, own_splits, beside, stream))
-                                       : D == 96 ? (exact ? launch_own<96, 3>(a, first, R, own_splits, beside, stream) : launch_own<96, 1>(a, first, R, own_splits, beside, stream))
-                                                 : (exact ? launch_own<128, 3>(a, first, R, own_splits, beside, stream) : launch_own<128, 1>(a, first, R, own_splits, beside, stream)))
+  const int rc = tc && own_takes(D) ? (exact ? launch_own_d<3>(a, first, R, own_splits, beside, stream) : launch_own_d<1>(a, first, R, own_splits, beside, stream))
                  : nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
                                             first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err, exact,
                                             softcap, beside, stream);

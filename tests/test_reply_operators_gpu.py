@@ -440,6 +440,30 @@ def test_attention_with_infinities_and_nan_where_no_row_looks(dtype, D):
     assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
 
 
+@pytest.mark.parametrize("D,page", [(64, 16), (80, 32), (96, 64), (128, 32), (256, 16)])
+@pytest.mark.parametrize("sink", [None, 0.5])
+def test_attention_with_infinities_and_nan_behind_the_rows_ends(D, page, sink):
+    """The same for the other head and page sizes, with a row that ends where its prefix does and one without a prefix."""
+    lengths = [page * 2, page * 4 + 9, page * 3 + 1, 5, page * 2 + page // 2]
+    c = Case(6, 2, D, lengths, [([0, 1, 2, 4], page * 2)], page, extra=2)
+    want, weight, score = c.want(sink)
+    used = torch.zeros(c.k.shape[0], page, dtype=torch.bool, device=DEV)
+    for r, n in enumerate(lengths):
+        for j in range(n):
+            used[int(c.table[r, j // page]), j % page] = True
+    bad = torch.tensor([NAN, INF, -INF], device=DEV).to(c.k.dtype)
+    for x in (c.k, c.v):
+        x.copy_(torch.where(used[:, None, :, None], x, bad[torch.arange(page, device=DEV) % 3][None, None, :, None]))
+    got = c.run(stale=NAN, sink_score=sink)
+    assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+
+
+def test_attention_of_many_rows_with_long_keys_of_their_own():
+    """More keys in a split than a warp keeps places of."""
+    lengths = [2100 + r % 40 for r in range(520)]
+    Case(4, 2, 64, lengths, [([0, 1], 16)]).check()
+
+
 def test_attention_on_two_streams_at_once():
     c, d = (Case(16, 16, 128, [500 + r for r in range(8)], [(list(range(8)), 480)], seed=s) for s in (1, 2))
     alone = c.run(), d.run()
