@@ -194,17 +194,18 @@ class CacheManager:
 
     def shared_prefixes(self, rids: list, group: int) -> list:
         """Which of these requests begin with the same full pages of a group: (places in ``rids``, positions in common) per
-        set of two or more, in the order of their first members."""
+        set of two or more, in the order of their first members.  Requests that are not open share nothing."""
         S = len(rids)
-        ids = (ctypes.c_int64 * max(S, 1))(*[self._native(r) for r in rids])
+        ids = (ctypes.c_int64 * max(S, 1))(*[r if type(r) is int else self._ids.get(r, -1) for r in rids])
         group_of, pages = (ctypes.c_int * max(S, 1))(), (ctypes.c_int * max(S, 1))()
         n = host.lib().nvh_shared_prefixes(self._h, S, ids, group, group_of, pages)
         if n < 0:
             raise RuntimeError(host.last_error())
         out = [([], pages[k] * self.page_size) for k in range(n)]
-        for i in range(S if n else 0):
-            if group_of[i] >= 0:
-                out[group_of[i]][0].append(i)
+        if n:
+            for i, k in enumerate(group_of[:S]):
+                if k >= 0:
+                    out[k][0].append(i)
         return out
 
     # ------------------------------------------------------------------ pages

@@ -1030,16 +1030,18 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
 }
 
 // Whether `repeated` positions that need not be read again are worth a kernel more and a join (1) or not (0), in bytes of keys and
-// values.  Tensor-core form: 16 MB, some three microseconds of reading, and 32 KB for every row and kv head, whose parts are joined
-// (shared and not: four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37 MB, 10.3 and 14.0; eight
-// of 4 behind 1,000, 14 MB, 11.5 and 11.1, behind 1,500, 22 MB, 11.6 and 14.3; 64 of 16 behind 64, 33 MB, 19.0 and 18.7, behind 128,
-// 66 MB, 19.9 and 23.8).  Plain form: 192 KB for every row and kv head, since the kernel without groups is slow at few rows of these
+// values.  Tensor-core form: 32 MB, and 32 KB for every row and kv head, whose parts are joined.  (Calls behind one another would have
+// it pay from half of that on: shared and not, four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37
+// MB, 10.3 and 14.0; eight of 4 behind 1,500, 22 MB, 11.6 and 14.3; 64 of 16 behind 64, 33 MB, 19.0 and 18.7, behind 128, 66 MB, 19.9
+// and 23.8.  In a model's step the kernel without groups begins beside the one in front, and the step has to look for groups: 16 layers
+// with eight rows of 4 behind 2,048, 29 MB, take 2.28 ms either way, with 32 behind 1,024, 65 MB, 2.65 and 2.74.)  Plain form: 192 KB
+// for every row and kv head, since the kernel without groups is slow at few rows of these
 // types (four float32 rows of 8 heads on 2 behind 500, 3 MB, 15.6 and 21.5; 32 of 28 on 4 behind 128, 16 MB, 30.1 and 25.9, behind
 // 256, 33 MB, 34.8 and 44.6), and half a tile of pairs a group (four rows of 16 on 16 behind 1,000, 49 MB, 21.1 and 15.1).
 NV_API int nv_attention_shared_pays(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, long long repeated) {
   if (groups <= 0 || Hkv <= 0) return 0;
   const long long saved = repeated * Hkv * D * 2 * (cache_dt == NV_DT_BF16 ? 2 : 4), parts = (long long)R * Hkv;
-  if (tc_takes(cache_dt, D, page)) return saved >= (16LL << 20) + 32768 * parts;
+  if (tc_takes(cache_dt, D, page)) return saved >= (32LL << 20) + 32768 * parts;
   return saved >= 196608 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
 }
 

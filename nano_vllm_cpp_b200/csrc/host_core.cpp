@@ -392,8 +392,9 @@ class CacheManager {
     requests.emplace(child, std::move(rc));
     return OK;
   }
-  // Which of S open requests begin with the same pages of group g?  group_of[i]: the number of entry i's group, or -1; pages[k]: how
-  // many pages the entries of group k have in common, one at least.  Returns the number of groups, each of two entries or more.
+  // Which of S requests begin with the same pages of group g?  group_of[i]: the number of entry i's group, or -1 (also where it is not
+  // open); pages[k]: how many pages the entries of group k have in common, one at least.  Returns the number of groups, each of two
+  // entries or more.
   int shared_prefixes(int S, const int64_t* rids, int g, int* group_of, int* pages) const {
     std::unordered_map<int, int> by_page;                    // first page -> the first entry that has it
     std::vector<const std::vector<int>*> tables(S, nullptr);
@@ -401,7 +402,7 @@ class CacheManager {
     for (int i = 0; i < S; ++i) {
       group_of[i] = -1;
       auto it = requests.find(rids[i]);
-      if (it == requests.end()) return fail(ERR_STATE, "request is not open");
+      if (it == requests.end()) continue;
       tables[i] = &it->second.tables[g];
       const int full = it->second.num_tokens / page_size;    // (a page that is still being written is nobody else's)
       if (full < 1 || tables[i]->empty() || (*tables[i])[0] < 0) continue;
@@ -413,9 +414,11 @@ class CacheManager {
         n = std::min(n, common[l]);
         const int* a = tables[l]->data();
         const int* b = tables[i]->data();
-        int k = 0;
-        while (k < n && a[k] == b[k]) ++k;
-        n = k;
+        if (std::memcmp(a, b, n * sizeof(int)) != 0) {
+          int k = 0;
+          while (a[k] == b[k]) ++k;
+          n = k;
+        }
       }
       common[l] = n;
     }

@@ -495,14 +495,15 @@ class SharedPrefix:
         empty = max(0, room - len(groups))
         first, group, members, cu, lens = [0] * rows, [-1] * rows, [], [0], []
         for g, (own, n) in enumerate(groups):
+            n = int(n)
             _need(len(own) > 0 and n >= 0, "SharedPrefix: a group has a row at least and no negative prefix")
             for r in own:
-                _need(0 <= r < rows, f"SharedPrefix: row {r} is not among the {rows} rows")
-                _need(group[r] < 0, f"SharedPrefix: row {r} is named twice")
-                first[r], group[r] = int(n), g
-                members.append(int(r))
+                if not 0 <= r < rows or group[r] >= 0:
+                    raise KernelError(f"SharedPrefix: row {r} is not among the {rows} rows, or is named twice")
+                first[r], group[r] = n, g
+            members += own
             cu.append(len(members))
-            lens.append(int(n))
+            lens.append(n)
         leads = [int(own[0]) for own, _ in groups]
         none = [0] * empty
         return first + group + members + [0] * (rows - len(members)) + cu + [cu[-1]] * empty + lens + none + leads + none, len(members)

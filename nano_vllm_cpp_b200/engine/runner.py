@@ -419,30 +419,31 @@ class ModelRunner:
         have every row read its own keys anyway."""
         if self._whole_group is None:
             return None
-        single = [e for e in entries if len(e.tokens) == 1]
-        known = [i for i, e in enumerate(single) if self.manager.has(e.rid)]
-        if len(known) < 2:
+        single = [e.rid for e in entries if len(e.tokens) == 1]
+        groups = self.manager.shared_prefixes(single, self._whole_group)
+        if not groups:
             return None
-        groups = self.manager.shared_prefixes([single[i].rid for i in known], self._whole_group)
-        groups = [([known[i] for i in members], n) for members, n in groups]
         Hkv, D = self._whole_heads
-        repeated, members = sum(n * (len(m) - 1) for m, n in groups), sum(len(m) for m, _ in groups)
-        pays = ops.attention_sharing_pays(len(single), members, len(groups), Hkv, Hkv, D, self.page_size, torch.bfloat16, repeated)
+        (_, _, repeated), (members, rooms) = self._rounded_facts(groups, len(single))
+        pays = ops.attention_sharing_pays(len(single), members, rooms, Hkv, Hkv, D, self.page_size, torch.bfloat16, repeated)
         return (groups, len(single)) if pays else None
 
     @staticmethod
     def _rounded_facts(groups, rows: int):
-        """What a captured step's launches go by, so that steps of about the same prefixes share a capture: the powers of two
-        around the prefixes' lengths, and room for some more grouped rows and groups (up to a quarter)."""
+        """What a captured step's launches go by, so that steps of about the same prefixes share a capture: the prefixes' lengths
+        to three bits, the longest rounded up, the others down, and room for up to a quarter more grouped rows and groups."""
         longest, shortest, repeated = ops.SharedPrefix.facts(groups, rows)
-        floor = lambda n: 1 << (n.bit_length() - 1) if n > 0 else 0
 
-        def room(n):
-            step = 1 << max(0, (n - 1).bit_length() - 3)
-            return (n + step - 1) // step * step
+        def down(n):
+            bits = max(0, n.bit_length() - 3)
+            return n >> bits << bits
 
-        members = min(rows, room(sum(len(own) for own, _ in groups)))
-        return (1 << max(0, longest - 1).bit_length(), floor(shortest), floor(repeated)), (members, room(len(groups)))
+        def up(n):
+            bits = max(0, (n - 1).bit_length() - 3)
+            return -(-n >> bits) << bits
+
+        members = min(rows, up(sum(len(own) for own, _ in groups)))
+        return (up(longest), down(shortest), down(repeated)), (members, up(len(groups)))
 
     def _captured_form(self, entries: list, sampling, shared):
         """The step's ``_graph_key``, and its groups: none, where they would take one capture too many."""

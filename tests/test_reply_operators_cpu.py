@@ -79,12 +79,15 @@ def test_shared_prefix_refuses_arrays_and_room_that_do_not_fit():
 def test_steps_of_about_the_same_prefixes_share_a_capture():
     from nano_vllm_cpp_b200.engine.runner import ModelRunner
     rounded = lambda sizes, n, rows: ModelRunner._rounded_facts([([0] * s, n) for s in sizes], rows)
-    assert rounded([8], 2048, 8) == ((2048, 2048, 8192), (8, 1)) and rounded([8], 2049, 8) == ((4096, 2048, 8192), (8, 1))
-    assert rounded([3, 2], 100, 6) == ((128, 0, 256), (5, 2)) and rounded([33], 64, 64)[1] == (40, 1) and rounded([33], 64, 34)[1] == (34, 1)
+    assert rounded([8], 2048, 8) == ((2048, 2048, 14336), (8, 1)) and rounded([8], 2049, 8) == ((2560, 2048, 14336), (8, 1))
+    assert rounded([3, 2], 100, 6) == ((112, 0, 256), (5, 2)) and rounded([33], 64, 64)[1] == (40, 1) and rounded([33], 64, 34)[1] == (34, 1)
     for rows in range(2, 70):
         for k in range(2, rows + 1):
             members, groups = rounded([k] * 9, 16, 9 * rows)[1]
             assert 9 * k <= members <= min(9 * rows, 9 * k * 5 // 4 + 1) and groups == 10
+    for n in range(1, 3000):
+        longest, shortest, repeated = rounded([2], n, 2)[0]
+        assert n <= longest <= n * 5 // 4 + 1 and shortest == repeated and shortest <= n <= shortest * 5 // 4 + 1
 
 
 def test_sharing_is_a_matter_of_bytes_rows_and_heads():
