@@ -24,6 +24,7 @@ int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void
 
 namespace {
 
+// (Keys, values and parts are read past the first cache: kernels in front may write them while a kernel here has begun.)
 struct SharedArgs {
   const void* q;
   const void* kc;
@@ -83,14 +84,14 @@ struct Eight;                                    // eight elements as they lie i
 template <>
 struct Eight<float> {
   float4 a, b;
-  __device__ __forceinline__ void load(const float* p) { a = __ldg((const float4*)p); b = __ldg((const float4*)p + 1); }
+  __device__ __forceinline__ void load(const float* p) { a = __ldcg((const float4*)p); b = __ldcg((const float4*)p + 1); }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void put(float* to) const { *(float4*)to = a; *(float4*)(to + 4) = b; }
 };
 template <>
 struct Eight<bf16> {
   uint4 a;
-  __device__ __forceinline__ void load(const bf16* p) { a = __ldg((const uint4*)p); }
+  __device__ __forceinline__ void load(const bf16* p) { a = __ldcg((const uint4*)p); }
   __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void put(float* to) const {
     const __nv_bfloat162* h = (const __nv_bfloat162*)&a;
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_plain_kernel(SharedArgs a) 
       const int x = tid + c * SP_THREADS, key = x / (D / 8), at = x % (D / 8), j = j0 + key;
       part[c].zero();
       if (key < SP_KEYS && j < j_hi) {
-        const int blk = __ldg(bt + j / a.page);
+        const int blk = bt[j / a.page];
         if (blk >= 0 && blk < a.num_pages) part[c].load((const T*)cache + (((size_t)blk * a.Hkv + kvh) * a.page + j % a.page) * D + at * 8);
         else if (a.err) atomicExch(a.err, 1 + lead_t);
       }
@@ -683,8 +684,8 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       const bool in = c * 32 + tq * 8 < D;
-      ka[c] = in ? __ldg((const uint4*)(x + c * 32)) : make_uint4(0, 0, 0, 0);
-      kb[c] = in ? __ldg((const uint4*)(x + 8 * D + c * 32)) : make_uint4(0, 0, 0, 0);
+      ka[c] = in ? __ldcg((const uint4*)(x + c * 32)) : make_uint4(0, 0, 0, 0);
+      kb[c] = in ? __ldcg((const uint4*)(x + 8 * D + c * 32)) : make_uint4(0, 0, 0, 0);
     }
   };
   auto fetch_values = [&](long long at, int left) {                  // zeros behind the row's position
@@ -695,16 +696,16 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
       const bool there = at >= 0 && key < left;
 #pragma unroll
       for (int u = 0; u < RUNS; ++u) {
-        v[u][i] = there ? __ldg((const uint4*)(x + u * 128 + g * 8)) : make_uint4(0, 0, 0, 0);
+        v[u][i] = there ? __ldcg((const uint4*)(x + u * 128 + g * 8)) : make_uint4(0, 0, 0, 0);
         if (MORE == 4) {
-          const uint4 y = there ? __ldg((const uint4*)(x + u * 128 + 64 + g * 8)) : make_uint4(0, 0, 0, 0);
+          const uint4 y = there ? __ldcg((const uint4*)(x + u * 128 + 64 + g * 8)) : make_uint4(0, 0, 0, 0);
           w[u][i][0] = y.x; w[u][i][MORE > 1 ? 1 : 0] = y.y; w[u][i][MORE > 2 ? 2 : 0] = y.z; w[u][i][MORE > 3 ? 3 : 0] = y.w;
         }
         if (MORE == 2) {
-          const uint2 y = there ? __ldg((const uint2*)(x + 64 + g * 4)) : make_uint2(0, 0);
+          const uint2 y = there ? __ldcg((const uint2*)(x + 64 + g * 4)) : make_uint2(0, 0);
           w[u][i][0] = y.x; w[u][i][MORE > 1 ? 1 : 0] = y.y;
         }
-        if (MORE == 1) w[u][i][0] = there ? __ldg((const uint32_t*)(x + 64 + g * 2)) : 0u;
+        if (MORE == 1) w[u][i][0] = there ? __ldcg((const uint32_t*)(x + 64 + g * 2)) : 0u;
       }
     }
   };
@@ -850,7 +851,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const floa
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int s = s0 + i * W, d = (c * 32 + lane) * 4;
-        v[i][c] = s < n && d < D ? __ldg((const float4*)(part_o + (at + s) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i][c] = s < n && d < D ? __ldcg((const float4*)(part_o + (at + s) * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     if (!weighed) {                                  // (behind the loads, which need not wait for it)
       const float mm = warp_max(fmaxf(x.x, y.x));
@@ -1030,18 +1031,19 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
 }
 
 // Whether `repeated` positions that need not be read again are worth a kernel more and a join (1) or not (0), in bytes of keys and
-// values.  Tensor-core form: 32 MB, and 32 KB for every row and kv head, whose parts are joined.  (Calls behind one another would have
-// it pay from half of that on: shared and not, four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37
-// MB, 10.3 and 14.0; eight of 4 behind 1,500, 22 MB, 11.6 and 14.3; 64 of 16 behind 64, 33 MB, 19.0 and 18.7, behind 128, 66 MB, 19.9
-// and 23.8.  In a model's step the kernel without groups begins beside the one in front, and the step has to look for groups: 16 layers
-// with eight rows of 4 behind 2,048, 29 MB, take 2.28 ms either way, with 32 behind 1,024, 65 MB, 2.65 and 2.74.)  Plain form: 192 KB
+// values.  Tensor-core form: 24 MB, and 32 KB for every row and kv head, whose parts are joined.  (Calls behind one another would have
+// it pay a little sooner: shared and not, four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37 MB,
+// 10.3 and 14.0; eight of 4 behind 1,500, 22 MB, 11.6 and 14.3, behind 2,048, 29 MB, 11.7 and 15.1; 64 of 16 behind 64, 33 MB, 19.0 and
+// 18.7, behind 128, 66 MB, 19.9 and 23.8.  In a model's step the kernel without groups begins beside the one in front, and the step
+// has to look for groups: 16 layers with eight rows of 4 behind 1,500 take 2.26 and 2.27 ms without and with groups, behind 2,048 2.28
+// either way, 32 rows behind 1,024, 65 MB, 2.74 and 2.65.)  Plain form: 192 KB
 // for every row and kv head, since the kernel without groups is slow at few rows of these
 // types (four float32 rows of 8 heads on 2 behind 500, 3 MB, 15.6 and 21.5; 32 of 28 on 4 behind 128, 16 MB, 30.1 and 25.9, behind
 // 256, 33 MB, 34.8 and 44.6), and half a tile of pairs a group (four rows of 16 on 16 behind 1,000, 49 MB, 21.1 and 15.1).
 NV_API int nv_attention_shared_pays(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, long long repeated) {
   if (groups <= 0 || Hkv <= 0) return 0;
   const long long saved = repeated * Hkv * D * 2 * (cache_dt == NV_DT_BF16 ? 2 : 4), parts = (long long)R * Hkv;
-  if (tc_takes(cache_dt, D, page)) return saved >= (32LL << 20) + 32768 * parts;
+  if (tc_takes(cache_dt, D, page)) return saved >= (24LL << 20) + 32768 * parts;
   return saved >= 196608 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
 }
 
