@@ -627,6 +627,14 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 // multiprocessor, for which registers are spilled, 58.6 us where three take 55.7.)
 constexpr int OW_WARPS = 4, OW_HEADS = 8;
 
+// Where a row's keys are all in one part, its result needs no join (out: nullptr where it does).
+struct OwnResult {
+  void* out;
+  int out_dt, has_sink;
+  float sink;
+  HeadGate gate;
+};
+
 __device__ __forceinline__ void mma_16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -639,14 +647,14 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {        // 8 x 8 ele
 
 template <int D, int TERMS>
 __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kernel(SharedArgs a, const int* __restrict__ first, int own_splits, ScoreMap map,
-                                                                int beside) {
+                                                                int beside, OwnResult result) {
   // 16-byte pieces of a key a lane; runs of 128 elements; registers of a value behind a run's first 64
   constexpr int KC = (D + 31) / 32, RUNS = (D + 127) / 128, MORE = D < 128 ? (D - 64) / 16 : 4;
   __shared__ float o_s[OW_WARPS][OW_HEADS][D + 4], m_s[OW_WARPS][OW_HEADS], l_s[OW_WARPS][OW_HEADS];
   const int r = blockIdx.x, t = a.rows ? a.rows[r] : r, G = a.Hq / a.Hkv, parts = (G + OW_HEADS - 1) / OW_HEADS;
   const int kvh = blockIdx.y / parts, h0 = kvh * G + blockIdx.y % parts * OW_HEADS, heads = min(OW_HEADS, (kvh + 1) * G - h0), split = blockIdx.z;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, tq = lane % 4;
-  const int n = a.positions[t] + 1, lo = first[r] / a.page * a.page;
+  const int n = a.positions[t] + 1, lo = first ? first[r] / a.page * a.page : 0;
   const int units = max(0, (n - lo + 15) / 16), per = (units + own_splits - 1) / own_splits;
   const int u0 = split * per, u1 = min(units, u0 + per);
   const int* bt = a.block_table + (long long)a.row_entry[t] * a.max_blocks;
@@ -809,6 +817,14 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
       ll = fmaf(l_s[x][h], c, ll);
       sum.x = fmaf(y.x, c, sum.x); sum.y = fmaf(y.y, c, sum.y); sum.z = fmaf(y.z, c, sum.z); sum.w = fmaf(y.w, c, sum.w);
     }
+    if (result.out) {
+      if (result.has_sink) ll += ex2_fast(result.sink * 1.4426950408889634f - ref);
+      const float by = (ll > 0.f ? 1.f / ll : 0.f) * head_gate_of(result.gate, t, h0 + h);
+      const float z[4] = {sum.x * by, sum.y * by, sum.z * by, sum.w * by};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) st_dt(result.out, result.out_dt, ((size_t)t * a.Hq + h0 + h) * D + d + x, z[x]);
+      continue;
+    }
     const size_t at_p = ((size_t)r * a.Hq + h0 + h) * a.slots + split;
     *(float4*)(a.part_o + at_p * D + d) = sum;
     if (d == 0) {
@@ -832,7 +848,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const floa
   __shared__ float4 sum_s[W > 1 ? JOIN_WARPS : 1][C * 32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = warp % W;
   const int pair = min((int)blockIdx.x * (JOIN_WARPS / W) + warp / W, pairs - 1), r = pair / Hq, h = pair % Hq, t = rows ? rows[r] : r;
-  const int n = group[r] >= 0 ? slots : own;
+  const int n = group && group[r] >= 0 ? slots : own;
   const size_t at = (size_t)pair * slots;
   grid_dep_wait();
   grid_dep_launch();
@@ -949,17 +965,17 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
 }
 
 template <int D, int TERMS>
-int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int beside, cudaStream_t s) {
+int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int beside, const OwnResult& result, cudaStream_t s) {
   const int parts = (a.Hq / a.Hkv + OW_HEADS - 1) / OW_HEADS;
   NV_RETURN_IF(launch_dep(own_keys_kernel<D, TERMS>, dim3(R, a.Hkv * parts, own_splits), dim3(OW_WARPS * 32), 0, s, a, first, own_splits,
-                          score_map(a.scale, a.softcap), beside));
+                          score_map(a.scale, a.softcap), beside, result));
   NV_RETURN_LAST();
 }
 
 template <int TERMS>
-int launch_own_d(const SharedArgs& a, const int* first, int R, int own_splits, int beside, cudaStream_t s) {
-  return a.D == 64 ? launch_own<64, TERMS>(a, first, R, own_splits, beside, s) : a.D == 80 ? launch_own<80, TERMS>(a, first, R, own_splits, beside, s)
-         : a.D == 96 ? launch_own<96, TERMS>(a, first, R, own_splits, beside, s) : a.D == 128 ? launch_own<128, TERMS>(a, first, R, own_splits, beside, s) : launch_own<256, TERMS>(a, first, R, own_splits, beside, s);
+int launch_own_d(const SharedArgs& a, const int* first, int R, int own_splits, int beside, const OwnResult& result, cudaStream_t s) {
+  return a.D == 64 ? launch_own<64, TERMS>(a, first, R, own_splits, beside, result, s) : a.D == 80 ? launch_own<80, TERMS>(a, first, R, own_splits, beside, result, s)
+         : a.D == 96 ? launch_own<96, TERMS>(a, first, R, own_splits, beside, result, s) : a.D == 128 ? launch_own<128, TERMS>(a, first, R, own_splits, beside, result, s) : launch_own<256, TERMS>(a, first, R, own_splits, beside, result, s);
 }
 template <int TERMS>
 int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
@@ -1023,7 +1039,7 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
   const int G = Hq / Hkv;
   const long long sms = num_multiprocessors(), blocks = (long long)R * Hkv * ((G + 15) / 16);
   const long long shared = shared_splits <= 0 ? 0 : shared_tiles(M, groups, Hq, Hkv, tc_takes(cache_dt, D, page) ? ST_PAIRS : SP_PAIRS) * Hkv * shared_splits;
-  const long long room = shared <= sms ? shared + 3 * (sms - shared) : 7 * sms;
+  const long long room = shared <= sms ? shared + (D > 128 ? 2 : 3) * (sms - shared) : 7 * sms;
   long long n = room / blocks;
   const long long least = shared <= sms || blocks * ((most + 127) / 128) <= 3 * sms ? 128 : 256;
   if (n > (most + least - 1) / least) n = (most + least - 1) / least;
@@ -1032,9 +1048,10 @@ NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int 
 
 // Whether `repeated` positions that need not be read again are worth a kernel more and a join (1) or not (0), in bytes of keys and
 // values.  Tensor-core form: 24 MB, and 32 KB for every row and kv head, whose parts are joined.  (Calls behind one another would have
-// it pay a little sooner: shared and not, four rows of 16 kv heads behind 700 positions, 17 MB, 9.9 and 10.5 us, behind 1,500, 37 MB,
-// 10.3 and 14.0; eight of 4 behind 1,500, 22 MB, 11.6 and 14.3, behind 2,048, 29 MB, 11.7 and 15.1; 64 of 16 behind 64, 33 MB, 19.0 and
-// 18.7, behind 128, 66 MB, 19.9 and 23.8.  In a model's step the kernel without groups begins beside the one in front, and the step
+// it pay about as soon: shared and not, four rows of 16 kv heads behind 1,000 positions, 24 MB, 10.5 and 11.2 us, behind 1,500, 37 MB,
+// 10.5 and 12.8; eight of 4 behind 1,500, 22 MB, 11.7 and 10.9, behind 2,048, 29 MB, 11.6 and 12.3, behind 4,000, 57 MB, 12.6 and 15.5;
+// 64 of 16 behind 64, 33 MB, 17.1 and 16.2, behind 128, 66 MB, 18.0 and 20.5; 16 rows of 16 heads of 256 on 1 behind 1,000, 15 MB,
+// 14.9 and 13.6, behind 2,000, 31 MB, 15.3 and 23.1.  In a model's step the kernel without groups begins beside the one in front, and the step
 // has to look for groups: 16 layers with eight rows of 4 behind 1,500 take 2.26 and 2.27 ms without and with groups, behind 2,048 2.28
 // either way, 32 rows behind 1,024, 65 MB, 2.74 and 2.65.)  Plain form: 192 KB
 // for every row and kv head, since the kernel without groups is slow at few rows of these
@@ -1047,10 +1064,17 @@ NV_API int nv_attention_shared_pays(int R, int M, int groups, int Hq, int Hkv, i
   return saved >= 196608 * parts && 2LL * M * (Hq / Hkv) >= (long long)SP_PAIRS * groups;
 }
 
+// Whether rows that share nothing take the own-key kernel and, from two parts on, the join instead of the split-key kernel: its types
+// and sizes (both: 40 rows of 28 heads on 4, 400 to 700 positions, 16.8 and 21.4 us, in pages of 32 16.8 and 21.1; two behind 4,000 9.1 and
+// 13.1; four of 16 on 16 behind 496 9.4 and 9.6; eight of 16 heads of 256 on 1 behind 300, pages of 32, 9.5 and 32.7).
+NV_API int nv_attention_shared_alone(int D, int page, int cache_dt) {
+  return tc_takes(cache_dt, D, page) && own_takes(D) ? 1 : 0;
+}
+
 NV_API int nv_attention_shared_usable(int D, int page) { return D >= 8 && D <= 256 && D % 8 == 0 && page >= 16 && page % 16 == 0; }
 
 // R rows (rows: their batch rows, nullptr: all); first [R]: positions of the row that are shared (0 without a group), group [R]: its
-// group or -1, members [M], cu [groups + 1], len and lead [groups]: see SharedArgs.  own_splits and shared_splits parts a (row, head);
+// group or -1 (both nullptr: none shares, see nv_attention_shared_alone), members [M], cu [groups + 1], len and lead [groups]: see SharedArgs.  own_splits and shared_splits parts a (row, head);
 // scratch: R * Hq * (own_splits + shared_splits) * (D + 2) floats.
 NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                                       const int* block_table, int max_blocks, const int* row_entry, const int* positions,
@@ -1081,12 +1105,16 @@ NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, c
                    : exact ? launch_tc_d<3>(a, tiles, stream) : launch_tc_d<1>(a, tiles, stream);
     if (rc) return rc;
   }
-  const int rc = tc && own_takes(D) ? (exact ? launch_own_d<3>(a, first, R, own_splits, beside, stream) : launch_own_d<1>(a, first, R, own_splits, beside, stream))
+  const HeadGate gated{gate, gate_ld};
+  const bool direct = tc && own_takes(D) && slots == 1 && !beside;
+  const OwnResult result{direct ? out : nullptr, out_dt, has_sink, sink_score, gated};
+  const int rc = tc && own_takes(D) ? (exact ? launch_own_d<3>(a, first, R, own_splits, beside, result, stream)
+                                             : launch_own_d<1>(a, first, R, own_splits, beside, result, stream))
+                 : !first ? NV_ERR_UNSUPPORTED
                  : nv_attention_decode_rest(qkv, q_dt, q_stride, kc, vc, cache_dt, block_table, max_blocks, row_entry, positions, rows,
                                             first, R, scale, out_dt, Hq, Hkv, D, page, num_pages, own_splits, slots, scratch, err, exact,
                                             softcap, beside, stream);
-  if (rc) return rc;
-  const HeadGate gated{gate, gate_ld};
+  if (rc || direct) return rc;
   // A warp a pair where there are many with few parts, else two (128 rows of 28 heads, 11 parts: 51.4 and 52.2 us; 64 rows, 18: 35.1 and
   // 34.0; 50 of 24, three terms, 9: 17.9 and 16.9).
   return slots <= 12 && (long long)R * Hq >= 2048

@@ -523,14 +523,17 @@ class SharedPrefix:
         if key not in self._splits:
             _need(attention_decode_shared_usable(k_cache, D), f"attention_decode_shared: heads of {D} elements in pages of {page} are not supported")
             pair = lib().nv_attention_decode_splits_of(self.R, Hq, Hkv, D, max_context, num_sms()), 0, None
+            sizes = self.members, self.groups, Hq, Hkv, D, page, _DT[dtype]
             if attention_sharing_pays(self.R, self.members, self.groups, Hq, Hkv, D, page, dtype, self.repeated):
-                sizes = self.members, self.groups, Hq, Hkv, D, page, _DT[dtype]
                 own = max(1, max_context - self.shortest // page * page)          # the most keys a row reads for itself
                 ours = lib().nv_attention_shared_splits(*sizes, terms, self.longest)
                 splits = lib().nv_attention_shared_own_splits(self.R, *sizes, ours, own)
                 first, group, members, cu, lens, leads = self.places
                 pair = splits, ours, (ctypes.c_longlong * 17)(_DT[dtype], Hq, Hkv, D, page, self.R, first, group, members, self.members, cu,
                                                               lens, leads, self.groups, splits, ours, terms)
+            elif lib().nv_attention_shared_alone(D, page, _DT[dtype]):
+                splits = lib().nv_attention_shared_own_splits(self.R, *sizes, 0, max_context)
+                pair = splits, 0, (ctypes.c_longlong * 17)(_DT[dtype], Hq, Hkv, D, page, self.R, 0, 0, 0, 0, 0, 0, 0, 0, splits, 0, terms)
             self._splits[key] = pair
         return self._splits[key]
 
@@ -574,7 +577,7 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
           "attention_decode_shared: a prefix reaches beyond the block tables")
     terms = 1 if float_weights or sink_score is not None else 0
     splits, ours, plan = shared.splits(Hq, Hkv, D, k_cache, terms, max_context)
-    if ours == 0:
+    if ours == 0 and (plan is None or width % 8 or (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
         return _launch_decode(qkv, k_cache, v_cache, block_table, row_entry, positions, scale, 0, out, Hq, Hkv, D, R, splits, rows, err,
                               sink_score, float_weights, softcap, gate, (0, None, None, 0), True)
     scratch = torch.empty(R * Hq * (splits + ours) * (D + 2), dtype=torch.float32, device=qkv.device)

@@ -458,6 +458,14 @@ def test_attention_with_infinities_and_nan_behind_the_rows_ends(D, page, sink):
     assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
 
 
+def test_attention_of_queries_off_any_boundary():
+    c = Case(8, 2, 64, *GROUPS[0][::-1])
+    q = torch.empty(c.q.numel() + 4, dtype=c.q.dtype, device=DEV)[4:].view_as(c.q)
+    c.q = q.copy_(c.q)
+    assert c.q.data_ptr() % 16 == 8
+    c.check()
+
+
 def test_attention_of_many_rows_with_long_keys_of_their_own():
     """More keys in a split than a warp keeps places of."""
     lengths = [2100 + r % 40 for r in range(520)]
