@@ -664,7 +664,9 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
   uint4 q[KC];
 #pragma unroll
   for (int c = 0; c < KC; ++c)
-    q[c] = g < heads && c * 32 + tq * 8 < D ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8) : make_uint4(0, 0, 0, 0);
+    q[c] = g < heads && c * 32 + tq * 8 < D
+               ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8)
+               : make_uint4(0, 0, 0, 0);
 
   float o[8 * RUNS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -949,7 +951,8 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
   rc = nv_tensor_map_bf16(a.vc, rows, a.D, a.D, a.page, &tm_v);
   if (rc) return rc;
   constexpr int SL = D / 64;
-  constexpr size_t tiles_bytes = (size_t)SL * ST_PAIRS * 128 + (2 + st_v_buffers<D, TERMS>()) * (size_t)SL * ST_KEYS * 128 + (TERMS > 1 ? (size_t)TERMS * ST_PAIRS * 128 : 0);
+  constexpr size_t tiles_bytes = (size_t)SL * ST_PAIRS * 128 + (2 + st_v_buffers<D, TERMS>()) * (size_t)SL * ST_KEYS * 128 +
+                                 (TERMS > 1 ? (size_t)TERMS * ST_PAIRS * 128 : 0);
   constexpr size_t smem = tiles_bytes + 1024;
   static_assert(tiles_bytes >= (size_t)ST_PAIRS * (D * 4 + 16), "a row of results has its place");
   static bool attr_done = false;
@@ -974,8 +977,11 @@ int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int
 
 template <int TERMS>
 int launch_own_d(const SharedArgs& a, const int* first, int R, int own_splits, int beside, const OwnResult& result, cudaStream_t s) {
-  return a.D == 64 ? launch_own<64, TERMS>(a, first, R, own_splits, beside, result, s) : a.D == 80 ? launch_own<80, TERMS>(a, first, R, own_splits, beside, result, s)
-         : a.D == 96 ? launch_own<96, TERMS>(a, first, R, own_splits, beside, result, s) : a.D == 128 ? launch_own<128, TERMS>(a, first, R, own_splits, beside, result, s) : launch_own<256, TERMS>(a, first, R, own_splits, beside, result, s);
+  return a.D == 64   ? launch_own<64, TERMS>(a, first, R, own_splits, beside, result, s)
+         : a.D == 80 ? launch_own<80, TERMS>(a, first, R, own_splits, beside, result, s)
+         : a.D == 96 ? launch_own<96, TERMS>(a, first, R, own_splits, beside, result, s)
+         : a.D == 128 ? launch_own<128, TERMS>(a, first, R, own_splits, beside, result, s)
+                      : launch_own<256, TERMS>(a, first, R, own_splits, beside, result, s);
 }
 template <int TERMS>
 int launch_tc_d(const SharedArgs& a, int tiles, cudaStream_t s) {
@@ -1074,7 +1080,8 @@ NV_API int nv_attention_shared_alone(int D, int page, int cache_dt) {
 NV_API int nv_attention_shared_usable(int D, int page) { return D >= 8 && D <= 256 && D % 8 == 0 && page >= 16 && page % 16 == 0; }
 
 // R rows (rows: their batch rows, nullptr: all); first [R]: positions of the row that are shared (0 without a group), group [R]: its
-// group or -1 (both nullptr: none shares, see nv_attention_shared_alone), members [M], cu [groups + 1], len and lead [groups]: see SharedArgs.  own_splits and shared_splits parts a (row, head);
+// group or -1 (both nullptr: none shares, see nv_attention_shared_alone), members [M], cu [groups + 1], len and lead [groups]: see
+// SharedArgs.  own_splits and shared_splits parts a (row, head);
 // scratch: R * Hq * (own_splits + shared_splits) * (D + 2) floats.
 NV_API int nv_attention_decode_shared(const void* qkv, int q_dt, int q_stride, const void* kc, const void* vc, int cache_dt,
                                       const int* block_table, int max_blocks, const int* row_entry, const int* positions,
