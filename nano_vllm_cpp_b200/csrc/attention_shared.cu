@@ -540,8 +540,12 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int position = a.positions[t];
       grid_dep_wait();
       grid_dep_launch();
-      gather_queries<D>(a, Qs, q, lane, pairs, t, h);
-      if (lane == 0) mbar_arrive(&q_full);
+      // (A split without keys has no products: nobody waits for its queries, and nothing would order one warp's gathering before
+      // another's results, which take the same shared memory.)
+      if (n_blocks > 0) {
+        gather_queries<D>(a, Qs, q, lane, pairs, t, h);
+        if (lane == 0) mbar_arrive(&q_full);
+      }
       const int limit = live ? min(j_hi, position + 1) : j_hi;                  // the first key that this row does not see
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n_blocks; ++i) {
