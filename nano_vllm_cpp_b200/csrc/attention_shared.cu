@@ -614,6 +614,9 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (some)
         leave_part<D>(a, smem + (size_t)p * (D * 4 + 16), tmem_o + lane_off, n_blocks > 0, live, ((size_t)r * a.Hq + h) * a.slots + a.slot0 + split, m, l, map.in);
     }
+  } else {                       // no tile: a block waits all the same, since the kernel of the own keys relies on it (and there may be none with one)
+    grid_dep_wait();
+    grid_dep_launch();
   }
   tc_fence_before();
   __syncthreads();

@@ -35,3 +35,37 @@ def test_a_query_that_is_no_number_stays_in_its_row(Hq, Hkv, D, float_weights, b
         got = c.run(float_weights=float_weights, stale=3.0)
         assert torch.equal(got[healthy], clean[healthy]) and bool(torch.isnan(got[17]).all())
     assert bool(((clean.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(8, 2, 64, 16), (28, 4, 128, 32), (6, 2, 112, 16), (4, 2, 40, 16)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_arrays_without_groups_behind_the_kernel_that_writes_the_queries(Hq, Hkv, D, page, captured):
+    """A call with room for groups, bound to arrays that have none (a step whose last family has ended), waits for the kernel in
+    front, which is still at work on the queries when the call's kernels may begin."""
+    o = ops()
+    lengths = [5, 33, 170, 64]
+    c = Case(Hq, Hkv, D, lengths, [([0, 1], page), ([2, 3], page)], page)
+    shared = o.SharedPrefix(c.groups, 4, DEV, room=(4, 2))
+    shared.bind(i32(o.SharedPrefix.pack([], 4, 2)[0]))
+    x, w = rnd(4, 16384, seed=7, dtype=torch.bfloat16), rnd(c.q.shape[1], 16384, seed=8, dtype=torch.bfloat16) / 128
+    out = torch.empty(4, Hq * D, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        c.q.fill_(NAN)
+        o.gemm_plain(x, w, c.q)
+        c.run(shared=shared, out=out)
+
+    step()
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        step = graph.replay
+    for k in range(20):
+        x.copy_(rnd(4, 16384, seed=20 + k, dtype=torch.bfloat16))
+        out.fill_(NAN)
+        step()
+        torch.cuda.synchronize()
+        want, weight, score = c.want()
+        assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score)).all())
