@@ -64,7 +64,8 @@ struct DecArgs {
   const int* first;
   int slots;
   // REST: the kernel in front writes nothing that is read here, and waited itself for the kernel in front of it: this one runs
-  // beside it and waits for it where it ends, so that who waits for this kernel has waited for both
+  // beside it and waits for it where it ends, so that who waits for this kernel has waited for both (it reads the queries past the
+  // first cache, having waited for nobody when it does)
   int beside;
   void* out;
   float* part_o;          // [rows, Hq, splits, D]
@@ -237,7 +238,8 @@ __global__ void __launch_bounds__((WARPS + 1) * 32) attention_decode_kernel(DecA
   grid_dep_launch();
   for (int i = threadIdx.x; i < ng * D; i += (WARPS + 1) * 32) {
     int g = i / D, d = i % D;
-    q_s[g][d] = ld_dt(a.qkv, a.q_dt, (size_t)t * a.q_stride + (size_t)(kvh * G + g0 + g) * D + d) * a.scale;
+    const size_t at = (size_t)t * a.q_stride + (size_t)(kvh * G + g0 + g) * D + d;
+    q_s[g][d] = (REST ? ld_dt_cg(a.qkv, a.q_dt, at) : ld_dt(a.qkv, a.q_dt, at)) * a.scale;
   }
   const int* bt = a.block_table + (size_t)a.row_entry[t] * a.max_blocks;
   // the producer must not wait for a block-table entry per page: that load's latency would bound the stream
@@ -521,7 +523,8 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __gri
     for (int i = threadIdx.x; i < TC_ROWS * D; i += WARPS * 32) {
       const int g = i / D, d = i % D;
       float v = 0.f;
-      if (g < ng && d < a.D) v = ld_dt(a.qkv, a.q_dt, (size_t)t * a.q_stride + (size_t)(kvh * G + g0 + g) * a.D + d);
+      const size_t at = (size_t)t * a.q_stride + (size_t)(kvh * G + g0 + g) * a.D + d;
+      if (g < ng && d < a.D) v = REST ? ld_dt_cg(a.qkv, a.q_dt, at) : ld_dt(a.qkv, a.q_dt, at);
       q_s[g * QLD + d] = __float2bfloat16_rn(v);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");      // the consumer warps only

@@ -24,7 +24,8 @@ int nv_attention_decode_rest(const void* qkv, int q_dt, int q_stride, const void
 
 namespace {
 
-// (Keys, values and parts are read past the first cache: kernels in front may write them while a kernel here has begun.)
+// (Queries, keys, values, parts and their sums are read past the first cache where a kernel reads them beside the one in front or without
+// a wait of its own: kernels in front may write them while a kernel here has begun.)
 struct SharedArgs {
   const void* q;
   const void* kc;
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
 #pragma unroll
   for (int c = 0; c < KC; ++c)
     q[c] = g < heads && c * 32 + tq * 8 < D
-               ? *(const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8)
+               ? __ldcg((const uint4*)((const bf16*)a.q + (long long)t * a.q_stride + (long long)(h0 + g) * D + c * 32 + tq * 8))
                : make_uint4(0, 0, 0, 0);
 
   float o[8 * RUNS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -849,7 +850,7 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
 constexpr int MAX_PARTS = 64, JOIN_WARPS = 4;
 
 template <int W, bool WIDE>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+__global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const float* part_o, const float* part_ml,
                                                                       const int* __restrict__ rows, const int* __restrict__ group,
                                                                       void* out, int out_dt, int pairs, int Hq, int D, int own, int slots,
                                                                       int has_sink, float sink, HeadGate gate, int whole) {
@@ -863,7 +864,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) shared_join_kernel(const floa
   grid_dep_launch();
   const float2 none = make_float2(-1e30f, 0.f);
   const float2* ml = (const float2*)part_ml + at;
-  const float2 x = lane < n ? ml[lane] : none, y = lane + 32 < n ? ml[lane + 32] : none;
+  const float2 x = lane < n ? __ldcg(ml + lane) : none, y = lane + 32 < n ? __ldcg(ml + lane + 32) : none;
   float4 o[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -44,6 +44,10 @@ __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat1
 __device__ __forceinline__ float ld_dt(const void* p, int dt, size_t i) {
   return dt == NV_DT_F32 ? ((const float*)p)[i] : __bfloat162float(((const bf16*)p)[i]);
 }
+// ... past the first cache
+__device__ __forceinline__ float ld_dt_cg(const void* p, int dt, size_t i) {
+  return dt == NV_DT_F32 ? __ldcg((const float*)p + i) : __bfloat162float(__ldcg((const bf16*)p + i));
+}
 __device__ __forceinline__ void st_dt(void* p, int dt, size_t i, float v) {
   if (dt == NV_DT_F32) ((float*)p)[i] = v;
   else ((bf16*)p)[i] = __float2bfloat16_rn(v);

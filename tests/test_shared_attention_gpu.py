@@ -69,3 +69,40 @@ def test_arrays_without_groups_behind_the_kernel_that_writes_the_queries(Hq, Hkv
         torch.cuda.synchronize()
         want, weight, score = c.want()
         assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(28, 4, 128), (8, 2, 64), (6, 2, 112), (6, 2, 40), (16, 1, 256)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_layers_one_after_the_other_in_the_same_buffers(Hq, Hkv, D, captured):
+    """As a step's layers call it: the product in front writes the queries into one buffer, over those of the layer before, and the
+    calls' scratch is the same memory; no layer takes the queries, parts or sums of another."""
+    o = ops()
+    lengths = [700 + 13 * r for r in range(8)] + [40, 3]
+    c = Case(Hq, Hkv, D, lengths, [(list(range(8)), 656)])
+    shared, layers, q = o.SharedPrefix(c.groups, 10, DEV), 12, c.q
+    xs = [rnd(10, 2048, seed=s, dtype=torch.bfloat16) for s in range(layers)]
+    w = rnd(q.shape[1], 2048, seed=99, dtype=torch.bfloat16) / 45
+    outs = [torch.empty(10, Hq * D, dtype=torch.bfloat16, device=DEV) for _ in range(layers)]
+
+    def step():
+        for x, out in zip(xs, outs):
+            o.gemm_plain(x, w, q)
+            c.run(shared=shared, out=out)
+
+    step()
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        step = graph.replay
+    for _ in range(5):
+        for out in outs:
+            out.fill_(NAN)
+        step()
+    torch.cuda.synchronize()
+    for x, out in zip(xs, outs):
+        c.q = torch.empty_like(q)
+        o.gemm_plain(x, w, c.q)
+        want, weight, score = c.want()
+        assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score)).all())
