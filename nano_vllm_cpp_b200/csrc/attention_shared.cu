@@ -446,7 +446,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       grid_dep_launch();
       auto load = [&](int i, bool values, int blk) {
         if (blk != -2 && (blk < 0 || blk >= a.num_pages)) {                    // it should be there and is not
-          atomicExch(a.err, 1 + lead_t);
+          if (a.err) atomicExch(a.err, 1 + lead_t);
           blk = -1;
         }
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, blk >= 0));

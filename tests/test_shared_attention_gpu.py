@@ -106,3 +106,24 @@ def test_layers_one_after_the_other_in_the_same_buffers(Hq, Hkv, D, captured):
         o.gemm_plain(x, w, c.q)
         want, weight, score = c.want()
         assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+
+
+# ------------------------------------------------------------------------------------------------ pages that are not there
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.bfloat16, 112), (torch.float32, 64)])
+def test_the_c_entry_without_an_error_flag_passes_a_missing_page_by(dtype, D):
+    """Nobody is told, and nothing else happens: rows that do not read the page have their results."""
+    o = ops()
+    c = Case(4, 2, D, [200, 210, 90], [([0, 1], 192)], 16, dtype)
+    c.table[0, 3] = -1
+    shared, out = o.SharedPrefix(c.groups, 3, DEV), torch.empty(3, 4 * D, dtype=dtype, device=DEV)
+    scratch = torch.empty(3 * 4 * 2 * (D + 2), dtype=torch.float32, device=DEV)
+    first, group, members, cu, lens, leads = shared.places
+    dt = o.dt(c.q)
+    assert o.lib().nv_attention_decode_shared(c.q.data_ptr(), dt, c.q.shape[1], c.k.data_ptr(), c.v.data_ptr(), dt, c.table.data_ptr(),
+                                              c.table.shape[1], c.entry.data_ptr(), c.positions.data_ptr(), None, 3, first, group, members, 2,
+                                              cu, lens, leads, 1, c.scale, out.data_ptr(), dt, 4, 2, D, 16, c.k.shape[0], 1, 1,
+                                              scratch.data_ptr(), None, 0, 0.0, 0, 0.0, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    c.table[0, 3] = 0
+    want, weight, score = c.want()
+    assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score))[2].all())
