@@ -52,7 +52,8 @@ struct Tile {
   int group, pair0, pairs, member0, len, lead;
 };
 // Which tile of `rows_per_tile` pairs of which group is tile number x?  A whole warp looks, 32 groups at a time; group < 0: none (a
-// launch has as many tiles as there may be).
+// launch has as many tiles as there may be).  A prefix that reaches beyond the block tables is read as far as these go, and reported:
+// the arrays may have been replaced since the host last looked.
 __device__ __forceinline__ Tile find_tile(const SharedArgs& a, int x, int G, int rows_per_tile, int lane) {
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = min(g0 + lane, a.groups - 1);
@@ -67,8 +68,9 @@ __device__ __forceinline__ Tile find_tile(const SharedArgs& a, int x, int G, int
     const uint32_t who = __ballot_sync(0xffffffffu, x < end);
     if (who) {
       const int l = __ffs(who) - 1, pair0 = (x - __shfl_sync(0xffffffffu, end - tiles, l)) * rows_per_tile;
+      if (lane == l && len / a.page > a.max_blocks && a.err) atomicExch(a.err, 1 + (a.rows ? a.rows[lead] : lead));
       return Tile{g0 + l, pair0, __shfl_sync(0xffffffffu, pairs, l) - pair0, __shfl_sync(0xffffffffu, from, l),
-                  __shfl_sync(0xffffffffu, len, l) / a.page * a.page, __shfl_sync(0xffffffffu, lead, l)};
+                  min(__shfl_sync(0xffffffffu, len, l) / a.page, a.max_blocks) * a.page, __shfl_sync(0xffffffffu, lead, l)};
     }
     x -= __shfl_sync(0xffffffffu, end, 31);
   }

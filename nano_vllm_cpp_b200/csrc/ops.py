@@ -477,8 +477,7 @@ class SharedPrefix:
         _need(members <= self.members <= rows, "SharedPrefix: room for the grouped rows, and no more than there are rows")
         self.R = rows
         self.longest, self.shortest, self.repeated = self.facts(groups, rows) if facts is None else facts
-        self.reach = max((n for _, n in groups), default=0)          # positions that the block tables must cover
-        self.bind(torch.tensor(packed, dtype=torch.int32).to(device) if buf is None else buf)
+        self.bind(torch.tensor(packed, dtype=torch.int32).to(device) if buf is None else buf, max((n for _, n in groups), default=0))
 
     @staticmethod
     def facts(groups, rows: int):
@@ -508,10 +507,13 @@ class SharedPrefix:
         none = [0] * empty
         return first + group + members + [0] * (rows - len(members)) + cu + [cu[-1]] * empty + lens + none + leads + none, len(members)
 
-    def bind(self, buf) -> None:
-        """Has the calls read the packed arrays ``buf``, of as many rows and groups as these."""
+    def bind(self, buf, reach: int = 0) -> None:
+        """Has the calls read the packed arrays ``buf``, of as many rows and groups as these.  ``reach``: positions of their longest
+        prefix, which the block tables must cover.  Where that is not said, or the arrays' contents are replaced later, a prefix
+        that reaches beyond the tables sets the error flag, and is read as far as they go."""
         R, G, at = self.R, self.groups, buf.data_ptr()
         _need(buf.dtype == torch.int32 and buf.numel() >= 3 * R + 3 * G + 1, "SharedPrefix: the packed arrays are int32, of these rows and groups")
+        self.reach = int(reach)
         self.buf, self._splits = buf, {}                             # (what the launcher takes for a plan has their addresses)
         self.places = tuple(at + 4 * n for n in (0, R, 2 * R, 3 * R, 3 * R + G + 1, 3 * R + 2 * G + 1))
 

@@ -112,3 +112,13 @@ def test_tensors_of_the_host_are_refused():
         ops.PageArrays([torch.zeros(4, 2, 16, 8)])
     with pytest.raises(ops.KernelError):
         ops.PageArrays([])
+
+
+def test_bound_arrays_come_with_what_the_block_tables_must_cover():
+    shared = ops.SharedPrefix([([0, 1], 32)], 3, "cpu", room=(3, 2))
+    pack = lambda groups: torch.tensor(ops.SharedPrefix.pack(groups, 3, 2)[0], dtype=torch.int32)
+    assert shared.reach == 32
+    shared.bind(pack([([0, 1, 2], 4096)]), reach=4096)
+    assert shared.reach == 4096
+    shared.bind(pack([([2], 5)]))                                           # (not said: the kernels look)
+    assert shared.reach == 0

@@ -127,3 +127,25 @@ def test_the_c_entry_without_an_error_flag_passes_a_missing_page_by(dtype, D):
     c.table[0, 3] = 0
     want, weight, score = c.want()
     assert bool(((out.double() - want).abs() <= c.tolerance(want, weight, score))[2].all())
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.bfloat16, 112), (torch.float32, 64)])
+def test_bound_arrays_that_reach_beyond_the_block_tables(dtype, D):
+    """Refused where ``bind`` says how far they reach; else reported, and the rows, which end inside the tables, have their results."""
+    o = ops()
+    c = Case(4, 2, D, [160, 150, 33, 130], [([0, 1, 2], 160)], 16, dtype)
+    c.table = c.table[:, :10].contiguous()
+    shared = o.SharedPrefix(c.groups, 4, DEV)
+    far = i32(o.SharedPrefix.pack([([0, 1, 2], 100000)], 4)[0])
+    shared.bind(far, reach=100000)
+    with pytest.raises(o.KernelError):
+        c.run(shared=shared)
+    want, weight, score = c.want()
+    for bound in (True, False):
+        shared.bind(far if bound else i32(o.SharedPrefix.pack(c.groups, 4)[0]))
+        shared.buf.copy_(far)                                               # (a replaced content, as steps of one shape replace it)
+        err = o.ErrorFlag(DEV)
+        got = c.run(shared=shared, err=err)
+        assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+        with pytest.raises(o.KernelError):
+            err.check("shared")
