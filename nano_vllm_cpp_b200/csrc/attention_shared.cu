@@ -273,13 +273,26 @@ __device__ __forceinline__ void gather_queries(const SharedArgs& a, uint8_t* Qs,
   __syncwarp();
 }
 
+// A score's cap, in base-2 units.  TERMS 3, where the weights keep all their bits: tanhf's tangent, whose error is one of the result; that
+// of capped_log2 is some 2^-22 of the cap, however small the score.  (shared_map has the factor that either takes.)
+template <int TERMS>
+__device__ __forceinline__ float capped(const ScoreMap& map, float s) {
+  return TERMS > 1 ? map.cap1 * tanhf(s * map.cap_k) : capped_log2(map, s);
+}
+static inline ScoreMap shared_map(float scale, float softcap, int terms) {
+  ScoreMap map = score_map(scale, softcap);
+  if (terms > 1 && softcap > 0.f) map.cap_k = scale / softcap;
+  return map;
+}
+
 // A pair's next block of scores, from key j on, becomes weights against its reference m; returns the sum of its weights, l among them.
 // The reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost bfloat16 and the float32
 // sums nothing), so that O is rescaled, by alpha, once in a long while.
+template <int TERMS>
 __device__ __forceinline__ float softmax_step(const ScoreMap& map, float* s, int j, int limit, float& m, float& alpha, float l) {
   if (map.cap1 > 0.f) {
 #pragma unroll
-    for (int c = 0; c < ST_KEYS; ++c) s[c] = capped_log2(map, s[c]);
+    for (int c = 0; c < ST_KEYS; ++c) s[c] = capped<TERMS>(map, s[c]);
   }
   if (j + ST_KEYS > limit) {
 #pragma unroll
@@ -567,7 +580,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free);
         if (some) {
-          l = softmax_step(map, s, j0, limit, m, alpha, l);
+          l = softmax_step<TERMS>(map, s, j0, limit, m, alpha, l);
         }
         // O += P(i-1) V(i-1) must have ended before O is rescaled and P is overwritten (a warp without pairs waits too: its
         // arrival is one for this block)
@@ -747,7 +760,7 @@ __global__ void __launch_bounds__(OW_WARPS * 32, D <= 128 ? 3 : 2) own_keys_kern
     // s: keys g (heads 2 tq, 2 tq + 1) and g + 8, in base-2 units from here on
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      s[x] = map.cap1 > 0.f ? capped_log2(map, s[x]) : s[x] * map.in;
+      s[x] = map.cap1 > 0.f ? capped<TERMS>(map, s[x]) : s[x] * map.in;
       if (!here || g + (x >> 1) * 8 >= left) s[x] = -INFINITY;
     }
     float alpha[2], ref[2];
@@ -971,7 +984,7 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
     attr_done = true;
   }
   // scores go to base-2 units by map.in; capped ones are there already
-  ScoreMap map = score_map(a.scale, a.softcap);
+  ScoreMap map = shared_map(a.scale, a.softcap, TERMS);
   if (a.softcap > 0.f) map.in = 1.f;
   NV_RETURN_IF(launch_dep(shared_tc_kernel<D, TERMS>, dim3(tiles, a.Hkv, a.splits), dim3(ST_THREADS), smem, s, tm_k, tm_v, a, map));
   NV_RETURN_LAST();
@@ -981,7 +994,7 @@ template <int D, int TERMS>
 int launch_own(const SharedArgs& a, const int* first, int R, int own_splits, int beside, const OwnResult& result, cudaStream_t s) {
   const int parts = (a.Hq / a.Hkv + OW_HEADS - 1) / OW_HEADS;
   NV_RETURN_IF(launch_dep(own_keys_kernel<D, TERMS>, dim3(R, a.Hkv * parts, own_splits), dim3(OW_WARPS * 32), 0, s, a, first, own_splits,
-                          score_map(a.scale, a.softcap), beside, result));
+                          shared_map(a.scale, a.softcap, TERMS), beside, result));
   NV_RETURN_LAST();
 }
 

@@ -149,3 +149,17 @@ def test_bound_arrays_that_reach_beyond_the_block_tables(dtype, D):
         assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
         with pytest.raises(o.KernelError):
             err.check("shared")
+
+
+# ------------------------------------------------------------------------------------------------ precision
+@pytest.mark.parametrize("Hq,Hkv,D", [(28, 4, 128), (24, 4, 96), (8, 2, 64), (16, 1, 256), (6, 2, 112)])
+@pytest.mark.parametrize("grouped", [True, False])
+def test_a_cap_beside_a_sink_costs_no_bits(Hq, Hkv, D, grouped):
+    """A cap far above the scores: its function is the identity there, and an error in units of the cap would be one of 2 % in a weight
+    or more.  Weights keep all their bits beside a sink; tanhf is off by two units of its result at most, the scale and the cap by
+    half a unit each, within the eight units of a score that the tolerance holds beside the products' own."""
+    lengths = [301, 44, 17, 333, 37, 300, 90, 100, 131, 1]
+    c = Case(Hq, Hkv, D, lengths, [([3, 0, 5], 300), ([8, 7], 96)] if grouped else [], seed=6)
+    got = c.run(sink_score=0.5, softcap=1e5, stale=NAN)
+    want, weight, score = c.want(sink=0.5, softcap=1e5)
+    assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
