@@ -25,6 +25,9 @@ from ..csrc import host
 from .block_pool import BlockPool, NoFreePages
 
 
+_NOBODY = -1 << 63         # no request's native id: those of requests that are not named by a number count down from -1
+
+
 class NoFreeSlot(RuntimeError):
     pass
 
@@ -196,7 +199,7 @@ class CacheManager:
         """Which of these requests begin with the same full pages of a group: (places in ``rids``, positions in common) per
         set of two or more, in the order of their first members.  Requests that are not open share nothing."""
         S = len(rids)
-        ids = (ctypes.c_int64 * max(S, 1))(*[r if type(r) is int else self._ids.get(r, -1) for r in rids])
+        ids = (ctypes.c_int64 * max(S, 1))(*[r if type(r) is int else self._ids.get(r, _NOBODY) for r in rids])
         group_of, pages = (ctypes.c_int * max(S, 1))(), (ctypes.c_int * max(S, 1))()
         n = host.lib().nvh_shared_prefixes(self._h, S, ids, group, group_of, pages)
         if n < 0:

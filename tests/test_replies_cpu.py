@@ -196,3 +196,15 @@ def test_sampling_parameters_refuse(kw):
 def test_sampling_parameters_take():
     for kw in (dict(n=5), dict(logprobs=0), dict(logprobs=32), dict(logprobs=None)):
         SamplingParams(**kw).validate()
+
+
+def test_requests_that_are_not_open_share_nothing():
+    """Names that the manager does not know, beside the request that was named first."""
+    m = CacheManager([0], 20, 16, 4)
+    m.open("first")
+    run(m, "first", 40)
+    assert m.shared_prefixes(["first", "nobody", 7, ("nor", 1)], 0) == []
+    m.fork("first", "second")
+    assert m.shared_prefixes(["nobody", "second", 7, "first"], 0) == [([1, 3], 32)]
+    m.close("first")
+    assert m.shared_prefixes(["first", "second", "nobody"], 0) == []
