@@ -195,13 +195,15 @@ class CacheManager:
             self._raise(rc)
         return Fork(out[0], out[1], [tuple(out[3 + 4 * i:7 + 4 * i]) for i in range(out[2])])
 
-    def shared_prefixes(self, rids: list, group: int) -> list:
+    def shared_prefixes(self, rids: list, group: int, best: bool = False) -> list:
         """Which of these requests begin with the same full pages of a group: (places in ``rids``, positions in common) per
-        set of two or more, in the order of their first members.  Requests that are not open share nothing."""
+        set of two or more, in the order of their first members.  Requests that are not open share nothing.  A set is of all that
+        have one first page; with ``best`` of those that have to read the fewest positions if a set reads its common ones once
+        (families of replies behind one system prompt are sets of their own, a request that parts from them early is in none)."""
         S = len(rids)
         ids = (ctypes.c_int64 * max(S, 1))(*[r if type(r) is int else self._ids.get(r, _NOBODY) for r in rids])
         group_of, pages = (ctypes.c_int * max(S, 1))(), (ctypes.c_int * max(S, 1))()
-        n = host.lib().nvh_shared_prefixes(self._h, S, ids, group, group_of, pages)
+        n = host.lib().nvh_shared_prefixes(self._h, S, ids, group, int(best), group_of, pages)
         if n < 0:
             raise RuntimeError(host.last_error())
         out = [([], pages[k] * self.page_size) for k in range(n)]

@@ -39,7 +39,7 @@ _PROTOS = {
     "nvh_has": (c_int, [c_void_p, c_int64]),
     "nvh_open": (c_int, [c_void_p, c_int64]),
     "nvh_fork": (c_int, [c_void_p, c_int64, c_int64, _IP]),
-    "nvh_shared_prefixes": (c_int, [c_void_p, c_int, _LP, c_int, _IP, _IP]),
+    "nvh_shared_prefixes": (c_int, [c_void_p, c_int, _LP, c_int, c_int, _IP, _IP]),
     "nvh_close": (c_int, [c_void_p, c_int64]),
     "nvh_extend": (c_int, [c_void_p, c_int64, c_int, c_int]),
     "nvh_can_extend": (c_int, [c_void_p, c_int64, c_int, c_int]),

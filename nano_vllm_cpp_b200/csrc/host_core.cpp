@@ -166,6 +166,101 @@ struct RequestCache {
   uint64_t last_hash = 0;
 };
 
+// The full pages that a request begins with.
+struct Prefix {
+  const int* table = nullptr;
+  int full = 0;
+  // how many of its first `most` pages (where they are there) are the other's, of which `from` are known to be
+  int in_common(const Prefix& other, int from, int most) const {
+    const int n = std::min(most, std::min(full, other.full));
+    if (n <= from || std::memcmp(table + from, other.table + from, (n - from) * sizeof(int)) == 0) return std::max(n, from);
+    int k = from;
+    while (table[k] == other.table[k]) ++k;
+    return k;
+  }
+};
+
+// Requests that all begin with the same `common` pages, in sets whose members have more in common, where that saves more: a set of m
+// with n pages in common reads (m - 1) n pages less than its members by themselves, and a request is in one set.  The requests are
+// the leaves of the tree of their tables, a set belongs to the node where its members part, and a request goes to the deepest node
+// above it that has a set.  So with a node's set the requests below it, unless a deeper one takes them, count its depth instead of
+// that of the set above, and the set costs its depth once: for every set that may be above, worked out from the leaves on.
+struct FamilyTree {
+  struct Node {
+    int depth, level;                    // pages in common; nodes above
+    std::vector<int> leaves, children;   // requests that no deeper node holds; nodes
+    std::vector<long long> saved;        // pages, where the nearest set above is at level k - 1 of the path (0: none)
+    long long with_set;                  // ... where the node has a set
+  };
+  const std::vector<Prefix>& rows;
+  std::vector<int>& set;
+  std::vector<int>& set_pages;
+  std::vector<Node> nodes;
+
+  int grow(std::vector<int> own, int depth, int level) {
+    const int v = (int)nodes.size();
+    nodes.push_back({depth, level, {}, {}, {}, 0});
+    std::vector<std::pair<int, int>> next;                   // (the page behind, request)
+    for (int i : own)
+      if (rows[i].full > depth) next.push_back({rows[i].table[depth], i});
+      else nodes[v].leaves.push_back(i);
+    std::sort(next.begin(), next.end());
+    for (size_t a = 0, b; a < next.size(); a = b) {
+      for (b = a + 1; b < next.size() && next[b].first == next[a].first; ++b) {}
+      if (b == a + 1) {
+        nodes[v].leaves.push_back(next[a].second);
+        continue;
+      }
+      std::vector<int> below;
+      int n = rows[next[a].second].full;
+      for (size_t i = a; i < b; ++i) {
+        below.push_back(next[i].second);
+        if (i > a) n = rows[next[i].second].in_common(rows[next[a].second], depth + 1, n);
+      }
+      const int c = grow(std::move(below), n, level + 1);
+      nodes[v].children.push_back(c);
+    }
+    return v;
+  }
+  void count() {
+    std::vector<int> depths;                                 // of the nodes above, root first
+    for (int v = (int)nodes.size() - 1; v >= 0; --v) nodes[v].saved.resize(nodes[v].level + 1);
+    count(0, depths);
+  }
+  void count(int v, std::vector<int>& depths) {
+    depths.push_back(nodes[v].depth);
+    for (int c : nodes[v].children) count(c, depths);
+    depths.pop_back();
+    Node& x = nodes[v];
+    x.with_set = ((long long)x.leaves.size() - 1) * x.depth;
+    for (int c : x.children) x.with_set += nodes[c].saved[x.level + 1];
+    for (int k = 0; k <= x.level; ++k) x.saved[k] = std::max(x.with_set, without_set(x, k, k ? depths[k - 1] : 0));
+  }
+  long long without_set(const Node& x, int k, int depth) const {
+    long long n = (long long)x.leaves.size() * depth;
+    for (int c : x.children) n += nodes[c].saved[k];
+    return n;
+  }
+  // `above`: the number of the nearest set above, at level k - 1 of the path and of `depth` pages (-1, 0 and 0: none)
+  void assign(int v, int k, int depth, int above) {
+    const Node& x = nodes[v];
+    if (x.with_set > without_set(x, k, depth)) {
+      k = x.level + 1;
+      depth = x.depth;
+      above = (int)set_pages.size();
+      set_pages.push_back(depth);
+    }
+    for (int i : x.leaves) set[i] = above;
+    for (int c : x.children) assign(c, k, depth, above);
+  }
+};
+inline void split_family(const std::vector<Prefix>& rows, std::vector<int> own, int common, std::vector<int>& set, std::vector<int>& set_pages) {
+  FamilyTree tree{rows, set, set_pages, {}};
+  tree.grow(std::move(own), common, 0);
+  tree.count();
+  tree.assign(0, 0, 0, -1);
+}
+
 class CacheManager {
  public:
   std::vector<int> windows;
@@ -394,43 +489,48 @@ class CacheManager {
   }
   // Which of S requests begin with the same pages of group g?  group_of[i]: the number of entry i's group, or -1 (also where it is not
   // open); pages[k]: how many pages the entries of group k have in common, one at least.  Returns the number of groups, each of two
-  // entries or more.
-  int shared_prefixes(int S, const int64_t* rids, int g, int* group_of, int* pages) const {
+  // entries or more.  A group is of the requests that have one first page; `best`: of those that read the fewest pages together
+  // (split_family).
+  int shared_prefixes(int S, const int64_t* rids, int g, bool best, int* group_of, int* pages) const {
     std::unordered_map<int, int> by_page;                    // first page -> the first entry that has it
-    std::vector<const std::vector<int>*> tables(S, nullptr);
-    std::vector<int> lead(S, -1), common(S, 0), members(S, 0);
+    std::vector<Prefix> rows(S);
+    std::vector<int> lead(S, -1), common(S, 0), members(S, 0), set_pages;
     for (int i = 0; i < S; ++i) {
-      group_of[i] = -1;
       auto it = requests.find(rids[i]);
       if (it == requests.end()) continue;
-      tables[i] = &it->second.tables[g];
+      const std::vector<int>& table = it->second.tables[g];
       const int full = it->second.num_tokens / page_size;    // (a page that is still being written is nobody else's)
-      if (full < 1 || tables[i]->empty() || (*tables[i])[0] < 0) continue;
-      const int l = by_page.emplace((*tables[i])[0], i).first->second;
+      if (full < 1 || table.empty() || table[0] < 0) continue;
+      rows[i] = {table.data(), std::min(full, (int)table.size())};
+      const int l = by_page.emplace(table[0], i).first->second;
       lead[i] = l;
       ++members[l];
-      int n = std::min(full, (int)tables[i]->size());
-      if (l != i) {
-        n = std::min(n, common[l]);
-        const int* a = tables[l]->data();
-        const int* b = tables[i]->data();
-        if (std::memcmp(a, b, n * sizeof(int)) != 0) {
-          int k = 0;
-          while (a[k] == b[k]) ++k;
-          n = k;
-        }
-      }
-      common[l] = n;
+      common[l] = l == i ? rows[i].full : rows[i].in_common(rows[l], 0, common[l]);
     }
-    int groups = 0;
-    std::vector<int> number(S, -1);
+    std::vector<int> set(S, -1);                             // an entry's set, by the numbers of set_pages
+    for (int l = 0; l < S; ++l) {
+      if (members[l] < 2) continue;
+      const int first = (int)set_pages.size();
+      if (!best || members[l] == 2) set_pages.push_back(common[l]);
+      std::vector<int> own;
+      for (int i = l; i < S; ++i)
+        if (lead[i] == l) {
+          own.push_back(i);
+          set[i] = first;
+        }
+      if (best && members[l] > 2) split_family(rows, std::move(own), common[l], set, set_pages);
+    }
+    int groups = 0;                                          // ... and by their first members
+    std::vector<int> number(set_pages.size(), -1);
     for (int i = 0; i < S; ++i) {
-      if (lead[i] < 0 || members[lead[i]] < 2) continue;
-      if (number[lead[i]] < 0) {
-        pages[groups] = common[lead[i]];
-        number[lead[i]] = groups++;
+      group_of[i] = -1;
+      if (set[i] < 0) continue;
+      int& k = number[set[i]];
+      if (k < 0) {
+        pages[groups] = set_pages[set[i]];
+        k = groups++;
       }
-      group_of[i] = number[lead[i]];
+      group_of[i] = k;
     }
     return groups;
   }
@@ -684,10 +784,10 @@ NVH_API int nvh_manager_num_requests(void* m) { return (int)((CacheManager*)m)->
 NVH_API int nvh_has(void* m, int64_t rid) { return ((CacheManager*)m)->find(rid) ? 1 : 0; }
 NVH_API int nvh_open(void* m, int64_t rid) { return ((CacheManager*)m)->open(rid); }
 NVH_API int nvh_fork(void* m, int64_t parent, int64_t child, int* out) { return ((CacheManager*)m)->fork(parent, child, out); }
-NVH_API int nvh_shared_prefixes(void* m, int S, const int64_t* rids, int g, int* group_of, int* pages) {
+NVH_API int nvh_shared_prefixes(void* m, int S, const int64_t* rids, int g, int best, int* group_of, int* pages) {
   CacheManager* cm = (CacheManager*)m;
   if (g < 0 || g >= (int)cm->pools.size()) return fail(ERR_STATE, "no such cache group");
-  return cm->shared_prefixes(S, rids, g, group_of, pages);
+  return cm->shared_prefixes(S, rids, g, best != 0, group_of, pages);
 }
 NVH_API int nvh_close(void* m, int64_t rid) { return ((CacheManager*)m)->close(rid); }
 NVH_API int nvh_extend(void* m, int64_t rid, int start, int end) { return ((CacheManager*)m)->extend(rid, start, end); }

@@ -420,7 +420,7 @@ class ModelRunner:
         if self._whole_group is None:
             return None
         single = [e.rid for e in entries if len(e.tokens) == 1]
-        groups = self.manager.shared_prefixes(single, self._whole_group)
+        groups = self.manager.shared_prefixes(single, self._whole_group, best=True)
         if not groups:
             return None
         Hkv, D = self._whole_heads

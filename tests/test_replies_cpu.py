@@ -208,3 +208,93 @@ def test_requests_that_are_not_open_share_nothing():
     assert m.shared_prefixes(["nobody", "second", 7, "first"], 0) == [([1, 3], 32)]
     m.close("first")
     assert m.shared_prefixes(["first", "second", "nobody"], 0) == []
+
+
+def least_read(tables, fulls):
+    """What sets save at most, in pages: every way to put the requests into sets is tried."""
+    def common(members):
+        n = min(fulls[i] for i in members)
+        k = 0
+        while k < n and len({tables[i][k] for i in members}) == 1:
+            k += 1
+        return k
+
+    def ways(rest):
+        if not rest:
+            return 0
+        first, others = rest[0], rest[1:]
+        most = ways(others)
+        for mask in range(1, 1 << len(others)):
+            members = [first] + [x for b, x in enumerate(others) if mask >> b & 1]
+            n = common(members)
+            if n:
+                most = max(most, (len(members) - 1) * n + ways([x for b, x in enumerate(others) if not mask >> b & 1]))
+        return most
+    return ways(list(range(len(tables)))), common
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_best_sets_of_forks_against_every_way_to_make_them(seed):
+    rnd = random.Random(seed)
+    m = CacheManager([0], 400, 16, 40)
+    live = []
+    for k in range(rnd.randint(2, 7)):
+        if live and rnd.random() < 0.85:
+            m.fork(rnd.choice(live), k)
+        else:
+            m.open(k)
+        live.append(k)
+        for rid in live:
+            if rnd.random() < 0.5:
+                run(m, rid, rnd.randint(1, 60))
+    rnd.shuffle(live)
+    tables, fulls = [m.get(r).tables[0] for r in live], [m.get(r).num_tokens // 16 for r in live]
+    most, pages_of = least_read(tables, fulls)
+    got = m.shared_prefixes(live, 0, best=True)
+    assert sum((len(members) - 1) * n for members, n in got) == most * 16
+    members = [i for own, _ in got for i in own]
+    assert len(members) == len(set(members)) and all(len(own) > 1 and own == sorted(own) and 0 < n == 16 * pages_of(own) for own, n in got)
+    assert [own[0] for own, _ in got] == sorted(own[0] for own, _ in got)
+
+
+def test_families_behind_one_system_prompt_are_sets_of_their_own():
+    """Eight prompts of 2,064 tokens that begin with the same 64, eight replies each: by first pages one set of 64 with 64 positions."""
+    m = CacheManager([0], 4000, 16, 80)
+    m.open("system")
+    run(m, "system", 64)
+    rids = []
+    for f in range(8):
+        m.fork("system", (f, 0))
+        run(m, (f, 0), 2000)
+        for r in range(1, 8):
+            m.fork((f, 0), (f, r))
+        rids += [(f, r) for r in range(8)]
+    random.Random(1).shuffle(rids)
+    for rid in rids:
+        run(m, rid, 30)
+    assert m.shared_prefixes(rids, 0) == [(list(range(64)), 64)]
+    got = m.shared_prefixes(rids, 0, best=True)
+    assert sorted(n for _, n in got) == [2064] * 8 and all(len({rids[i][0] for i in own}) == 1 and len(own) == 8 for own, _ in got)
+    # requests that part from them early, and a lone one behind the system prompt
+    m.fork("system", "early")
+    run(m, "early", 20)
+    m.fork((3, 0), "late")
+    more = rids + ["early", "late"]
+    got = m.shared_prefixes(more, 0, best=True)
+    assert sorted((len(own), n) for own, n in got) == [(8, 2064)] * 7 + [(9, 2064)] and 64 not in [i for own, _ in got for i in own]
+    # two that have more in common with one another than with their family, which is better off whole
+    run(m, "late", 40)
+    m.fork("late", "later")
+    got = m.shared_prefixes(rids + ["late", "later"], 0, best=True)
+    assert sorted((len(own), n) for own, n in got) == [(8, 2064)] * 7 + [(10, 2064)]
+
+
+def test_best_sets_of_many_requests_that_part_one_after_the_other():
+    m = CacheManager([0], 4000, 16, 300)
+    m.open(0)
+    for k in range(1, 300):
+        run(m, k - 1, 16)
+        m.fork(k - 1, k)
+    got = m.shared_prefixes(list(range(300)), 0, best=True)
+    # request k holds k + 1 pages (the last k): those from a on, with a + 1 pages in common, save (299 - a) (a + 1), more below
+    assert sum((len(own) - 1) * n for own, n in got) >= 16 * 150 * 150 and m.shared_prefixes([], 0, best=True) == []
