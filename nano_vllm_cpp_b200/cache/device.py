@@ -162,9 +162,9 @@ class DeviceCache:
         every layer of their group, and the state slots, a launch per group and per state buffer.  ``stager``: brings the
         index arrays to the device in one copy."""
         from ..csrc import ops
-        if not forks:
-            return
         pages = [[p for f in forks for p in f.pages if p[0] == g] for g in range(len(self.windows))]
+        if not any(pages) and not (forks and self.state_buffers):
+            return
         flat = [x for g in pages for k in (1, 2, 3) for x in [p[k] for p in g]]
         flat += [f.slot_from for f in forks] + [f.slot_to for f in forks]
         at, n = 0, len(flat)

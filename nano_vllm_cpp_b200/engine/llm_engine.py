@@ -12,7 +12,6 @@ from __future__ import annotations
 import os
 from dataclasses import dataclass, field
 
-from ..cache import NoFreePages, NoFreeSlot
 from ..config.engine_config import EngineConfig, MAX_LOGPROBS, SamplingParams
 from ..sampling import Sampler, uniform
 from .batch import StepEntry
@@ -199,14 +198,12 @@ class LLMEngine:
                                            again=again or None, logprobs=max(asked) if asked else None)
         pending = _Pending(scheduled, sampled_seqs, handle, n_prefill, n_decode)
         pending.replies, pending.scored = replies, bool(asked)
-        for seq in parents:                     # the prompt is in the cache, behind what has just been queued
+        for seq in parents:
             seq.forked = True
             self._to_fork.discard(seq.seq_id)
-            for q in seq.replies:
-                try:
-                    self.runner.fork(seq.seq_id, [q.seq_id])
-                except (NoFreePages, NoFreeSlot):
-                    break                       # this reply and the others wait and run the prompt again
+        if parents:                             # the prompts are in the cache, behind what has just been queued
+            # (replies without room for a fork wait and run the prompt again)
+            self.runner.fork_replies([(seq.seq_id, [q.seq_id for q in seq.replies]) for seq in parents])
         return pending
 
     def _stand_ins(self, cur) -> None:

@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from ..cache import CacheManager, DeviceCache
+from ..cache import CacheManager, DeviceCache, NoFreePages, NoFreeSlot
 from ..csrc import ops
 from ..parts.base import RunContext, KVCacheSpec
 from ..weights.loader import load_model
@@ -158,11 +158,25 @@ class ModelRunner:
         """Opens ``new_rids`` with the cache of ``rid`` as it is, so that each goes on from there by itself: full pages are
         shared, part-full ones and recurrent states are copied on the device (behind whatever is queued there).  All of
         them or none: ``NoFreeSlot`` / ``NoFreePages`` leave everything as it was."""
+        self._fork([(rid, new_rids)], some=False)
+
+    def fork_replies(self, families: list) -> None:
+        """``fork`` for every (request, new requests) of ``families``, with the copies of all of them in one launch per cache group
+        and state buffer; where a slot or pages run out, the rest of that family is not opened."""
+        self._fork(families, some=True)
+
+    def _fork(self, families: list, some: bool) -> None:
         forks, opened = [], []
         try:
-            for new in new_rids:
-                forks.append(self.manager.fork(rid, new))
-                opened.append(new)
+            for rid, new_rids in families:
+                for new in new_rids:
+                    try:
+                        forks.append(self.manager.fork(rid, new))
+                    except (NoFreePages, NoFreeSlot):
+                        if some:
+                            break
+                        raise
+                    opened.append(new)
             self.cache.copy_forks(forks, self.stager)
         except BaseException:
             for new in opened:

@@ -29,3 +29,55 @@ def test_families_behind_one_system_prompt_share_their_prompts(graphs, folders, 
         assert float((got - want).abs().max()) <= 2e-2 + 3e-2 * float(want.abs().max())
     assert shared[-1] == ([([0, 4, 8], 112), ([1, 5, 7], 144), ([2, 6, 9], 80)], 10)
     assert bool(runners[0]._graphs) == graphs
+
+
+@pytest.fixture
+def copies(monkeypatch):
+    """How many copies each launch made."""
+    from nano_vllm_cpp_b200.csrc import ops
+    made, inner = [], ops.copy_pages
+    monkeypatch.setattr(ops, "copy_pages", lambda arrays, src, dst, **kw: made.append(src.numel()) or inner(arrays, src, dst, **kw))
+    return made
+
+
+@pytest.mark.parametrize("case,launches", [("A", [9]), ("P", [9, 9])])
+def test_the_forks_of_a_step_are_copied_together(case, launches, folders, copies):
+    """Three prompts that one step completes, four replies each: one launch per cache group and state buffer."""
+    from nano_vllm_cpp_b200 import SamplingParams
+    prompts = [ids_for(case, n, salt=7) for n in (5, 37, 50)]
+    eng = engine(folders[case])
+    outs = eng.generate(prompts, SamplingParams(n=4, temperature=0.9, seed=11, max_tokens=6, ignore_eos=True))
+    assert copies == launches[:1] * len(eng.runner.cache.windows) + launches[1:] * len(eng.runner.cache.state_buffers)
+    for p, o in zip(prompts, outs):
+        for i, reply in enumerate(o["replies"]):
+            alone = eng.generate([p], SamplingParams(temperature=0.9, seed=11 + i, max_tokens=6, ignore_eos=True))
+            assert reply["token_ids"] == alone[0]["token_ids"], (len(p), i)
+    eng.runner.manager.check()
+
+
+def test_prompts_of_whole_pages_copy_nothing(folders, copies):
+    from nano_vllm_cpp_b200 import SamplingParams
+    eng = engine(folders["A"])
+    eng.generate([ids_for("A", 32), ids_for("A", 64)], SamplingParams(n=3, temperature=0.5, seed=1, max_tokens=3, ignore_eos=True))
+    assert copies == []
+
+
+def test_forks_for_which_there_is_room(folders, copies):
+    """A family is opened as far as slots go; nothing stays open where the copies fail."""
+    r = make_runner(folders["A"], "float32", max_requests=5)
+    r.step([entry("a", ids_for("A", 20)), entry("b", ids_for("A", 30))])
+    r.fork_replies([("a", ["a1", "a2"]), ("b", ["b1", "b2", "b3"])])
+    assert copies == [3] and [r.manager.has(x) for x in ("a1", "a2", "b1", "b2", "b3")] == [True, True, True, False, False]
+    r.manager.check()
+    for x in ("a1", "a2", "b1"):
+        r.close(x)
+    free = r.manager.pools[0].num_free()
+
+    def refuse(*a):
+        raise RuntimeError("no copies")
+
+    r.cache.copy_forks = refuse
+    with pytest.raises(RuntimeError, match="no copies"):
+        r.fork_replies([("a", ["a1"]), ("b", ["b1"])])
+    assert r.manager.free_slots() == 3 and r.manager.pools[0].num_free() == free
+    r.manager.check()
