@@ -25,7 +25,7 @@ class StepOutput:
     finished: list                                  # [(seq_id, completion token ids)]
     num_prefill_tokens: int = 0
     num_decode_tokens: int = 0
-    new_tokens: list = field(default_factory=list)  # [(seq_id, token)] for every token drawn this step
+    new_tokens: list = field(default_factory=list)  # [(seq_id, token)] for every token that a sequence got in this step
     logprobs: list = field(default_factory=list)    # [(seq_id, TokenLogprob)] where SamplingParams.logprobs asks for them
 
 
@@ -228,12 +228,14 @@ class LLMEngine:
             sampled = {seq.seq_id: tok for seq, tok in zip(cur.sampled_seqs, tokens)}
             before = [seq.num_tokens for seq in cur.sampled_seqs]
             finished = self.scheduler.postprocess(cur.scheduled, sampled)
-            for seq, n, s in zip(cur.sampled_seqs, before, scores):
-                if seq.num_tokens > n:                           # (else it was preempted after it was scheduled)
+            new = []
+            for seq, n, tok, s in zip(cur.sampled_seqs, before, tokens, scores):
+                if seq.num_tokens > n:                           # (else it was preempted after it was scheduled, or ended a step earlier)
+                    new.append((seq.seq_id, tok))
                     score(seq, s)
             for seq, tok, s in zip(cur.replies, tokens[W:], scores[W:]):
                 seq.token_ids.append(tok)
-                sampled[seq.seq_id] = tok
+                new.append((seq.seq_id, tok))
                 score(seq, s)
                 if (tok == self.config.eos and not seq.ignore_eos) or seq.max_tokens <= 1 or seq.num_tokens >= self.config.max_model_len:
                     if self.runner.manager.has(seq.seq_id):
@@ -245,8 +247,7 @@ class LLMEngine:
                     if seq.nucleus_sampling:
                         self._nucleus_live.add(seq.seq_id)
             self._nucleus_live.difference_update(q.seq_id for q in finished)
-            return StepOutput([(q.seq_id, q.completion_token_ids) for q in finished], cur.n_prefill, cur.n_decode,
-                              list(sampled.items()), told)
+            return StepOutput([(q.seq_id, q.completion_token_ids) for q in finished], cur.n_prefill, cur.n_decode, new, told)
         finished, new = list(cur.finished), []
         for seq, place, tok, s in zip(cur.sampled_seqs, cur.places, tokens, scores):
             if place is None:                                    # preempted meanwhile, or ended a step earlier

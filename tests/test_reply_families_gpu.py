@@ -81,3 +81,28 @@ def test_forks_for_which_there_is_room(folders, copies):
         r.fork_replies([("a", ["a1"]), ("b", ["b1"])])
     assert r.manager.free_slots() == 3 and r.manager.pools[0].num_free() == free
     r.manager.check()
+
+
+@pytest.mark.parametrize("late", [dict(top_p=0.7, temperature=0.9, seed=3), dict(n=2, temperature=0.9, seed=3)])
+def test_told_tokens_are_those_of_the_results(late, folders):
+    """A request ends by its stop token while the step behind is under way, and a request that wants the plain order comes just then:
+    what the steps report as new tokens is what the sequences hold."""
+    from nano_vllm_cpp_b200 import SamplingParams
+    p = ids_for("A", 20, salt=5)
+    stop = engine(folders["A"]).generate([p], SamplingParams(temperature=1.0, seed=3, max_tokens=8, ignore_eos=True))[0]["token_ids"]
+    at = next(i for i in range(3, 8) if stop[i] not in stop[:i])
+    eng = engine(folders["A"], eos=stop[at])
+    for after in range(1, at + 3):
+        told, done = {}, {}
+        first = eng.add_request(p, SamplingParams(temperature=1.0, seed=3, max_tokens=20))
+        eng.add_request(ids_for("A", 30, salt=6), SamplingParams(temperature=0.0, max_tokens=20, ignore_eos=True))
+        steps = 0
+        while not eng.is_finished():
+            out = eng.step()
+            steps += 1
+            for seq_id, token in out.new_tokens:
+                told.setdefault(seq_id, []).append(token)
+            done.update(out.finished)
+            if steps == after:
+                eng.add_request(ids_for("A", 9, salt=7), SamplingParams(max_tokens=6, ignore_eos=True, **late))
+        assert done[first] == stop[:at + 1] and told == done, after
