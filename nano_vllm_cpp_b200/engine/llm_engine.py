@@ -76,7 +76,6 @@ class LLMEngine:
             self._warm_up()
         self._pending = None
         self._nucleus_live = set()      # ids of live requests that are sampled by the nucleus rule
-        self._to_fork = set()           # ids of requests whose further replies wait for their prompt
 
     def _warm_up(self) -> None:
         """The largest step the scheduler can ask for runs once before the first request: what its activations
@@ -137,8 +136,6 @@ class LLMEngine:
         self.scheduler.add(seq)
         if seq.nucleus_sampling:
             self._nucleus_live.add(seq.seq_id)
-        if seq.replies:
-            self._to_fork.add(seq.seq_id)
         return seq.seq_id
 
     # ------------------------------------------------------------------ one step
@@ -158,8 +155,8 @@ class LLMEngine:
         cur, nxt = self._pending, None
         # (a request under the nucleus rule needs its latest tokens on the host for the repetition penalty:
         # while one is live, steps run in the plain order)
-        # (nor from before a prompt whose replies begin with forks of its cache until their first tokens are there)
-        if self.config.run_ahead and not self._nucleus_live and not self._to_fork and not cur.replies:
+        # (and none is decided while the step in flight draws the first tokens of further replies, which join behind it)
+        if self.config.run_ahead and not self._nucleus_live and not cur.replies:
             self._stand_ins(cur)
             nxt = self._launch()
         tokens = self.runner.collect(cur.handle)
@@ -200,7 +197,6 @@ class LLMEngine:
         pending.replies, pending.scored = replies, bool(asked)
         for seq in parents:
             seq.forked = True
-            self._to_fork.discard(seq.seq_id)
         if parents:                             # the prompts are in the cache, behind what has just been queued
             # (replies without room for a fork wait and run the prompt again)
             self.runner.fork_replies([(seq.seq_id, [q.seq_id for q in seq.replies]) for seq in parents])

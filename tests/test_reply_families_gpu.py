@@ -106,3 +106,43 @@ def test_told_tokens_are_those_of_the_results(late, folders):
             if steps == after:
                 eng.add_request(ids_for("A", 9, salt=7), SamplingParams(max_tokens=6, ignore_eos=True, **late))
         assert done[first] == stop[:at + 1] and told == done, after
+
+
+def test_steps_run_ahead_while_prompts_with_replies_wait(folders):
+    """Two requests hold all slots while three prompts with further replies wait: only the steps that complete such a prompt are followed
+    in the plain order.  Every reply is that of a request of its own, and the tokens told step by step are the results'."""
+    from nano_vllm_cpp_b200 import SamplingParams
+    eng = engine(folders["C"], max_num_seqs=2, max_num_batched_tokens=64)
+    counted = dict(ahead=0)
+    inner = eng._stand_ins
+
+    def stand_ins(cur):
+        assert not cur.replies
+        counted["ahead"] += 1
+        inner(cur)
+
+    eng._stand_ins = stand_ins
+    long = [eng.add_request(ids_for("C", n, salt=2), SamplingParams(temperature=0.0, max_tokens=30, ignore_eos=True)) for n in (20, 31)]
+    sps = [SamplingParams(temperature=0.8, seed=4 + 10 * k, n=2 + k % 2, max_tokens=8, ignore_eos=True, logprobs=k % 2 or None) for k in range(3)]
+    prompts = [ids_for("C", n, salt=3) for n in (70, 33, 12)]
+    first = [eng.add_request(p, sp) for p, sp in zip(prompts, sps)]
+    told, done = {}, {}
+    for step in range(29):
+        out = eng.step()
+        done.update(out.finished)
+        for seq_id, token in out.new_tokens:
+            told.setdefault(seq_id, []).append(token)
+    assert counted["ahead"] >= 28
+    while not eng.is_finished():
+        out = eng.step()
+        done.update(out.finished)
+        for seq_id, token in out.new_tokens:
+            told.setdefault(seq_id, []).append(token)
+    assert counted["ahead"] > 28 and told == done and len(done) == 2 + 2 + 3 + 2
+    eng.runner.manager.check()
+    alone = engine(folders["C"])
+    for p, sp, q in zip(prompts, sps, first):
+        for i in range(sp.n):
+            own = SamplingParams(temperature=0.8, seed=sp.seed + i, max_tokens=8, ignore_eos=True)
+            assert done[q + i] == alone.generate([p], own)[0]["token_ids"]
+    assert done[long[0]] == alone.generate([ids_for("C", 20, salt=2)], SamplingParams(temperature=0.0, max_tokens=30, ignore_eos=True))[0]["token_ids"]
