@@ -1061,17 +1061,22 @@ NV_API int nv_attention_shared_splits(int M, int groups, int Hq, int Hkv, int D,
 // room, they run beside it, one block on its multiprocessors and three on the others, 128 keys a split or more, and a second wave
 // would come after it (eight rows of 16 heads behind 2,048: 11.8 us in one wave, 15.3 in two); where it fills the GPU they come
 // after it anyway, 256 keys a split or more unless 128 make one wave (64 rows of 28 heads on 4 behind 8,192, up to 512 of their own:
-// one split 38.5, two 34.1, four 36.2; up to 1,000: 49.1, 39.0, 38.1; four of 16 behind 16,384, up to 200: 33.2, two 31.1).
+// one split 38.5, two 34.1, four 36.2; up to 1,000: 49.1, 39.0, 38.1; four of 16 behind 16,384, up to 200: 33.2, two 31.1).  A block takes
+// eight heads of the own-key kernel, 16 of the split-key kernel (44 rows of 32 heads on 2 behind 1,000, up to 300 of their own: 13.1 in one
+// wave, 18.7 in three splits; 40 rows of 64 heads of 64 on 4 that share nothing, up to 700: 11.4 and 14.8 in two).  Heads of more than 128
+// elements: 384 keys a split at most, whose time is beyond that of a second wave (64 rows of 16 heads of 256 on 1 behind 8,192, up to 512 of
+// their own: one split 44.6, two 37.7; up to 1,000: 59.5, 46.0, three 45.1; 44 behind 1,000, up to 300: 16.3 and 16.0).
 NV_API int nv_attention_shared_own_splits(int R, int M, int groups, int Hq, int Hkv, int D, int page, int cache_dt, int shared_splits,
                                           int most) {
   if (R <= 0 || Hkv <= 0 || most <= 0) return 1;
-  const int G = Hq / Hkv;
-  const long long sms = num_multiprocessors(), blocks = (long long)R * Hkv * ((G + 15) / 16);
+  const int G = Hq / Hkv, heads = tc_takes(cache_dt, D, page) && own_takes(D) ? OW_HEADS : 16;      // of a block
+  const long long sms = num_multiprocessors(), blocks = (long long)R * Hkv * ((G + heads - 1) / heads);
   const long long shared = shared_splits <= 0 ? 0 : shared_tiles(M, groups, Hq, Hkv, tc_takes(cache_dt, D, page) ? ST_PAIRS : SP_PAIRS) * Hkv * shared_splits;
   const long long room = shared <= sms ? shared + (D > 128 ? 2 : 3) * (sms - shared) : 7 * sms;
   long long n = room / blocks;
   const long long least = shared <= sms || blocks * ((most + 127) / 128) <= 3 * sms ? 128 : 256;
   if (n > (most + least - 1) / least) n = (most + least - 1) / least;
+  if (D > 128 && shared > 0 && n < (most + 383) / 384) n = (most + 383) / 384;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
 

@@ -122,3 +122,12 @@ def test_bound_arrays_come_with_what_the_block_tables_must_cover():
     assert shared.reach == 4096
     shared.bind(pack([([2], 5)]))                                           # (not said: the kernels look)
     assert shared.reach == 0
+
+
+def test_own_keys_are_cut_by_the_heads_that_a_block_takes():
+    splits = lambda R, Hq, Hkv, D, ours, most, page=16: ops.lib().nv_attention_shared_own_splits(R, R, 1, Hq, Hkv, D, page, 1, ours, most)
+    assert splits(40, 64, 4, 64, 0, 700) == 1                               # 320 blocks of eight heads, of 444 that live on the GPU
+    assert splits(40, 64, 4, 112, 0, 700) == 2                              # 160 of 16 heads
+    assert splits(44, 32, 2, 128, 4, 300) == 1 and splits(40, 28, 4, 128, 0, 700) == splits(40, 32, 4, 128, 0, 700) == 2
+    # heads of 256: 88 blocks, where 24 of the shared part leave 124 multiprocessors with two each; 128 in what 128 leave, 384 keys a split
+    assert splits(44, 16, 1, 256, 4, 300) == (24 + 2 * 124) // 88 == 3 and splits(64, 16, 1, 256, 16, 512) == 2
