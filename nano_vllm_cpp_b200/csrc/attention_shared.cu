@@ -12,7 +12,7 @@
 // (here).  A row that belongs to no group has no shared part; of a group's keys a row sees those up to its own position.
 //
 // What bounds it (bfloat16, heads of 128): 64 rows of 28 heads on 4 behind 8,192 positions, 16 to 512 of their own, take 34 us (each
-// row by itself: 221), 18 of it the shared part, 10 the rows' own keys, 5 the join of up to 18 parts.  128 rows behind 16,384 take 50
+// row by itself: 221), 18 of it the shared part, 10 the rows' own keys, 5 the join of up to 18 parts.  128 rows behind 16,384 take 51
 // (673), 38 of it the shared part: 64 keys of two blocks of 128 pairs in 1.1 us a multiprocessor, where its exponentials alone take
 // 0.6, the products 0.8 (those of different shapes do not overlap), and the 64 KB of keys and values from L2 0.9.
 #include "tcgen05.cuh"
@@ -1018,6 +1018,8 @@ constexpr int TC_SPLIT_KEYS = 256, PLAIN_SPLIT_KEYS = 64;
 bool tc_takes(int cache_dt, int D, int page) {
   return cache_dt == NV_DT_BF16 && D >= 32 && D % 16 == 0 && (page == 16 || page == 32 || page == 64);
 }
+// (The head sizes of the models here and of the measured range.  Others, such as the 112, 160 and 192 that heads can be padded to, take the
+// split-key kernel.)
 bool own_takes(int D) { return D == 64 || D == 80 || D == 96 || D == 128 || D == 256; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

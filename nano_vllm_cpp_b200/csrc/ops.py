@@ -555,7 +555,7 @@ def attention_decode_shared(qkv, k_cache, v_cache, block_table, row_entry, posit
                             float_weights: bool = False, softcap: float = 0.0, gate=None) -> None:
     """``attention_decode`` for rows of which some share a prefix (``shared``): a group's shared keys and values are read once
     for all its rows, as one product of their query heads, and joined with what each row has of its own, where that pays
-    (``attention_sharing_pays``; else ``attention_decode`` runs, and every row reads its keys itself).  A row sees the
+    (``attention_sharing_pays``; else every row reads its keys itself).  A row sees the
     positions up to its own, none of them masked otherwise (layers with a window, chunks or biases by distance take
     ``attention_decode``).  What lies behind a row's position in its newest page may be anything.  Queries, cache and result have
     one type, ``scale`` is positive.  ``sink_score``, ``float_weights``, ``softcap``, ``gate``: see there.  As there, the kernel

@@ -7,7 +7,8 @@
 // read the older pages of their rows before the kernel in front of them has ended.
 //
 // What bounds it: the bytes.  Four sequences of 128 pages, 48 arrays, 3.2 GB read and written: 481 us, 6.7 TB/s; eight copies of a
-// state of 25 MB (225 MB, most of them written) 46 us, 4.9 TB/s; a fork's part-full pages the latency of four loads in turn.
+// state of 25 MB (225 MB, most of them written) 46 us, 4.9 TB/s; a fork's part-full pages the latency of a launch and two
+// loads in turn (the array's description beside the copy's places, then the source) and a store.
 #include "common.cuh"
 
 namespace {
