@@ -273,11 +273,26 @@ __device__ __forceinline__ void gather_queries(const SharedArgs& a, uint8_t* Qs,
   __syncwarp();
 }
 
-// A score's cap, in base-2 units.  TERMS 3, where the weights keep all their bits: tanhf's tangent, whose error is one of the result; that
-// of capped_log2 is some 2^-22 of the cap, however small the score.  (shared_map has the factor that either takes.)
+// A score's cap, in base-2 units.  capped_log2's error is some 2^-22 of the cap, however small the score.  TERMS 3, where the weights keep
+// all their bits: an error of some units of the result.  Up to half the cap the tangent's series (x^15 is its last term, the next is
+// 2^-27 of the sum; 1.1 units), beyond 1 - 2 / (e^2x + 1), which is no difference of like numbers there (7.5 units at most).  (64 rows of 28 heads on 4 behind 8,192 with a sink
+// and a cap: 54.3 us by capped_log2, 61.9 so, 70.8 by tanhf.)  shared_map has the factor that either takes.
+__device__ __forceinline__ float capped_small(const ScoreMap& map, float s) {
+  const float x = s * map.cap_k, z = x * x;
+  float p = -929569.f / 638512875.f;
+  p = fmaf(p, z, 21844.f / 6081075.f);
+  p = fmaf(p, z, -1382.f / 155925.f);
+  p = fmaf(p, z, 62.f / 2835.f);
+  p = fmaf(p, z, -17.f / 315.f);
+  p = fmaf(p, z, 2.f / 15.f);
+  p = fmaf(p, z, -1.f / 3.f);
+  return map.cap1 * fmaf(x * z, p, x);
+}
 template <int TERMS>
 __device__ __forceinline__ float capped(const ScoreMap& map, float s) {
-  return TERMS > 1 ? map.cap1 * tanhf(s * map.cap_k) : capped_log2(map, s);
+  if (TERMS == 1) return capped_log2(map, s);
+  const float x = s * map.cap_k, e = ex2_fast(fabsf(x) * 2.8853900817779268f);
+  return fabsf(x) <= 0.5f ? capped_small(map, s) : map.cap1 * copysignf(fmaf(-2.f, rcp_fast(e + 1.f), 1.f), x);
 }
 static inline ScoreMap shared_map(float scale, float softcap, int terms) {
   ScoreMap map = score_map(scale, softcap);
@@ -288,11 +303,23 @@ static inline ScoreMap shared_map(float scale, float softcap, int terms) {
 // A pair's next block of scores, from key j on, becomes weights against its reference m; returns the sum of its weights, l among them.
 // The reference follows the maximum only when that has moved by more than 2^8 (weights of up to 256 cost bfloat16 and the float32
 // sums nothing), so that O is rescaled, by alpha, once in a long while.
-template <int TERMS>
+template <int TERMS, bool CAP>
 __device__ __forceinline__ float softmax_step(const ScoreMap& map, float* s, int j, int limit, float& m, float& alpha, float l) {
-  if (map.cap1 > 0.f) {
+  if (CAP && TERMS == 1 && map.cap1 > 0.f) {
 #pragma unroll
     for (int c = 0; c < ST_KEYS; ++c) s[c] = capped<TERMS>(map, s[c]);
+  }
+  if (CAP && TERMS > 1) {
+    float most = 0.f;
+#pragma unroll
+    for (int c = 0; c < ST_KEYS; ++c) most = fmaxf(most, fabsf(s[c]));
+    if (__all_sync(0xffffffffu, most * map.cap_k <= 0.5f)) {
+#pragma unroll
+      for (int c = 0; c < ST_KEYS; ++c) s[c] = capped_small(map, s[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < ST_KEYS; ++c) s[c] = capped<TERMS>(map, s[c]);
+    }
   }
   if (j + ST_KEYS > limit) {
 #pragma unroll
@@ -391,7 +418,8 @@ constexpr int st_tmem_cols() { return 2 * ST_KEYS + D <= 256 ? 256 : 512; }
 template <int D, int TERMS>
 constexpr int st_v_buffers() { return D > 128 && TERMS > 1 ? 1 : 2; }
 
-template <int D, int TERMS>
+// CAP: scores may be capped (TERMS 1) or are (TERMS 3, whose cap has a form of its own: in one with the other it took 2 % of its time).
+template <int D, int TERMS, bool CAP>
 __global__ void __launch_bounds__(ST_THREADS, D <= 128 ? 2 : 1)
 shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, SharedArgs a, ScoreMap map) {
   constexpr int SL = D / 64, VB = st_v_buffers<D, TERMS>();
@@ -580,7 +608,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free);
         if (some) {
-          l = softmax_step<TERMS>(map, s, j0, limit, m, alpha, l);
+          l = softmax_step<TERMS, CAP>(map, s, j0, limit, m, alpha, l);
         }
         // O += P(i-1) V(i-1) must have ended before O is rescaled and P is overwritten (a warp without pairs waits too: its
         // arrival is one for this block)
@@ -978,15 +1006,17 @@ int launch_tc(const SharedArgs& a, int tiles, cudaStream_t s) {
                                  (TERMS > 1 ? (size_t)TERMS * ST_PAIRS * 128 : 0);
   constexpr size_t smem = tiles_bytes + 1024;
   static_assert(tiles_bytes >= (size_t)ST_PAIRS * (D * 4 + 16), "a row of results has its place");
+  constexpr auto capped_kernel = shared_tc_kernel<D, TERMS, true>, plain_kernel = shared_tc_kernel<D, TERMS, TERMS == 1>;
   static bool attr_done = false;
   if (!attr_done) {
-    NV_RETURN_IF(cudaFuncSetAttribute(shared_tc_kernel<D, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    NV_RETURN_IF(cudaFuncSetAttribute(capped_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    NV_RETURN_IF(cudaFuncSetAttribute(plain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr_done = true;
   }
   // scores go to base-2 units by map.in; capped ones are there already
   ScoreMap map = shared_map(a.scale, a.softcap, TERMS);
   if (a.softcap > 0.f) map.in = 1.f;
-  NV_RETURN_IF(launch_dep(shared_tc_kernel<D, TERMS>, dim3(tiles, a.Hkv, a.splits), dim3(ST_THREADS), smem, s, tm_k, tm_v, a, map));
+  NV_RETURN_IF(launch_dep(a.softcap > 0.f ? capped_kernel : plain_kernel, dim3(tiles, a.Hkv, a.splits), dim3(ST_THREADS), smem, s, tm_k, tm_v, a, map));
   NV_RETURN_LAST();
 }
 

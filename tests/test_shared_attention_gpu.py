@@ -163,3 +163,14 @@ def test_a_cap_beside_a_sink_costs_no_bits(Hq, Hkv, D, grouped):
     got = c.run(sink_score=0.5, softcap=1e5, stale=NAN)
     want, weight, score = c.want(sink=0.5, softcap=1e5)
     assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(28, 4, 128), (8, 2, 64), (16, 1, 256)])
+@pytest.mark.parametrize("softcap", [0.5, 2.0, 8.0])
+def test_caps_among_the_scores(Hq, Hkv, D, softcap):
+    """Scores on both sides of half the cap and far beyond it: the cap's function is a series below and an exponential above."""
+    lengths = [301, 44, 17, 333, 37, 300, 90, 100, 131, 1]
+    c = Case(Hq, Hkv, D, lengths, [([3, 0, 5], 300), ([8, 7], 96)], seed=11)
+    got = c.run(sink_score=-0.5, softcap=softcap, stale=NAN)
+    want, weight, score = c.want(sink=-0.5, softcap=softcap)
+    assert bool(((got.double() - want).abs() <= c.tolerance(want, weight, score)).all())
